@@ -10,6 +10,10 @@ model component (mstar/engine/kv_cache_engine.py:132-136); here a page keeps the
 tokens of one head contiguous, so a page of one head is one 16-byte-aligned run
 that bulk copies can move.
 
+With ``kv_cache_dtype`` "float8_e4m3" the pages hold e4m3 codes, half the bytes of bfloat16, and a
+second tensor [pages, planes, kv_heads, page_size] a scale byte for every row
+(``mstar_b200.ops.kv8``).
+
 State slots hold per-request state of fixed size for mixers that ask for it; the
 architecture served here asks for none, so the pool exists with zero bytes.
 """
@@ -22,6 +26,7 @@ import torch
 from ..parts.base import CacheNeed, LayerCache
 from .manager import CacheManager, GroupConfig
 
+KV_CACHE_DTYPES = ("auto", "float8_e4m3")
 _STATE_DTYPES = {"float32": torch.float32, "bfloat16": torch.bfloat16, "int32": torch.int32}
 
 
@@ -50,6 +55,22 @@ def _kv_shape(kv, pages: int, page_size: int) -> tuple:
     return (pages, kv.planes, kv.num_kv_heads, page_size, kv.head_dim)
 
 
+def eight_bit_cache(kv_cache_dtype: Optional[str], needs: Sequence[Optional[CacheNeed]]) -> bool:
+    """Whether ``kv_cache_dtype`` asks for an 8-bit cache ("auto" or None: pages hold the compute
+    type).  Every cache of the model must be able to be one."""
+    if kv_cache_dtype is None or kv_cache_dtype == "auto":
+        return False
+    if kv_cache_dtype not in KV_CACHE_DTYPES:
+        raise ValueError(f"kv_cache_dtype {kv_cache_dtype!r} is not known (one of {', '.join(KV_CACHE_DTYPES)})")
+    kept = [i for i, n in enumerate(needs) if n is not None and n.kv is not None]
+    unable = [i for i in kept if not needs[i].kv.eight_bit]
+    if unable or not kept:
+        raise ValueError(f"kv_cache_dtype {kv_cache_dtype!r} is for models whose every cache holds plain keys and "
+                         "values (rotary or no positions, one head size, no norms, biases or caps on scores); "
+                         + (f"caches {unable} of this one do not" if unable else "this one has none"))
+    return True
+
+
 def group_page_sizes(page_size, num_groups: int) -> list:
     """One page size per group from one int for all, or a sequence with one per group."""
     if isinstance(page_size, int):
@@ -64,23 +85,29 @@ def group_page_sizes(page_size, num_groups: int) -> list:
 
 
 def bytes_per_page(needs: Sequence[CacheNeed], group_of, group: int, page_size: int,
-                   dtype: torch.dtype) -> int:
-    item = torch.empty((), dtype=dtype).element_size()
+                   dtype: torch.dtype, kv_cache_dtype: Optional[str] = None) -> int:
+    eight = eight_bit_cache(kv_cache_dtype, needs)
+    item = 1 if eight else torch.empty((), dtype=dtype).element_size()
     total = 0
     for need, g in zip(needs, group_of):
         if g == group:
             shape = _kv_shape(need.kv, 1, page_size)
             total += item * int(torch.Size(shape).numel())
+            if eight:                           # and a scale byte a row
+                total += int(torch.Size(shape[:4]).numel())
     return total
 
 
 class CacheStorage:
     def __init__(self, needs: Sequence[Optional[CacheNeed]], dtype: torch.dtype,
-                 device: torch.device, page_size, num_pages, num_slots: int):
+                 device: torch.device, page_size, num_pages, num_slots: int,
+                 kv_cache_dtype: Optional[str] = None):
         """``page_size`` and ``num_pages``: one int for every group, or a list with one per
         group (a group of windowed layers may want smaller pages than one that keeps every
-        key: it gives them back sooner)."""
+        key: it gives them back sooner).  ``kv_cache_dtype``: None or "auto" keeps pages in
+        ``dtype``, "float8_e4m3" in 8 bits a number (``mstar_b200.ops.kv8``)."""
         self.needs = list(needs)
+        self.eight_bit = eight_bit_cache(kv_cache_dtype, self.needs)
         self.dtype = dtype
         self.device = device
         self.num_slots = int(num_slots)
@@ -94,16 +121,21 @@ class CacheStorage:
                               for p, n, w in zip(self.page_sizes, num_pages, self.windows)]
         self.manager = CacheManager(self.group_configs, self.num_slots)
         self.kv: list = []
+        self.kv_scales: list = []
         self.state: list = []
         for need, g in zip(self.needs, self.group_of):
             if g is None:
                 self.kv.append(None)
+                self.kv_scales.append(None)
             else:
                 # one page more than the manager hands out: padding entries of
                 # fixed-shape (CUDA graph) batches write their keys there
                 n = self.group_configs[g].num_pages + 1
-                self.kv.append(torch.zeros(_kv_shape(need.kv, n, self.page_sizes[g]), dtype=dtype,
-                                           device=device))
+                shape = _kv_shape(need.kv, n, self.page_sizes[g])
+                pages = torch.zeros(shape, dtype=torch.uint8 if self.eight_bit else dtype, device=device)
+                self.kv.append(pages.view(torch.float8_e4m3fn) if self.eight_bit else pages)
+                self.kv_scales.append(torch.zeros(shape[:4], dtype=torch.uint8, device=device)
+                                      if self.eight_bit else None)
             if need is not None and need.state is not None:
                 self.state.append(torch.zeros((self.num_slots + 1,) + tuple(need.state.shape),
                                               dtype=_STATE_DTYPES[need.state.dtype],
@@ -156,4 +188,4 @@ class CacheStorage:
         return LayerCache(kv=self.kv[cache_id],
                           page_size=0 if g is None else self.page_sizes[g],
                           block_table=None if g is None else block_tables[g],
-                          state=self.state[cache_id])
+                          state=self.state[cache_id], kv_scales=self.kv_scales[cache_id])

@@ -9,7 +9,7 @@ Options keep the reference CLI's names and meanings where it has them
 (mstar/cli/main.py:138-167: positional model, --gpus, --config, --log-level,
 --log-stats, --log-stats-file); the deployment file given with --config carries, as in
 the reference's YAML (docs/serving.rst:161-238), ``max_concurrent_requests``,
-``autocast_dtype`` and a ``kv_cache:`` section with ``page_size`` and ``max_num_pages``.
+``autocast_dtype`` and a ``kv_cache:`` section with ``page_size``, ``max_num_pages`` and ``dtype``.
 Sampling options are the fields of the reference's SamplingConfig
 (mstar/utils/sampling.py:207-226).  ``serve`` (an HTTP server) is not part of this
 engine; prompts are token ids because tokenisation lives in the reference's API server.
@@ -72,7 +72,8 @@ def _generate(args) -> None:
               max_num_batched_tokens=args.max_num_batched_tokens,
               max_concurrent_requests=args.max_concurrent_requests
               or deploy.get("max_concurrent_requests", 64),
-              log_stats=args.log_stats or bool(args.log_stats_file))
+              log_stats=args.log_stats or bool(args.log_stats_file),
+              kv_cache_dtype=args.kv_cache_dtype or kv.get("dtype"))
     d = GenerationDefaults.from_folder(args.model)
 
     def pick(value, default):
@@ -141,6 +142,8 @@ def build_parser() -> argparse.ArgumentParser:
     gen.add_argument("--seed", type=int, default=None)
     gen.add_argument("--page-size", type=int, default=None)
     gen.add_argument("--max-num-pages", type=int, default=None)
+    gen.add_argument("--kv-cache-dtype", default=None, choices=["auto", "float8_e4m3"],
+                     help="type of the cached keys and values (auto: the compute type)")
     gen.add_argument("--max-num-batched-tokens", type=int, default=2048)
     gen.add_argument("--max-concurrent-requests", type=int, default=None)
     gen.add_argument("--log-level", default="INFO",

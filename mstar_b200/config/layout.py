@@ -17,7 +17,7 @@ sizes from a hard-coded dataclass (mstar/model/orpheus/config.py:4-53).
 """
 from __future__ import annotations
 
-from dataclasses import dataclass, field
+from dataclasses import dataclass, field, replace
 from typing import Optional, Sequence
 
 
@@ -140,6 +140,13 @@ class AttentionSpec:
                 and self.q_temp is None and self.softcap is None and self.sink is None
                 and self.chunk is None and self.weights == "softmax" and not self.score_bias
                 and self.value_mix is None)
+
+
+    @property
+    def eight_bit(self) -> bool:
+        """Whether its keys and values can be kept in 8 bits: the plain attention, which may keep
+        first keys beside its window there."""
+        return replace(self, keep_first=0).plain and self.head_dim % 8 == 0 and self.head_dim <= 256
 
 
 @dataclass(frozen=True)

@@ -52,19 +52,22 @@ class LLM:
                  kv_cache_memory_fraction: float = 0.85,
                  max_num_batched_tokens: int = 2048,
                  max_concurrent_requests: Optional[int] = 64, max_batch_size: int = 64,
-                 log_stats: bool = False):
+                 log_stats: bool = False, kv_cache_dtype: Optional[str] = None):
         """``model``: a folder with config.json and safetensors, or a built ``Model``.
         ``page_size`` and ``max_num_pages``: tokens per page and pages of a cache group, one
         number for all groups or a list with one per group; ``max_num_pages`` None sizes the
-        pools from ``kv_cache_memory_fraction`` of the memory free after loading."""
+        pools from ``kv_cache_memory_fraction`` of the memory free after loading.
+        ``kv_cache_dtype``: None or "auto" keeps keys and values in the compute type, "float8_e4m3"
+        in 8 bits a number with a scale a row: half the bytes of bfloat16, for models whose layers
+        all have the plain attention."""
         self.model: Model = model if isinstance(model, Model) else load_model(
             model, dtype=dtype, device=device)
         self.device = self.model.runtime.device
         slots = max_concurrent_requests or max_batch_size
         if max_num_pages is None:
-            max_num_pages = self._pages_from_memory(page_size, kv_cache_memory_fraction)
+            max_num_pages = self._pages_from_memory(page_size, kv_cache_memory_fraction, kv_cache_dtype)
         storage = CacheStorage(self.model.cache_needs, self.model.runtime.dtype, self.device,
-                               page_size, max_num_pages, slots)
+                               page_size, max_num_pages, slots, kv_cache_dtype)
         self.stepper = Stepper(self.model, storage)
         self.sampler = Sampler(self.model.vocab_size, slots, self.device)
         cfg = self.model.config
@@ -93,7 +96,7 @@ class LLM:
         self._turn = 0
         self._copy_stream = torch.cuda.Stream(device=self.device)
 
-    def _pages_from_memory(self, page_size, fraction: float) -> list:
+    def _pages_from_memory(self, page_size, fraction: float, kv_cache_dtype: Optional[str] = None) -> list:
         free, _ = torch.cuda.mem_get_info(self.device)
         free = max(free - self.model.workspace_bytes(), 0)
         windows, group_of = plan_groups(self.model.cache_needs)
@@ -104,7 +107,7 @@ class LLM:
         pages = []
         for g in range(len(windows)):
             b = bytes_per_page(self.model.cache_needs, group_of, g, sizes[g],
-                               self.model.runtime.dtype)
+                               self.model.runtime.dtype, kv_cache_dtype)
             pages.append(max(per_group // max(b, 1), 1))
         return pages
 

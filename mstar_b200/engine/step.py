@@ -342,10 +342,11 @@ class Stepper:
 
 def make_stepper(model: Model, *, page_size=16, num_pages=None,
                  max_tokens: Optional[int] = None, num_slots: int = 64,
-                 cuda_graphs: bool = True) -> Stepper:
+                 cuda_graphs: bool = True, kv_cache_dtype: Optional[str] = None) -> Stepper:
     """A stepper with a cache pool of ``num_pages`` pages per group, or enough pages
     for ``max_tokens`` cached tokens.  ``page_size`` and ``num_pages``: one number for
-    every cache group, or a list with one per group."""
+    every cache group, or a list with one per group.  ``kv_cache_dtype``: None or "auto" (pages
+    hold the compute type) or "float8_e4m3"."""
     if num_pages is None:
         if max_tokens is None:
             raise ValueError("give num_pages or max_tokens")
@@ -354,5 +355,5 @@ def make_stepper(model: Model, *, page_size=16, num_pages=None,
         if isinstance(page_size, int):
             num_pages = num_pages[0]
     storage = CacheStorage(model.cache_needs, model.runtime.dtype, model.runtime.device,
-                           page_size, num_pages, num_slots)
+                           page_size, num_pages, num_slots, kv_cache_dtype)
     return Stepper(model, storage, cuda_graphs=cuda_graphs)

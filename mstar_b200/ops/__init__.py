@@ -2389,3 +2389,8 @@ def linear_scan(r, k, v, decay, direct, ctx, state: torch.Tensor, offset: int, h
     if piece:
         lib.add_launches(2)                     # three kernels behind one call
     return out
+
+
+# the 8-bit key/value cache (its module uses the helpers above)
+from .kv8 import (KV8_DTYPE, kv8_read_rows, kv8_splits, kv8_supported, paged_decode_attention_kv8,  # noqa: E402
+                  paged_prefill_attention_kv8, rope_kv8_write)

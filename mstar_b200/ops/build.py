@@ -52,6 +52,8 @@ LIBRARIES = {
     "hyper": ("cuda", ["hyper.cu"], []),
     "side_by_side": ("cuda", ["side_by_side.cu"], []),
     "linear_recurrence": ("cuda", ["linear_recurrence.cu"], []),
+    "kv8_cache": ("cuda", ["kv8_cache.cu"], []),
+    "attention_kv8": ("cuda", ["attention_kv8.cu"], []),
     "host": ("host", ["host/cache_manager.cpp"], []),
 }
 

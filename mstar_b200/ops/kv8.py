@@ -1,0 +1,228 @@
+"""The 8-bit key/value cache: rows quantised as they are written, rows read back, and the attention
+of single tokens and of prompt portions over its pages.
+
+A cached row (the key or the value of one token and kv head) is held as e4m3 codes and one byte s
+that stands for 2^(s - 127), the smallest power of two with which the row's largest number is at
+most 448 codes' units (held in [2^-100, 2^119]).  Codes are rounded to nearest even; reading a row
+back rounds nothing, in bfloat16 as in float.  A row with a number that is not finite is held as
+NaNs (byte 255), and a query that sees its key or value gives NaNs.
+
+The cache of a layer is two tensors: ``kv_cache`` torch.float8_e4m3fn [pages, 2, kv_heads,
+page_size, head_dim] and ``kv_scales`` torch.uint8 [pages, 2, kv_heads, page_size].  Block tables
+and index arrays are those of the other paged kernels; a token writes nothing where its table has
+no page.  Tensors must lie on the current device; launches go to its current stream.
+
+The reference's caches hold the compute type only (mstar/engine/kv_cache_engine.py:132-136).
+"""
+from __future__ import annotations
+
+import torch
+
+from . import _DT, _dt, _need_cuda, _ptr, _stream, lib, num_sms
+from .lib import KernelError, check
+
+KV8_DTYPE = torch.float8_e4m3fn
+_INT = torch.int32
+
+
+def kv8_supported(head_dim: int) -> bool:
+    """Whether a head size can be held in 8 bits by these kernels."""
+    return head_dim % 8 == 0 and 0 < head_dim <= 256
+
+
+def _refuse(what: str, why: str) -> None:
+    raise KernelError(f"{what}: {why}")
+
+
+def _check_cache(what, kv_cache, kv_scales, num_kv_heads, page_size, head_dim) -> None:
+    shape = kv_cache.shape
+    if kv_cache.dtype != KV8_DTYPE or kv_scales.dtype != torch.uint8:
+        _refuse(what, f"the cache holds {KV8_DTYPE} codes and uint8 scales, got {kv_cache.dtype} and {kv_scales.dtype}")
+    if len(shape) != 5 or shape[0] < 1 or shape[1:] != (2, num_kv_heads, page_size, head_dim):
+        _refuse(what, f"the cache's shape {tuple(shape)} is not (pages, 2, {num_kv_heads}, {page_size}, {head_dim})")
+    if kv_scales.shape != shape[:4]:
+        _refuse(what, f"the scales' shape {tuple(kv_scales.shape)} is not the cache's {tuple(shape[:4])}")
+    if not (kv_cache.is_contiguous() and kv_scales.is_contiguous()):
+        _refuse(what, "the cache and its scales must be contiguous")
+    if not kv8_supported(head_dim):
+        _refuse(what, f"head_dim {head_dim} is not a multiple of 8 up to 256")
+
+
+def _check_index(what, block_table, *arrays) -> None:
+    """``arrays``: (tensor, least number of elements)."""
+    if block_table.dtype != _INT or block_table.dim() != 2 or block_table.stride(1) != 1:
+        _refuse(what, "the block table is int32 [entries, pages], its rows without gaps")
+    for t, n in arrays:
+        if t.dtype != _INT or t.dim() != 1 or t.shape[0] < n or (n > 1 and t.stride(0) != 1):
+            _refuse(what, f"index arrays are int32 [at least {n}], got {t.dtype} {tuple(t.shape)}")
+
+
+def _check_device(what, first, *others) -> None:
+    _need_cuda(first, *others)
+    device = first.get_device()
+    for t in others:
+        if t is not None and t.get_device() != device:
+            _refuse(what, "its tensors lie on different devices")
+    if device != torch._C._cuda_getDevice():
+        _refuse(what, f"its tensors lie on cuda:{device}, which is not the current device")
+
+
+def rope_kv8_write(qkv: torch.Tensor, positions, cache_pos, token_req, block_table, inv_freq, kv_cache: torch.Tensor,
+                   kv_scales: torch.Tensor, num_heads: int, num_kv_heads: int, head_dim: int, rotary_dim: int,
+                   interleaved: bool, page_size: int) -> torch.Tensor:
+    """Rotate queries and keys of ``qkv`` [tokens, (num_heads + 2 num_kv_heads) * head_dim], quantise keys
+    and values into their pages, and return the rotated queries [tokens, num_heads * head_dim] in a
+    tensor of their own (``qkv`` stays as it is).  ``inv_freq``: float [rotary_dim / 2], or None when
+    rotary_dim == 0.  Two tokens of a call that name the same place of a request leave either's row."""
+    what = "rope_kv8_write"
+    _dt(qkv)
+    if qkv.dim() != 2 or qkv.shape[1] != (num_heads + 2 * num_kv_heads) * head_dim or qkv.stride(1) != 1:
+        _refuse(what, f"qkv {tuple(qkv.shape)} is not [tokens, ({num_heads} + 2 * {num_kv_heads}) * {head_dim}] "
+                      "with rows without gaps")
+    if num_heads < 1 or num_kv_heads < 1:
+        _refuse(what, "there is at least one query head and one kv head")
+    if rotary_dim % 2 or not 0 <= rotary_dim <= head_dim:
+        _refuse(what, f"rotary_dim {rotary_dim} is not even and in [0, head_dim={head_dim}]")
+    _check_cache(what, kv_cache, kv_scales, num_kv_heads, page_size, head_dim)
+    if rotary_dim and (inv_freq is None or inv_freq.dtype != torch.float32 or inv_freq.numel() != rotary_dim // 2
+                       or not inv_freq.is_contiguous()):
+        _refuse(what, f"inv_freq is float32 [{rotary_dim // 2}]")
+    n = qkv.shape[0]
+    _check_index(what, block_table, (positions, n), (cache_pos, n), (token_req, n))
+    _check_device(what, qkv, positions, cache_pos, token_req, block_table, inv_freq if rotary_dim else None, kv_cache,
+                  kv_scales)
+    q = qkv.new_empty((n, num_heads * head_dim))
+    if n == 0:
+        return q
+    code = lib.get("kv8_cache").mstar_rope_kv8_write(
+        qkv.data_ptr(), _DT[qkv.dtype], qkv.stride(0), q.data_ptr(), positions.data_ptr(), cache_pos.data_ptr(),
+        token_req.data_ptr(), block_table.data_ptr(), block_table.stride(0), _ptr(inv_freq if rotary_dim else None),
+        kv_cache.data_ptr(), kv_scales.data_ptr(), kv_cache.shape[0], n, num_heads, num_kv_heads, head_dim, rotary_dim,
+        int(interleaved), page_size, _stream())
+    check(code, what)
+    return q
+
+
+def kv8_read_rows(kv_cache: torch.Tensor, kv_scales: torch.Tensor, block_table, token_req, cache_pos,
+                  dtype: torch.dtype) -> torch.Tensor:
+    """The cached rows of the given tokens as numbers, [tokens, 2, kv_heads, head_dim] (keys, then values) of
+    ``dtype``: exactly what the cache holds.  Token t is place ``cache_pos[t]`` of request
+    ``token_req[t]``; a place whose page the table does not have gives zeros."""
+    what = "kv8_read_rows"
+    if dtype not in _DT:
+        _refuse(what, f"rows are read as float32 or bfloat16, not {dtype}")
+    if kv_cache.dim() != 5:
+        _refuse(what, f"the cache's shape {tuple(kv_cache.shape)} is not (pages, 2, kv_heads, page_size, head_dim)")
+    pages, _, heads, page_size, head_dim = kv_cache.shape
+    _check_cache(what, kv_cache, kv_scales, heads, page_size, head_dim)
+    n = token_req.shape[0]
+    _check_index(what, block_table, (token_req, n), (cache_pos, n))
+    _check_device(what, kv_cache, kv_scales, block_table, token_req, cache_pos)
+    out = torch.empty((n, 2, heads, head_dim), dtype=dtype, device=kv_cache.device)
+    if n:
+        code = lib.get("kv8_cache").mstar_kv8_read_rows(
+            kv_cache.data_ptr(), kv_scales.data_ptr(), block_table.data_ptr(), block_table.stride(0),
+            token_req.data_ptr(), cache_pos.data_ptr(), out.data_ptr(), _DT[dtype], n, heads, head_dim, pages,
+            page_size, _stream())
+        check(code, what)
+    return out
+
+
+def _check_attention(what, q, out, rows, num_heads, num_kv_heads, head_dim, window, keep_first, scale) -> None:
+    width = num_heads * head_dim
+    _dt(q)
+    if num_kv_heads < 1 or num_heads < 1 or num_heads % num_kv_heads:
+        _refuse(what, f"{num_heads} query heads are no multiple of {num_kv_heads} kv heads")
+    if q.dim() != 2 or q.shape[0] < rows or q.shape[1] < width or q.stride(1) != 1:
+        _refuse(what, f"q {tuple(q.shape)} is not [at least {rows}, at least {width}] with rows without gaps")
+    if out.dtype != q.dtype or out.dim() != 2 or out.shape[0] < rows or out.shape[1] != width or not out.is_contiguous():
+        _refuse(what, f"out is contiguous {q.dtype} [at least {rows}, {width}], got {out.dtype} {tuple(out.shape)}")
+    if window < 0 or keep_first < 0:
+        _refuse(what, f"window {window} and keep_first {keep_first} are not negative")
+    if not scale > 0.0:
+        _refuse(what, f"the scale {scale} is not positive")
+
+
+def kv8_splits(blocks: int, max_keys: int, sms: int) -> int:
+    """Parts that the keys of ``blocks`` row tiles are cut into: two blocks an SM, parts of at least 128
+    keys, at most 64."""
+    return max(1, min(64, -(-2 * sms // max(blocks, 1)), -(-max_keys // 128)))
+
+
+def _parts(q, tokens, num_heads, head_dim, splits) -> tuple:
+    """(the tensor, addresses of the outputs' and of the statistics' parts)."""
+    if splits == 1:
+        return None, 0, 0
+    rows = tokens * num_heads * splits
+    t = q.new_empty(rows * (head_dim + 2), dtype=torch.float32)
+    return t, t.data_ptr(), t.data_ptr() + 4 * rows * head_dim
+
+
+def _float_attention(what, q, out, kv_cache, kv_scales, block_table, indptr, kv_len, req, pos, first_entry, count, max_q,
+                     max_keys, num_heads, num_kv_heads, head_dim, page_size, window, keep_first, scale) -> None:
+    """The kernel that takes every shape: portions by (indptr, kv_len), single tokens by (req, pos)."""
+    rows = max_q * (num_heads // num_kv_heads)
+    tiles = 1 if rows <= 8 else -(-rows // 64)
+    splits = kv8_splits(tiles * num_kv_heads * count, max_keys, num_sms(q.device))
+    tokens = min(out.shape[0], count * max_q)
+    part, part_o, part_ml = _parts(q, tokens, num_heads, head_dim, splits)
+    check(lib.get("attention_kv8").mstar_kv8_attention(
+        q.data_ptr(), q.stride(0), out.data_ptr(), _DT[q.dtype], kv_cache.data_ptr(), kv_scales.data_ptr(),
+        kv_cache.shape[0], block_table.data_ptr(), block_table.stride(0), _ptr(indptr), _ptr(kv_len), _ptr(req), _ptr(pos),
+        first_entry, count, max_q, tokens, num_heads, num_kv_heads, head_dim, page_size, window, keep_first, scale,
+        splits, part_o, part_ml, _stream()), what)
+    if splits > 1:
+        lib.add_launches(1)                     # the kernel that joins the parts
+
+
+def _most_keys(max_len, max_q, window, keep_first) -> int:
+    """A bound on the keys that a row tile walks."""
+    return max(1, min(max_len, window + max_q - 1 + keep_first) if window else max_len)
+
+
+def paged_decode_attention_kv8(q: torch.Tensor, out: torch.Tensor, kv_cache: torch.Tensor, kv_scales: torch.Tensor,
+                               block_table, token_req, cache_pos, tokens: int, num_heads: int, num_kv_heads: int,
+                               head_dim: int, page_size: int, window: int, keep_first: int, scale: float,
+                               max_len: int) -> None:
+    """Attention of ``tokens`` single-query rows (row i of q, out, token_req and cache_pos) over an 8-bit
+    cache: the token at place p of its request sees the keys up to p; with ``window`` W > 0 the keys
+    p - W + 1 .. p and those below ``keep_first``.  q [tokens, at least num_heads * head_dim], out
+    contiguous [tokens, num_heads * head_dim], both float32 or bfloat16; ``max_len`` bounds the keys of any
+    request (it decides how the work is cut, not what is computed).  A token at a place below 0 gives
+    zeros."""
+    what = "paged_decode_attention_kv8"
+    _check_attention(what, q, out, tokens, num_heads, num_kv_heads, head_dim, window, keep_first, scale)
+    _check_cache(what, kv_cache, kv_scales, num_kv_heads, page_size, head_dim)
+    _check_index(what, block_table, (token_req, tokens), (cache_pos, tokens))
+    _check_device(what, q, out, kv_cache, kv_scales, block_table, token_req, cache_pos)
+    if tokens <= 0:
+        return
+    _float_attention(what, q, out, kv_cache, kv_scales, block_table, None, None, token_req, cache_pos, 0, tokens, 1,
+                     _most_keys(max_len, 1, window, keep_first), num_heads, num_kv_heads, head_dim, page_size, window,
+                     keep_first, scale)
+
+
+def paged_prefill_attention_kv8(q: torch.Tensor, out: torch.Tensor, kv_cache: torch.Tensor, kv_scales: torch.Tensor,
+                                block_table, qo_indptr, kv_len, first_entry: int, entries: int, max_q_len: int,
+                                num_heads: int, num_kv_heads: int, head_dim: int, page_size: int, window: int,
+                                keep_first: int, scale: float, max_kv_len: int) -> None:
+    """Attention of the new tokens of batch entries [first_entry, first_entry + entries) over an 8-bit
+    cache; q and out hold all tokens of the step, entry e's are [qo_indptr[e], qo_indptr[e + 1]) and the
+    last of its ``kv_len[e]`` keys (the mask is causal and aligned to the end; window and keep_first as in
+    ``paged_decode_attention_kv8``).  ``max_q_len`` bounds the new tokens of these entries, ``max_kv_len``
+    their keys.  Rows of other entries are left as they are."""
+    what = "paged_prefill_attention_kv8"
+    _check_attention(what, q, out, 0, num_heads, num_kv_heads, head_dim, window, keep_first, scale)
+    _check_cache(what, kv_cache, kv_scales, num_kv_heads, page_size, head_dim)
+    if first_entry < 0 or q.shape[0] < out.shape[0]:
+        _refuse(what, "first_entry is not negative, and q has a row for every row of out")
+    last = first_entry + max(entries, 0)
+    if block_table.shape[0] < last:
+        _refuse(what, f"the block table has {block_table.shape[0]} rows and {last} entries are named")
+    _check_index(what, block_table, (qo_indptr, last + 1), (kv_len, last))
+    _check_device(what, q, out, kv_cache, kv_scales, block_table, qo_indptr, kv_len)
+    if entries <= 0 or max_q_len <= 0 or out.shape[0] == 0:
+        return
+    _float_attention(what, q, out, kv_cache, kv_scales, block_table, qo_indptr, kv_len, None, None, first_entry, entries,
+                     max_q_len, _most_keys(max_kv_len, max_q_len, window, keep_first), num_heads, num_kv_heads, head_dim,
+                     page_size, window, keep_first, scale)

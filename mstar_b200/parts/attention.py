@@ -25,6 +25,10 @@ number a head, or zero), a sigmoid gate a feature on the heads' outputs, an RMS 
 without a weight, values blended with those of an earlier layer of the same step, a mask of chunks
 instead of a window (the cache then keeps as many keys as a chunk is long), a learned number
 a head added to the scores, and weights that are sigmoids of the scores instead of a softmax.
+
+A plain layer, with or without kept first keys, may keep its cache in 8 bits (``LayerCache.kv_scales``):
+the fused product, a kernel that rotates, quantises and fills the pages, and attention kernels that
+read the codes, for single tokens and for portions.
 """
 from __future__ import annotations
 
@@ -84,7 +88,7 @@ class Attention:
                                    window=spec.chunk or spec.window, keep_first=spec.keep_first if spec.window
                                    else 0,
                                    v_head_dim=None if spec.value_dim == spec.head_dim
-                                   else spec.value_dim), state=state)
+                                   else spec.value_dim, eight_bit=spec.eight_bit), state=state)
 
     def __init__(self, spec, params: dict, runtime: Runtime):
         if spec.num_heads % spec.num_kv_heads:
@@ -158,6 +162,8 @@ class Attention:
 
     def forward(self, x, ctx: StepContext, cache: LayerCache):
         s = self.spec
+        if cache.kv_scales is not None:
+            return self._forward_kv8(x, ctx, cache)
         if not s.plain:
             return self._forward_general(x, ctx, cache)
         write_heads = 0 if s.shares_kv else s.num_kv_heads
@@ -172,6 +178,27 @@ class Attention:
                                 cache.page_size, s.num_heads, write_heads)
         out = qkv.new_empty((ctx.num_tokens, s.num_heads * s.head_dim))
         self.attend(qkv, out, ctx, cache)
+        return ops.linear(out, self.w_out, static_weights=True)
+
+    def _forward_kv8(self, x, ctx: StepContext, cache: LayerCache):
+        s = self.spec
+        q = ops.linear(x, self.w_in, static_weights=True)
+        if s.shares_kv:
+            self.position.apply(q, ctx, None, cache.block_table, cache.page_size, s.num_heads, 0)
+        else:
+            q = self.position.apply_kv8(q, ctx, cache.kv, cache.kv_scales, cache.block_table, cache.page_size,
+                                        s.num_heads, s.num_kv_heads)
+        out = q.new_empty((ctx.num_tokens, s.num_heads * s.head_dim))
+        window, keep, nd = s.window or 0, s.keep_first if s.window else 0, ctx.num_decode
+        if nd:
+            ops.paged_decode_attention_kv8(
+                q, out, cache.kv, cache.kv_scales, cache.block_table, ctx.token_req, ctx.cache_pos, nd, s.num_heads,
+                s.num_kv_heads, s.head_dim, cache.page_size, window, keep, self.scale, max(ctx.kv_lens[:nd]))
+        if ctx.num_entries > nd:
+            ops.paged_prefill_attention_kv8(
+                q, out, cache.kv, cache.kv_scales, cache.block_table, ctx.qo_indptr, ctx.kv_len, nd,
+                ctx.num_entries - nd, max(ctx.q_lens[nd:]), s.num_heads, s.num_kv_heads, s.head_dim, cache.page_size,
+                window, keep, self.scale, max(ctx.kv_lens[nd:]))
         return ops.linear(out, self.w_out, static_weights=True)
 
     def _forward_general(self, x, ctx: StepContext, cache: LayerCache):

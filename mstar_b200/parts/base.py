@@ -16,7 +16,8 @@ class KVNeed:
     them.  ``planes``: 2 for keys and values, 1 for a mixer that keeps one row per token (a
     latent that both are made from).  ``v_head_dim``: not None and other than ``head_dim``
     makes a page [num_kv_heads, page_size, head_dim] keys followed by [num_kv_heads,
-    page_size, v_head_dim] values, and the cache tensor [pages, elements of a page]."""
+    page_size, v_head_dim] values, and the cache tensor [pages, elements of a page].
+    ``eight_bit``: the mixer can keep these rows in 8 bits (``LayerCache.kv_scales``)."""
 
     num_kv_heads: int
     head_dim: int
@@ -24,6 +25,7 @@ class KVNeed:
     planes: int = 2
     keep_first: int = 0
     v_head_dim: Optional[int] = None
+    eight_bit: bool = False
 
 
 @dataclass(frozen=True)
@@ -93,6 +95,8 @@ class LayerCache:
     kv: Optional[torch.Tensor] = None           # [pages, planes, kv_heads, page_size, head_dim]
     page_size: int = 0
     block_table: Optional[torch.Tensor] = None  # int32 [entries, width] of the cache's group
+    # uint8 [pages, planes, kv_heads, page_size]: the rows' scales where ``kv`` holds 8-bit codes
+    kv_scales: Optional[torch.Tensor] = None
     state: Optional[torch.Tensor] = None        # [slots, *shape]
 
 

@@ -74,6 +74,13 @@ class RotaryEncoding:
                           self.inv_freq, kv_cache, num_heads, num_kv_heads, self.spec.head_dim,
                           self.spec.rotary_dim, self.spec.interleaved, page_size)
 
+    def apply_kv8(self, qkv, ctx, kv_cache, kv_scales, block_table, page_size, num_heads, num_kv_heads):
+        """The same over an 8-bit cache; returns the rotated queries, a tensor of their own."""
+        s = self.spec
+        return ops.rope_kv8_write(qkv, ctx.positions, ctx.cache_pos, ctx.token_req, block_table, self.inv_freq,
+                                  kv_cache, kv_scales, num_heads, num_kv_heads, s.head_dim, s.rotary_dim,
+                                  s.interleaved, page_size)
+
     def project_and_apply(self, x, w_qkv, ctx, kv_cache, block_table, page_size, num_heads,
                           num_kv_heads):
         """Optional entry of a position part: the mixer's first product together with
@@ -102,6 +109,10 @@ class NoPositionEncoding:
         ops.rope_kv_write(qkv, ctx.positions, ctx.cache_pos, ctx.token_req, block_table, None,
                           kv_cache, num_heads, num_kv_heads, self.spec.head_dim, 0, False,
                           page_size)
+
+    def apply_kv8(self, qkv, ctx, kv_cache, kv_scales, block_table, page_size, num_heads, num_kv_heads):
+        return ops.rope_kv8_write(qkv, ctx.positions, ctx.cache_pos, ctx.token_req, block_table, None, kv_cache,
+                                  kv_scales, num_heads, num_kv_heads, self.spec.head_dim, 0, False, page_size)
 
 
 register_part("position", "rope", RotaryEncoding)
