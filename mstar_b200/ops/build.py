@@ -54,6 +54,7 @@ LIBRARIES = {
     "linear_recurrence": ("cuda", ["linear_recurrence.cu"], []),
     "kv8_cache": ("cuda", ["kv8_cache.cu"], []),
     "attention_kv8": ("cuda", ["attention_kv8.cu"], []),
+    "attention_kv8_decode": ("cuda", ["attention_kv8_decode.cu"], []),
     "host": ("host", ["host/cache_manager.cpp"], []),
 }
 
