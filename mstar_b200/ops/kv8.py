@@ -18,7 +18,7 @@ from __future__ import annotations
 
 import torch
 
-from . import _DT, _dt, _need_cuda, _ptr, _stream, lib, num_sms
+from . import _DT, _dt, _error_ptr, _need_cuda, _ptr, _stream, lib, num_sms
 from .lib import KernelError, check
 
 KV8_DTYPE = torch.float8_e4m3fn
@@ -178,16 +178,20 @@ def _float_attention(what, q, out, kv_cache, kv_scales, block_table, indptr, kv_
 KV8_DECODE_HEAD_DIMS = (64, 128, 256)
 
 
+def _rows_fit(kv_cache) -> bool:
+    """Whether the cache's rows can be counted in 31 bits, as the copies by TMA count them."""
+    return kv_cache.numel() // kv_cache.shape[4] < 2 ** 31
+
+
 def kv8_decode_shape(pairs: int, max_keys: int, head_dim: int, sms: int) -> tuple:
-    """(blocks of a cluster, warps of a block) that share the keys of each of ``pairs`` (token, kv head,
-    8 query heads) in the decode kernel: enough warps for twelve an SM, none without a step of keys."""
-    keys, most = (32, 12) if head_dim <= 128 else (16, 8)
-    want = max(1, min(-(-max_keys // keys), -(-12 * sms // max(pairs, 1))))
-    warps = 4 if want <= 64 else 8 if want <= 128 else most
+    """(blocks of a cluster, warps of a block, tiles of a warp's ring) that share the keys of each of
+    ``pairs`` (token, kv head, 8 query heads) in the decode kernel."""
+    want = max(1, min(-(-max_keys // 32), -(-8 * sms // max(pairs, 1))))
+    warps = 4 if want <= 64 else 8
     blocks = 1
     while blocks < 16 and blocks * warps < want:
         blocks *= 2
-    return blocks, warps
+    return blocks, warps, 3 if head_dim <= 128 else 2
 
 
 def _most_keys(max_len, max_q, window, keep_first) -> int:
@@ -212,15 +216,16 @@ def paged_decode_attention_kv8(q: torch.Tensor, out: torch.Tensor, kv_cache: tor
     _check_device(what, q, out, kv_cache, kv_scales, block_table, token_req, cache_pos)
     if tokens <= 0:
         return
-    if (q.dtype == torch.bfloat16 and head_dim in KV8_DECODE_HEAD_DIMS and q.stride(0) % 8 == 0
-            and q.data_ptr() % 16 == 0):
+    if (q.dtype == torch.bfloat16 and head_dim in KV8_DECODE_HEAD_DIMS and page_size % 8 == 0
+            and q.stride(0) % 8 == 0 and (q.data_ptr() | kv_cache.data_ptr()) % 16 == 0 and _rows_fit(kv_cache)):
         most = _most_keys(max_len, 1, window, keep_first)
         pairs = tokens * num_kv_heads * -(-num_heads // num_kv_heads // 8)
-        blocks, warps = kv8_decode_shape(pairs, most, head_dim, num_sms(q.device))
+        blocks, warps, stages = kv8_decode_shape(pairs, most, head_dim, num_sms(q.device))
         check(lib.get("attention_kv8_decode").mstar_kv8_decode(
             q.data_ptr(), q.stride(0), out.data_ptr(), kv_cache.data_ptr(), kv_scales.data_ptr(), kv_cache.shape[0],
             block_table.data_ptr(), block_table.stride(0), token_req.data_ptr(), cache_pos.data_ptr(), tokens, num_heads,
-            num_kv_heads, head_dim, page_size, window, keep_first, scale, blocks, warps, _stream()), what)
+            num_kv_heads, head_dim, page_size, window, keep_first, scale, blocks, warps, stages, _error_ptr(q),
+            _stream()), what)
         return
     _float_attention(what, q, out, kv_cache, kv_scales, block_table, None, None, token_req, cache_pos, 0, tokens, 1,
                      _most_keys(max_len, 1, window, keep_first), num_heads, num_kv_heads, head_dim, page_size, window,
