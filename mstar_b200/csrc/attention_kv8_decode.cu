@@ -3,10 +3,11 @@
 //
 // The work is the cache's bytes: a token reads each of its keys and values once for up to 8 query heads, some 4 flops
 // a byte and head.  So the kernel is built around having copies in flight: every warp has a ring of tiles of 32 keys
-// of its own in shared memory, filled by TMA (boxes of 8 or 16 rows of a page) with the tiles after the one it works
-// on, and no warp waits for another before the end.  (Loads into registers did not do: what is loaded a step ahead is
-// waited for where the registers are handed on, 52 us instead of 20 for 64 requests with a window of 1,024.)  The
-// products run on the tensor cores with the keys as rows, since 16 rows of queries would be mostly padding:
+// of its own in shared memory, filled by asynchronous copies of 16 bytes a thread with the tiles after the one it works
+// on, and no warp waits for another before the end.  (TMA boxes of a page's rows took some 700 clocks a tile to issue
+// from one thread and 800 from several, against 350: 18.0 us for one token on 16,384 keys where these take 15.7.  Loads
+// into registers a step ahead are waited for where the registers are handed on: 52 us for 64 requests with a window of
+// 1,024 keys against 18.6.)  The products run on the tensor cores with the keys as rows, since 16 rows of queries would be mostly padding:
 //   S^T [16 keys x 8 heads] += K [16 x 16] Q^T [16 x 8],   O^T [16 features x 8 heads] += V^T [16 x 16 keys] P^T.
 // Which feature or key a fragment's element stands for is free as long as both operands agree.  So a thread's operands
 // are runs of 16 bytes of a row: of K the features [16 t, 16 t + 16) and every 64 after them, of V [D/8 g, D/8 (g + 1))
@@ -14,22 +15,32 @@
 // eight neighbouring lanes read into different banks of the swizzled tiles.  V's pairs of keys are put together by byte
 // permutes, P^T comes from S^T by a matrix transpose between registers (movmatrix).
 //
-// e4m3 is exact in float16, so both products take float16: the queries are scaled by a power of two a head (their
-// largest number into [1, 2); what falls below float16's range is 2^-25 of that), the weights lie in [0, 1].  The
-// rows' scales are put on the scores: a key's by a product, and a value's as an addend of the exponent, since 2^s_j *
-// 2^e_j v_j = 2^(s_j + e_j) v_j.  The weights of the values' product are therefore 2^(s_j + e_j - m') with a maximum m'
-// of their own, so that they use float16's range whatever the values' scales are; the normaliser's are 2^(s_j - m).
+// The scores' product takes the keys' codes as they are (e4m3 x e4m3).  A query is its largest number's power of two
+// times two codes, x = hi + lo / 32: the first rounding leaves 2^-4 of a number, the second 2^-22 of the head's largest
+// (a bfloat16 has 8 bits, which two codes hold but for numbers 2^-10 below the largest).  That costs a second product,
+// which takes 4.6 clocks where the float16 one with half the depth takes 8 and its operands' conversion as long; with up
+// to 4 query heads a kv head there is none: hi and lo are columns 0 - 3 and 4 - 7 of one product, and the threads that
+// would have idle columns take half of the keys of the softmax.
+//
+// Of the values' product the weights are float16, in which e4m3 is exact, so the codes are converted.  The rows' scales
+// are put on the scores: a key's by a product, and a value's as an addend of the exponent, since 2^s_j * 2^e_j v_j =
+// 2^(s_j + e_j) v_j.  The weights are therefore 2^(s_j + e_j - m') with a maximum m' of their own, so that they use
+// float16's range whatever the values' scales are; the normaliser's are 2^(s_j - m).  Both maxima follow the scores only
+// when these exceed them by more than 2^8, which a vote of the warp finds: exchanging the maxima at every tile costs as
+// much as its exponentials.
 //
 // The tiles of a (token, kv head) are dealt out in turn to the warps of a cluster of blocks, so that the lengths that
 // are there decide the balance, not the bounds a launch was sized for.  The warps of a block are joined in shared
-// memory, the blocks through distributed shared memory: one launch, no scratch memory, sums in a fixed order.
+// memory; the blocks send what each other block is to join into its shared memory (stores that nobody waits for, then
+// one barrier; reading it from there took 4,100 clocks, a wait for every block in turn): one launch, no scratch
+// memory, sums in a fixed order.
 //
-// Semantics are those of attention_generic.cu.  Waits are bounded; one that runs out sets the error word to 30.
+// Semantics are those of attention_generic.cu.
 #include <cooperative_groups.h>
 #include <cuda_fp16.h>
 
 #include "kv8.cuh"
-#include "tma_util.cuh"
+#include "mma_util.cuh"
 
 namespace cg = cooperative_groups;
 
@@ -41,8 +52,6 @@ struct Kv8DecodeArgs {
     int q_stride, bt_stride, pages, nq, nkv, window, keep_first, head_groups;
     float scale_log2e;
     PageSplit page;
-    int box, stages;        // rows of a copy (8 or 16), tiles of a warp's ring
-    int* error_word;
 };
 
 __device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t two) {
@@ -62,6 +71,13 @@ __device__ __forceinline__ void mma_f16_16816(float (&c)[4], uint32_t a0, uint32
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ void mma_e4m3_16832(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                               uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
 __device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
     uint32_t r;
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
@@ -76,102 +92,56 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
     const __half2 v = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&v);
 }
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
 // 2^(a - b) for maxima that may still be -inf (of a part without keys: 0)
 __device__ __forceinline__ float ratio(float a, float b) { return a == -INFINITY ? 0.f : ex2(a - b); }
 
 #define DEC8_KEYS 32     // keys of a tile
-// Shared memory of a warp: `stages` tiles of keys and of values (blocks of [32 rows x at most 128 bytes], swizzled),
-// then a scale pair a key, then the barriers; the outputs that the warps leave at the end lie over the tiles.
+#define DEC8_STAGES 3    // tiles of a warp's ring
+#define DEC8_SLACK 8.f   // how far (in powers of two) scores may exceed the maxima
+// Shared memory of a warp: tiles of keys and of values (blocks of [32 rows x at most 128 bytes], swizzled), then a scale
+// pair a key, then each tile's scale bytes; the outputs that the warps leave at the end lie over the tiles.
 template <int D> __host__ __device__ constexpr int dec8_tile() { return DEC8_KEYS * D; }
-template <int D> __host__ __device__ constexpr int dec8_stage() { return 2 * dec8_tile<D>(); }
-template <int D> __host__ __device__ constexpr int dec8_ring(int stages) { return stages * (dec8_stage<D>() + DEC8_KEYS * 8 + 8); }
-template <int D> __host__ __device__ constexpr int dec8_smem(int warps, int stages) {
-    return 1024 + warps * dec8_ring<D>(stages) + (32 + warps * 32) * 4;
+template <int D> __host__ __device__ constexpr int dec8_stage() { return 2 * dec8_tile<D>() + 2 * DEC8_KEYS; }
+template <int D> __host__ __device__ constexpr int dec8_ring() { return DEC8_STAGES * dec8_stage<D>() + DEC8_KEYS * 8; }
+// Of a block: the warps' statistics, the blocks' statistics [16][H][4], and a place for the parts of all blocks of what
+// this block joins, [C][H][D / C].
+template <int D> __host__ __device__ constexpr int dec8_smem(int warps) {
+    return warps * dec8_ring<D>() + (warps * 32 + 16 * 32 + 8 * D) * 4;
 }
+template <int D> __host__ __device__ constexpr int dec8_most_warps() { return D == 64 ? 16 : D == 128 ? 8 : 4; }
 
-template <int D> __host__ __device__ constexpr int dec8_most_warps() { return D == 64 ? 16 : D == 128 ? 12 : 8; }
-
-template <int D>
-__global__ void __launch_bounds__(32 * dec8_most_warps<D>(), 1) kv8_decode_kernel(const __grid_constant__ CUtensorMap map, Kv8DecodeArgs a) {
+// H: query heads of a block, 4 or 8
+template <int D, int H>
+__global__ void __launch_bounds__(32 * dec8_most_warps<D>(), 1)
+kv8_decode_kernel(Kv8DecodeArgs a) {
     constexpr int KC = D / 64;             // 16-byte runs of a key row a thread takes
     constexpr int VW = D / 32;             // 4-byte words of a value row a thread takes
     constexpr int MT = D / 16;             // blocks of 16 features
     constexpr int RB = D < 128 ? D : 128;  // bytes of a row in a block of the tile
-    constexpr int NB = D / RB;             // blocks of a tile
-    extern __shared__ unsigned char smem_dyn[];
-    unsigned char* smem8 = smem_dyn + ((1024u - (tc_smem(smem_dyn) & 1023u)) & 1023u);   // the swizzle's alignment
+    constexpr int S = DEC8_STAGES;
+    constexpr int E = H == 4 ? 1 : 2;      // keys of every 16 whose weights a thread makes, for two heads each
+    extern __shared__ __align__(1024) unsigned char smem8[];
+    const int W = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    // the tiles of all warps lie first, then the rest, so that the tiles keep their alignment
+    unsigned char* ring = smem8 + (size_t)warp * S * 2 * dec8_tile<D>();
+    float2* sc = reinterpret_cast<float2*>(smem8 + (size_t)W * S * 2 * dec8_tile<D>()) + warp * DEC8_KEYS;
+    unsigned char* bytes_s = smem8 + (size_t)W * (S * 2 * dec8_tile<D>() + DEC8_KEYS * 8) + warp * S * 2 * DEC8_KEYS;
+    cluster_arrive();                       // (everybody has started before anybody's memory is written)
     pdl_wait();
     cg::cluster_group cluster = cg::this_cluster();
-    const int W = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int C = cluster.num_blocks(), rank = cluster.block_rank(), S = a.stages;
+    const int C = cluster.num_blocks(), rank = cluster.block_rank();
     const int pair = blockIdx.x / C, token = blockIdx.y;
-    const int kvh = pair / a.head_groups, h0 = (pair % a.head_groups) * 8, G = a.nq / a.nkv, heads = min(8, G - h0);
     const int pos = a.cache_pos[token];
     const int* bt = a.block_table + (size_t)a.token_req[token] * a.bt_stride;
+    const int kvh = pair / a.head_groups, h0 = (pair % a.head_groups) * H, G = a.nq / a.nkv, heads = min(H, G - h0);
 
-    // the tiles: those of the kept first keys that lie before the window's first tile, then the window's
-    const int lo = a.window > 0 ? max(0, pos - a.window + 1) : 0, first = lo / DEC8_KEYS;
-    const int kept = min((min(a.keep_first, lo) + DEC8_KEYS - 1) / DEC8_KEYS, first);
-    const int tiles = pos < 0 ? 0 : kept + pos / DEC8_KEYS - first + 1, stride = C * W;
-    auto key0_of = [&](int i) { return (i < kept ? i : i - kept + first) * DEC8_KEYS; };
-
-    unsigned char* ring = smem8 + (size_t)warp * S * dec8_stage<D>();
-    float2* sc_s = reinterpret_cast<float2*>(smem8 + (size_t)W * S * dec8_stage<D>()) + warp * S * DEC8_KEYS;
-    const uint32_t full = tc_smem(smem8 + (size_t)W * S * (dec8_stage<D>() + DEC8_KEYS * 8)) + warp * S * 8;
-    if (lane < S) mbar_init(full + 8 * lane, 1);
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    __syncwarp();
-
-    // the row (of the cache as a matrix of D bytes a row) of this lane's key of a tile.  What lies past the table or on
-    // pages that are not there is brought into the cache and masked.
-    auto row_of = [&](int i) -> uint32_t {
-        const int key = key0_of(i) + lane, logical = page_of(a.page, key);
-        return ((uint32_t)page_id(bt, logical, a.bt_stride, a.pages) * 2 * a.nkv + kvh) * a.page.size +
-               (uint32_t)(key - logical * a.page.size);
-    };
-    const uint32_t plane = (uint32_t)a.nkv * a.page.size;
-    auto copy_tile = [&](int slot, uint32_t row) {
-        if (lane == 0) mbar_expect_tx(full + 8 * slot, dec8_stage<D>());
-        __syncwarp();
-        if ((lane & (a.box - 1)) == 0) {
-            const uint32_t dst = tc_smem(ring + (size_t)slot * dec8_stage<D>()) + lane * RB;
-#pragma unroll
-            for (int b = 0; b < NB; ++b) {
-                tma_load_2d(dst + b * DEC8_KEYS * RB, &map, full + 8 * slot, b * RB, (int)row);
-                tma_load_2d(dst + dec8_tile<D>() + b * DEC8_KEYS * RB, &map, full + 8 * slot, b * RB, (int)(row + plane));
-            }
-        }
-    };
-    // the scale bytes of a key and of its value, and what the softmax makes of them: 2^e and e; NaN for a bad row
-    auto load_scales = [&](uint32_t row) -> uint32_t {
-        return (uint32_t)a.scales[row] | ((uint32_t)a.scales[(size_t)row + plane] << 8);
-    };
-    auto keep_scales = [&](int slot, uint32_t two) {
-        const int ks = two & 255, vs = two >> 8;
-        const bool bad = ks == KV8_BAD_BYTE || vs == KV8_BAD_BYTE;
-        sc_s[slot * DEC8_KEYS + lane] = make_float2(bad ? __int_as_float(0x7fc00000) : kv8_scale(ks), (float)(vs - 127));
-    };
-
-    // the ring's first tiles; from then on the tile S turns ahead is copied when its place is free, its table entry
-    // being read a turn before that and its scales put into place a turn after
-    const int i0 = rank * W + warp;
-    uint32_t row = 0, pending = 0;
-    for (int s = 0; s < S; ++s)
-        if (i0 + s * stride < tiles) {
-            row = row_of(i0 + s * stride);
-            copy_tile(s, row);
-            keep_scales(s, load_scales(row));
-        }
-    if (i0 + S * stride < tiles) row = row_of(i0 + S * stride);
-
-    // queries: head g, the features this thread's part of K has
-    uint32_t qf[4 * KC][2];
-    float head_scale;
+    // this thread's part of a query (head g, with H = 4 head g % 4): the features that its part of K has
+    uint32_t raw[KC][8];
+    const int qh = H == 4 ? g & 3 : g;
     {
-        const bool there = g < heads;
-        const bf16* q = a.q + (size_t)token * a.q_stride + (size_t)(kvh * G + h0 + (there ? g : 0)) * D;
-        float most = 0.f;
-        uint32_t raw[KC][8];
+        const bf16* q = a.q + (size_t)token * a.q_stride + (size_t)(kvh * G + h0 + (qh < heads ? qh : 0)) * D;
 #pragma unroll
         for (int c = 0; c < KC; ++c)
 #pragma unroll
@@ -179,33 +149,104 @@ __global__ void __launch_bounds__(32 * dec8_most_warps<D>(), 1) kv8_decode_kerne
                 const uint4 w = *reinterpret_cast<const uint4*>(q + c * 64 + t * 16 + i * 8);
                 raw[c][4 * i] = w.x; raw[c][4 * i + 1] = w.y; raw[c][4 * i + 2] = w.z; raw[c][4 * i + 3] = w.w;
             }
+    }
+
+    // the tiles: those of the kept first keys that lie before the window's first tile, then the window's
+    const int lo = a.window > 0 ? max(0, pos - a.window + 1) : 0, first = lo / DEC8_KEYS;
+    const int kept = min((min(a.keep_first, lo) + DEC8_KEYS - 1) / DEC8_KEYS, first);
+    const int tiles = pos < 0 ? 0 : kept + pos / DEC8_KEYS - first + 1, stride = C * W;
+    auto key0_of = [&](int i) { return (i < kept ? i : i - kept + first) * DEC8_KEYS; };
+    // The row (of the cache as a matrix of D bytes a row) of this lane's key of a tile, from the table's entry for it.
+    // What lies past the table or on pages that are not there is brought into the cache and masked.  (Two steps: a warp
+    // issues in order, and would stand still at the first use of an entry just asked for.)
+    auto entry_of = [&](int i) -> int { return bt[min(page_of(a.page, key0_of(i) + lane), a.bt_stride - 1)]; };
+    auto row_of = [&](int i, int entry) -> uint32_t {
+        const int key = key0_of(i) + lane, page = (int)min((unsigned)entry, (unsigned)(a.pages - 1));
+        return ((uint32_t)page * 2 * a.nkv + kvh) * a.page.size + (uint32_t)(key - page_of(a.page, key) * a.page.size);
+    };
+    const uint32_t plane = (uint32_t)a.nkv * a.page.size;
+    // where a 16-byte run c of row r lies in a block of the tile: the swizzle of 128- or 64-byte rows
+    auto at = [](int r, int c) { return r * RB + ((RB == 128 ? c ^ (r & 7) : c ^ ((r >> 1) & 3)) << 4); };
+    // starts the copies of a tile; `row`: of this lane's key.  Groups of 8 keys lie in one page, their scale bytes side
+    // by side.  Always one group of copies, so that they can be counted.
+    auto copy_tile = [&](int slot, uint32_t row, bool there) {
+        if (there) {
+            constexpr int CPR = D / 16, RPI = 32 / CPR;       // 16-byte runs of a row, rows of a warp's copy
+            const uint32_t dst = smem_u32(ring) + slot * 2 * dec8_tile<D>();
+            const int run = lane % CPR;
+            // (all rows first: copies keep their order, and an exchange between two of them would be waited for)
+            const uint8_t* src[DEC8_KEYS / RPI];
+#pragma unroll
+            for (int k = 0; k < DEC8_KEYS / RPI; ++k)
+                src[k] = a.codes + (size_t)__shfl_sync(0xffffffffu, row, k * RPI + lane / CPR) * D + run * 16;
+#pragma unroll
+            for (int k = 0; k < DEC8_KEYS / RPI; ++k) {
+                const uint32_t to = dst + (run >> 3) * (DEC8_KEYS * RB) + at(k * RPI + lane / CPR, run & 7);
+                cp_async_16(to, src[k], 16);
+                cp_async_16(to + dec8_tile<D>(), src[k] + (size_t)plane * D, 16);
+            }
+            if ((lane & 7) == 0) {
+                const uint32_t to = smem_u32(bytes_s) + slot * 2 * DEC8_KEYS + lane;
+                cp_async_8(to, a.scales + row);
+                cp_async_8(to + DEC8_KEYS, a.scales + (size_t)row + plane);
+            }
+        }
+        cp_async_commit();
+    };
+
+    // the table's entries of the ring's first tiles; they come while the queries are made ready
+    const int i0 = rank * W + warp;
+    int entry = 0, entries[S];
+#pragma unroll
+    for (int s = 0; s < S; ++s) entries[s] = i0 + s * stride < tiles ? entry_of(i0 + s * stride) : 0;
+    if (i0 + S * stride < tiles) entry = entry_of(i0 + S * stride);
+
+    // the query's codes: hi and lo (with H = 4 in the threads of g < 4 and of g >= 4)
+    uint32_t qf[H == 4 ? 1 : 2][4 * KC];
+    float head_scale;
+    {
+        float most = 0.f;
 #pragma unroll
         for (int c = 0; c < KC; ++c)
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                if (!there) raw[c][i] = 0u;
+                if (qh >= heads) raw[c][i] = 0u;
                 const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw[c][i]));
-                most = fmaxf(most, fmaxf(fabsf(f.x), fabsf(f.y)));
+                most = fabsf(f.x) < INFINITY && fabsf(f.y) < INFINITY ? fmaxf(most, fmaxf(fabsf(f.x), fabsf(f.y))) : INFINITY;
             }
         most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
         most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
-        // the largest number's exponent, nothing where it has none (0, subnormal, not finite) or no inverse
-        const uint32_t e = __float_as_uint(most) >> 23;
-        const bool plain = e == 0 || e >= 254;
-        const float down = plain ? 1.f : __uint_as_float((254u - e) << 23);
-        head_scale = (plain ? 1.f : __uint_as_float(e << 23)) * a.scale_log2e;
+        // the largest number into [128, 256); a query that is not finite gives NaNs
+        const uint32_t e = max(__float_as_uint(most) >> 23, 8u);
+        const float down = e < 255u ? __uint_as_float((261u - e) << 23) : 1.f;
+        head_scale = e < 255u ? __uint_as_float((e - 7u) << 23) * a.scale_log2e : __int_as_float(0x7fc00000);
 #pragma unroll
         for (int c = 0; c < KC; ++c)
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw[c][2 * i + j]));
-                    qf[c * 4 + i][j] = pack_f16(f.x * down, f.y * down);
+            for (int i = 0; i < 4; ++i) {
+                const float2 x = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw[c][2 * i]));
+                const float2 y = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw[c][2 * i + 1]));
+                const float v[4] = {x.x * down, x.y * down, y.x * down, y.y * down};
+                const uint32_t hi = kv8_pack4(v[0], v[1], v[2], v[3]);
+                float r[4];
+                kv8_unpack4(hi, r);
+                const uint32_t rest = kv8_pack4((v[0] - r[0]) * 32.f, (v[1] - r[1]) * 32.f, (v[2] - r[2]) * 32.f, (v[3] - r[3]) * 32.f);
+                if constexpr (H == 4) {
+                    qf[0][4 * c + i] = g < 4 ? hi : rest;
+                } else {
+                    qf[0][4 * c + i] = hi;
+                    qf[H == 4 ? 0 : 1][4 * c + i] = rest;
                 }
+            }
     }
-    // of the two heads whose scores this thread has
-    const float hs0 = __shfl_sync(0xffffffffu, head_scale, 8 * t), hs1 = __shfl_sync(0xffffffffu, head_scale, 8 * t + 4);
+    // of the two heads whose scores this thread has: 2t, 2t + 1, with H = 4 2 (t % 2) and the next
+    const int th = H == 4 ? t & 1 : t;
+    const float hs0 = __shfl_sync(0xffffffffu, head_scale, 8 * th), hs1 = __shfl_sync(0xffffffffu, head_scale, 8 * th + 4);
+
+    // the ring's first tiles; from then on the tile S turns ahead is copied when its place is free, its table entry
+    // having been read a turn before
+#pragma unroll
+    for (int s = 0; s < S; ++s) copy_tile(s, row_of(i0 + s * stride, entries[s]), i0 + s * stride < tiles);
 
     float o[MT][4];
 #pragma unroll
@@ -214,46 +255,79 @@ __global__ void __launch_bounds__(32 * dec8_most_warps<D>(), 1) kv8_decode_kerne
 
     // a product's row g is key kg of its 8 (and kg + 8); a product's key 2t is key 2t, its key 2t + 1 is (2t + 1) ^ 4
     const int kg = (g & 1) ? g ^ 4 : g, kt = (2 * t + 1) ^ 4;
-    // where a 16-byte run c of row r lies in a block of the tile: the swizzle of 128- or 64-byte rows
-    auto at = [](int r, int c) { return r * RB + ((RB == 128 ? c ^ (r & 7) : c ^ ((r >> 1) & 3)) << 4); };
+    const int kmine = kg + (H == 4 && t >= 2 ? 8 : 0);        // the first key of 16 whose weights this thread makes
     int slot = 0;
-    uint32_t parity = 0;
-    int i = i0;
-    for (; i < tiles; i += stride) {
-        if (!__all_sync(0xffffffffu, mbar_wait(full + 8 * slot, parity))) {
-            if (lane == 0) atomicExch(a.error_word, 30);
-            break;
-        }
-        const unsigned char* kt_s = ring + (size_t)slot * dec8_stage<D>();
+    for (int i = i0; i < tiles; i += stride) {
+        cp_async_wait<S - 1>();
+        __syncwarp();
+        const unsigned char* kt_s = ring + slot * 2 * dec8_tile<D>();
         const unsigned char* vt_s = kt_s + dec8_tile<D>();
-        const float2* sc = sc_s + slot * DEC8_KEYS;
+        // a lane makes its key's scales ready: 2^e of the key (NaN for a bad row) and e of the value
+        {
+            const int ks = bytes_s[slot * 2 * DEC8_KEYS + lane], vs = bytes_s[(slot * 2 + 1) * DEC8_KEYS + lane];
+            const bool bad = ks == KV8_BAD_BYTE || vs == KV8_BAD_BYTE;
+            sc[lane] = make_float2(bad ? __int_as_float(0x7fc00000) : kv8_scale(ks), (float)(vs - 127));
+        }
         const int key0 = key0_of(i);
-        // ---- scores
-        float s[2][4];
+        // ---- scores: s[u][2k + h] of the thread's k-th key of 16 and its h-th head
+        float s[2][2 * E];
+        {
+            // (sums of hi and of lo products; all products before the exchanges, which would wait for theirs in turn)
+            float x[2][4], y[2][4];
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            s[u][0] = s[u][1] = s[u][2] = s[u][3] = 0.f;
+            for (int u = 0; u < 2; ++u)
 #pragma unroll
-            for (int c = 0; c < KC; ++c) {
-                const unsigned char* blk = kt_s + (c >> 1) * (DEC8_KEYS * RB);
-                const uint4 x = *reinterpret_cast<const uint4*>(blk + at(16 * u + kg, t + 4 * (c & 1)));
-                const uint4 y = *reinterpret_cast<const uint4*>(blk + at(16 * u + kg + 8, t + 4 * (c & 1)));
-                const uint32_t lo4[4] = {x.x, x.y, x.z, x.w}, hi4[4] = {y.x, y.y, y.z, y.w};
+                for (int k = 0; k < 4; ++k) x[u][k] = y[u][k] = 0.f;
 #pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    mma_f16_16816(s[u], e4m3x2_to_f16x2(lo4[k]), e4m3x2_to_f16x2(hi4[k]), e4m3x2_hi_to_f16x2(lo4[k]),
-                                  e4m3x2_hi_to_f16x2(hi4[k]), qf[c * 4 + k][0], qf[c * 4 + k][1]);
+            for (int c = 0; c < KC; ++c)
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const unsigned char* blk = kt_s + (c >> 1) * (DEC8_KEYS * RB);
+                    const uint4 ka = *reinterpret_cast<const uint4*>(blk + at(16 * u + kg, t + 4 * (c & 1)));
+                    const uint4 kb = *reinterpret_cast<const uint4*>(blk + at(16 * u + kg + 8, t + 4 * (c & 1)));
+                    if constexpr (H == 4) {
+                        mma_e4m3_16832(x[u], ka.x, kb.x, ka.y, kb.y, qf[0][4 * c], qf[0][4 * c + 1]);
+                        mma_e4m3_16832(y[u], ka.z, kb.z, ka.w, kb.w, qf[0][4 * c + 2], qf[0][4 * c + 3]);
+                    } else {
+                        mma_e4m3_16832(x[u], ka.x, kb.x, ka.y, kb.y, qf[0][4 * c], qf[0][4 * c + 1]);
+                        mma_e4m3_16832(y[u], ka.x, kb.x, ka.y, kb.y, qf[1][4 * c], qf[1][4 * c + 1]);
+                        mma_e4m3_16832(x[u], ka.z, kb.z, ka.w, kb.w, qf[0][4 * c + 2], qf[0][4 * c + 3]);
+                        mma_e4m3_16832(y[u], ka.z, kb.z, ka.w, kb.w, qf[1][4 * c + 2], qf[1][4 * c + 3]);
+                    }
+                }
+            if constexpr (H == 4) {
+                // threads of t < 2 have the hi sums, the others the lo sums; the former keep key kg, the latter kg + 8
+                float got[2][2];
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) x[u][k] += y[u][k];
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) got[u][h] = __shfl_xor_sync(0xffffffffu, t < 2 ? x[u][2 + h] : x[u][h], 2);
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+                        s[u][h] = t < 2 ? fmaf(got[u][h], 0.03125f, x[u][h]) : fmaf(x[u][2 + h], 0.03125f, got[u][h]);
+            } else {
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) s[u][k] = fmaf(y[u][k], 0.03125f, x[u][k]);
             }
         }
-        // ---- weights; this thread has keys kg, kg + 8 of every 16 and heads 2t, 2t + 1
+        // ---- weights
+        __syncwarp();
         const bool whole = key0 >= lo && key0 + DEC8_KEYS - 1 <= pos;
-        float p[2][4];                       // exponents of the values' weights
+        float p[2][2 * E];                   // exponents of the values' weights
         float x0 = -INFINITY, x1 = -INFINITY, y0 = -INFINITY, y1 = -INFINITY;
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                const int j = 16 * u + 8 * k + kg;
+            for (int k = 0; k < E; ++k) {
+                const int j = 16 * u + 8 * k + kmine;
                 const float2 f = sc[j];
                 float b0 = s[u][2 * k] * f.x * hs0, b1 = s[u][2 * k + 1] * f.x * hs1;
                 if (!whole) {
@@ -269,19 +343,20 @@ __global__ void __launch_bounds__(32 * dec8_most_warps<D>(), 1) kv8_decode_kerne
                 y0 = fmaxf(y0, b0 + f.y);
                 y1 = fmaxf(y1, b1 + f.y);
             }
-#pragma unroll
-        for (int d = 4; d < 32; d <<= 1) {
-            x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, d));
-            x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, d));
-            y0 = fmaxf(y0, __shfl_xor_sync(0xffffffffu, y0, d));
-            y1 = fmaxf(y1, __shfl_xor_sync(0xffffffffu, y1, d));
-        }
         // (a maximum is -inf only where every score so far is NaN or -inf: the sums are NaN or zero then)
-        x0 = fmaxf(m0, x0);
-        x1 = fmaxf(m1, x1);
-        y0 = fmaxf(w0, y0);
-        y1 = fmaxf(w1, y1);
-        if (__any_sync(0xffffffffu, (x0 != m0) | (x1 != m1) | (y0 != w0) | (y1 != w1))) {
+        if (__any_sync(0xffffffffu, (x0 > m0 + DEC8_SLACK) | (x1 > m1 + DEC8_SLACK) | (y0 > w0 + DEC8_SLACK) |
+                                        (y1 > w1 + DEC8_SLACK))) {
+#pragma unroll
+            for (int d = H == 4 ? 2 : 4; d < 32; d <<= 1) {
+                x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, d));
+                x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, d));
+                y0 = fmaxf(y0, __shfl_xor_sync(0xffffffffu, y0, d));
+                y1 = fmaxf(y1, __shfl_xor_sync(0xffffffffu, y1, d));
+            }
+            x0 = fmaxf(m0, x0);
+            x1 = fmaxf(m1, x1);
+            y0 = fmaxf(w0, y0);
+            y1 = fmaxf(w1, y1);
             l0 *= ratio(m0, x0);
             l1 *= ratio(m1, x1);
             const float r0 = ratio(w0, y0), r1 = ratio(w1, y1);
@@ -292,22 +367,36 @@ __global__ void __launch_bounds__(32 * dec8_most_warps<D>(), 1) kv8_decode_kerne
                 o[k][2] *= r0;
                 o[k][3] *= r1;
             }
+            m0 = x0;
+            m1 = x1;
+            w0 = y0;
+            w1 = y1;
         }
-        m0 = x0;
-        m1 = x1;
-        w0 = y0;
-        w1 = y1;
-        const float z0 = x0 == -INFINITY ? 0.f : x0, z1 = x1 == -INFINITY ? 0.f : x1;
-        const float q0 = y0 == -INFINITY ? 0.f : y0, q1 = y1 == -INFINITY ? 0.f : y1;
+        const float z0 = m0 == -INFINITY ? 0.f : m0, z1 = m1 == -INFINITY ? 0.f : m1;
+        const float q0 = w0 == -INFINITY ? 0.f : w0, q1 = w1 == -INFINITY ? 0.f : w1;
         uint32_t pf[2][2];
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
+            for (int k = 0; k < E; ++k) {
                 l0 += ex2(s[u][2 * k] - z0);
                 l1 += ex2(s[u][2 * k + 1] - z1);
-                pf[u][k] = transpose_8x8(pack_f16(ex2(p[u][2 * k] - q0), ex2(p[u][2 * k + 1] - q1)));
+                pf[u][k] = pack_f16(ex2(p[u][2 * k] - q0), ex2(p[u][2 * k + 1] - q1));
             }
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int k = 0; k < E; ++k) pf[u][k] = transpose_8x8(pf[u][k]);
+        if constexpr (H == 4) {
+            // row g < 4 of the transpose is head g with the first eight keys, row g + 4 the same head with the others
+#pragma unroll
+            for (int u = 0; u < 2; ++u) pf[u][1] = __shfl_xor_sync(0xffffffffu, pf[u][0], 16);
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                pf[u][0] = g < 4 ? pf[u][0] : 0u;
+                pf[u][1] = g < 4 ? pf[u][1] : 0u;
+            }
+        }
         // ---- values
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
@@ -347,120 +436,117 @@ __global__ void __launch_bounds__(32 * dec8_most_warps<D>(), 1) kv8_decode_kerne
         }
         // ---- the tile S turns ahead takes this one's place
         __syncwarp();
-        const int ahead = i + S * stride, before = slot == 0 ? S - 1 : slot - 1;
-        if (i != i0 && ahead - stride < tiles) keep_scales(before, pending);
-        if (ahead < tiles) {
-            copy_tile(slot, row);
-            pending = load_scales(row);
-            if (ahead + stride < tiles) row = row_of(ahead + stride);
-        }
-        __syncwarp();
-        if (++slot == S) {
-            slot = 0;
-            parity ^= 1;
-        }
+        const int ahead = i + S * stride;
+        copy_tile(slot, row_of(ahead, entry), ahead < tiles);
+        if (ahead + stride < tiles) entry = entry_of(ahead + stride);
+        if (++slot == S) slot = 0;
     }
-    for (int k = 0; k < S && i < tiles; ++k, i += stride) {      // given up: not to leave before the copies under way
-        mbar_wait(full + 8 * slot, parity);
-        if (++slot == S) {
-            slot = 0;
-            parity ^= 1;
-        }
-    }
+    cp_async_wait<0>();
     pdl_launch_dependents();
     __syncthreads();
 
-    // ---- the warps of the block: statistics (m, m', l) and outputs of 8 heads each
+    // ---- the warps of the block: statistics (m, m', l) and outputs of H heads each
     constexpr int LD = D + 4;
 #pragma unroll
-    for (int d = 4; d < 32; d <<= 1) {
+    for (int d = H == 4 ? 2 : 4; d < 32; d <<= 1) {
         l0 += __shfl_xor_sync(0xffffffffu, l0, d);
         l1 += __shfl_xor_sync(0xffffffffu, l1, d);
     }
-    float* o_s = reinterpret_cast<float*>(smem8);         // [W][8][LD], the block's own in the first warp's place
-    float* mine = reinterpret_cast<float*>(smem8 + (size_t)W * dec8_ring<D>(S));     // the block's own: [8][4]
-    float* st_s = mine + 32;                              // [W][8][4]
-    if (g == 0) {
-        float* st = st_s + warp * 32 + 2 * t * 4;
-        st[0] = m0; st[1] = w0; st[2] = l0;
-        st[4] = m1; st[5] = w1; st[6] = l1;
+    float* o_s = reinterpret_cast<float*>(smem8);         // [W][H][LD]
+    float4* st_s = reinterpret_cast<float4*>(smem8 + (size_t)W * dec8_ring<D>());     // [W][8]
+    float4* all_st = st_s + W * 8;                        // [C][8]: of the blocks
+    float* all_o = reinterpret_cast<float*>(all_st + 16 * 8);
+    if (g == 0 && 2 * t < H) {
+        st_s[warp * 8 + 2 * t] = make_float4(m0, w0, l0, 0.f);
+        st_s[warp * 8 + 2 * t + 1] = make_float4(m1, w1, l1, 0.f);
     }
-    {
-        float* dst = o_s + (size_t)warp * 8 * LD;
+    if (2 * t < H) {
+        float* dst = o_s + (size_t)(warp * H + 2 * t) * LD;
 #pragma unroll
-        for (int i = 0; i < MT; ++i) {
-            const int d = g * (D / 8) + 2 * i;            // rows g and g + 8 of the block: two neighbouring features
-            *reinterpret_cast<float2*>(dst + (2 * t) * LD + d) = make_float2(o[i][0], o[i][2]);
-            *reinterpret_cast<float2*>(dst + (2 * t + 1) * LD + d) = make_float2(o[i][1], o[i][3]);
+        for (int k = 0; k < MT; ++k) {
+            const int d = g * (D / 8) + 2 * k;            // rows g and g + 8 of the block: two neighbouring features
+            *reinterpret_cast<float2*>(dst + d) = make_float2(o[k][0], o[k][2]);
+            *reinterpret_cast<float2*>(dst + LD + d) = make_float2(o[k][1], o[k][3]);
         }
     }
     __syncthreads();
-    if (threadIdx.x < 8) {
+    // (m, m', l) of `n` parts together; a part whose every score was NaN has the maximum -inf and a sum of NaN
+    auto join = [](const float4* st, int n) -> float4 {
         float m = -INFINITY, w = -INFINITY, l = 0.f;
-        for (int i = 0; i < W; ++i) {
-            m = fmaxf(m, st_s[i * 32 + threadIdx.x * 4]);
-            w = fmaxf(w, st_s[i * 32 + threadIdx.x * 4 + 1]);
+#pragma unroll 4
+        for (int k = 0; k < n; ++k) {
+            m = fmaxf(m, st[k * 8].x);
+            w = fmaxf(w, st[k * 8].y);
         }
-        for (int i = 0; i < W; ++i) {
-            float* st = st_s + i * 32 + threadIdx.x * 4;
-            // (a warp whose every score was NaN has the maximum -inf and a sum of NaN)
-            l += st[2] == 0.f ? 0.f : st[0] == -INFINITY ? st[2] : st[2] * ex2(st[0] - m);
-            st[3] = ratio(st[1], w);
+#pragma unroll 4
+        for (int k = 0; k < n; ++k) {
+            const float4 x = st[k * 8];
+            l = fmaf(x.z, x.x == -INFINITY ? 1.f : ex2(x.x - m), l);      // (x.z is 0 or NaN where x.x is -inf)
         }
-        mine[threadIdx.x * 4] = m;
-        mine[threadIdx.x * 4 + 1] = w;
-        mine[threadIdx.x * 4 + 2] = l;
+        return make_float4(m, w, l, 0.f);
+    };
+    // sum of 2^(m'_k - w) x_k over `n` parts' four features
+    auto add = [](const float4* st, const float* x, int step, int n, float w) -> float4 {
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+        for (int k = 0; k < n; ++k) {
+            const float f = ratio(st[k * 8].y, w);
+            const float4 y = *reinterpret_cast<const float4*>(x + (size_t)k * step);
+            v.x = fmaf(y.x, f, v.x);
+            v.y = fmaf(y.y, f, v.y);
+            v.z = fmaf(y.z, f, v.z);
+            v.w = fmaf(y.w, f, v.w);
+        }
+        return v;
+    };
+    auto finish = [&](const float4& all, const float4& v, int h, int d) {
+        // 2^(m' - m) / l: the two maxima differ by the values' exponents and the slack at most
+        const float f = all.z == 0.f ? 0.f : ex2(all.y == -INFINITY ? 0.f : all.y - all.x) / all.z;
+        const float out[4] = {v.x * f, v.y * f, v.z * f, v.w * f};
+        store4(a.out + (size_t)token * a.nq * D + (size_t)(kvh * G + h0 + h) * D + d, out);
+    };
+    // four features a thread; block c joins the features [c D / C, (c + 1) D / C) of every head
+    constexpr int Q = D / 4;
+    const int log_c = 31 - __clz(C), q_share = Q >> log_c;
+    if (C > 1) {
+        cluster_wait();
+        for (int k = blockDim.x - 1 - threadIdx.x; k < heads * C; k += blockDim.x)
+            *cluster.map_shared_rank(all_st + rank * 8 + (k >> log_c), k & (C - 1)) = join(st_s + (k >> log_c), W);
     }
-    __syncthreads();
-    for (int i = threadIdx.x; i < heads * (D / 4); i += blockDim.x) {
-        const int h = i / (D / 4), d = (i % (D / 4)) * 4;
-        float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int w = 0; w < W; ++w) {
-            const float f = st_s[w * 32 + h * 4 + 3];
-            const float4 x = *reinterpret_cast<const float4*>(o_s + (size_t)(w * 8 + h) * LD + d);
-            sum.x = fmaf(x.x, f, sum.x);
-            sum.y = fmaf(x.y, f, sum.y);
-            sum.z = fmaf(x.z, f, sum.z);
-            sum.w = fmaf(x.w, f, sum.w);
+    for (int k = threadIdx.x; k < heads * Q; k += blockDim.x) {
+        const int h = k / Q, q = k % Q;
+        if (C == 1) {
+            const float4 all = join(st_s + h, W);
+            finish(all, add(st_s + h, o_s + (size_t)h * LD + q * 4, H * LD, W, all.y), h, q * 4);
+        } else {
+            float w = -INFINITY;
+#pragma unroll 4
+            for (int i = 0; i < W; ++i) w = fmaxf(w, st_s[i * 8 + h].y);
+            const int c = q / q_share;
+            float4* to = reinterpret_cast<float4*>(all_o) + (rank * H + h) * q_share + (q - c * q_share);
+            *cluster.map_shared_rank(to, c) = add(st_s + h, o_s + (size_t)h * LD + q * 4, H * LD, W, w);
         }
-        *reinterpret_cast<float4*>(o_s + (size_t)h * LD + d) = sum;       // (its own element of warp 0's part)
     }
-    cluster.sync();
-    // ---- the blocks of the cluster: each joins a share of the elements
-    const int total = heads * (D / 4);
-    for (int i = rank * blockDim.x + threadIdx.x; i < total; i += C * blockDim.x) {
-        const int h = i / (D / 4), d = (i % (D / 4)) * 4;
-        float m = -INFINITY, w = -INFINITY, l = 0.f;
-        for (int c = 0; c < C; ++c) {
-            const float* st = cluster.map_shared_rank(mine, c) + h * 4;
-            m = fmaxf(m, st[0]);
-            w = fmaxf(w, st[1]);
-        }
-        float v[4] = {0.f, 0.f, 0.f, 0.f};
-        for (int c = 0; c < C; ++c) {
-            const float* st = cluster.map_shared_rank(mine, c) + h * 4;
-            l += st[2] == 0.f ? 0.f : st[0] == -INFINITY ? st[2] : st[2] * ex2(st[0] - m);
-            const float f = ratio(st[1], w);
-            const float4 x = *reinterpret_cast<const float4*>(cluster.map_shared_rank(o_s, c) + (size_t)h * LD + d);
-            v[0] = fmaf(x.x, f, v[0]);
-            v[1] = fmaf(x.y, f, v[1]);
-            v[2] = fmaf(x.z, f, v[2]);
-            v[3] = fmaf(x.w, f, v[3]);
-        }
-        // 2^(m' - m) / l: the two maxima differ by the values' exponents at most
-        const float f = l == 0.f ? 0.f : ex2(w == -INFINITY ? 0.f : w - m) / l;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) v[k] *= f;
-        store4(a.out + (size_t)token * a.nq * D + (size_t)(kvh * G + h0 + h) * D + d, v);
+    if (C == 1) {
+        cluster_wait();
+        return;
     }
-    if (C > 1) cluster.sync();                            // nobody leaves while its memory is read
+    // ---- the blocks of the cluster: each joins its share
+    cluster_arrive();
+    cluster_wait();
+    for (int k = threadIdx.x; k < heads * q_share; k += blockDim.x) {
+        const int h = k / q_share, q = k - h * q_share;
+        const float4 all = join(all_st + h, C);
+        finish(all, add(all_st + h, all_o + (size_t)(h * q_share + q) * 4, H * q_share * 4, C, all.y), h,
+               (rank * q_share + q) * 4);
+    }
 }
 
-template <int D>
-static int launch_decode(const CUtensorMap& map, const Kv8DecodeArgs& a, int tokens, int blocks, int warps, cudaStream_t s) {
-    auto kernel = kv8_decode_kernel<D>;
-    const int smem = dec8_smem<D>(warps, a.stages);
-    if (warps < 1 || warps > dec8_most_warps<D>() || a.stages < 2 || a.stages > 8 || smem > 227 * 1024) return -1;
+template <int D, int H>
+static int launch_decode(const Kv8DecodeArgs& a, int tokens, int blocks, int warps, cudaStream_t s) {
+    auto kernel = kv8_decode_kernel<D, H>;
+    const int smem = dec8_smem<D>(warps);
+    if (warps < 1 || warps > dec8_most_warps<D>() || smem > 227 * 1024) return -1;
     static bool configured[64] = {false};
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
@@ -489,46 +575,31 @@ static int launch_decode(const CUtensorMap& map, const Kv8DecodeArgs& a, int tok
     attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
-    e = cudaLaunchKernelEx(&cfg, kernel, map, a);
+    e = cudaLaunchKernelEx(&cfg, kernel, a);
     return e != cudaSuccess ? (int)e : launch_status();
 }
 
 // Token i is row i of q (rows q_stride apart, 16-byte aligned), out, token_req and cache_pos.  `blocks` blocks (1, 2, 4,
-// 8 or 16, a cluster) of `warps` warps with rings of `stages` tiles share the keys of a (token, kv head, 8 query heads).
-// page_size: a multiple of 8.  Returns 0, a CUDA error code or -1 (shape refused).
+// 8 or 16, a cluster) of `warps` warps share the keys of a (token, kv head, 8 query heads, or up to 4 where a kv head has
+// no more).  page_size: a multiple of 8.  Returns 0, a CUDA error code or -1 (shape refused).
 MSTAR_API int mstar_kv8_decode(const void* q, int q_stride, void* out, const void* codes, const void* scales, int pages,
                                const int* block_table, int bt_stride, const int* token_req, const int* cache_pos,
                                int tokens, int nq, int nkv, int hd, int page_size, int window, int keep_first, float scale,
-                               int blocks, int warps, int stages, int* error_word, void* stream) {
+                               int blocks, int warps, void* stream) {
     if (tokens <= 0) return 0;
-    const long long rows = (long long)pages * 2 * nkv * page_size;
     if (nkv <= 0 || nq % nkv != 0 || page_size <= 0 || page_size % 8 != 0 || pages <= 0 || tokens > 65535 || blocks < 1 ||
         blocks > 16 || (blocks & (blocks - 1)) != 0 || ((uintptr_t)q & 15) != 0 || q_stride % 8 != 0 ||
-        ((uintptr_t)codes & 15) != 0 || ((uintptr_t)out & 7) != 0 || rows > 0x7fffffffll || error_word == nullptr ||
-        (hd != 64 && hd != 128 && hd != 256))
+        ((uintptr_t)codes & 15) != 0 || ((uintptr_t)scales & 7) != 0 || ((uintptr_t)out & 7) != 0 ||
+        (long long)pages * 2 * nkv * page_size > 0xffffffffll || (hd != 64 && hd != 128 && hd != 256))
         return -1;
-    const int box = page_size % 16 == 0 ? 16 : 8;
-    // the cache as a matrix of `rows` rows of hd bytes
-    CUtensorMap map;
-    {
-        EncodeTiledFn encode = encode_tiled_fn();
-        if (encode == nullptr) return (int)cudaErrorNotSupported;
-        const cuuint64_t dims[2] = {(cuuint64_t)hd, (cuuint64_t)rows};
-        const cuuint64_t strides[1] = {(cuuint64_t)hd};
-        const cuuint32_t size[2] = {(cuuint32_t)(hd < 128 ? hd : 128), (cuuint32_t)box};
-        const cuuint32_t elem[2] = {1, 1};
-        if (encode(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(codes), dims, strides, size, elem,
-                   CU_TENSOR_MAP_INTERLEAVE_NONE, hd < 128 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
-                   CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
-            return -1;
-    }
     const Kv8DecodeArgs a{(const bf16*)q, (bf16*)out, (const uint8_t*)codes, (const uint8_t*)scales, block_table,
                           token_req, cache_pos, q_stride, bt_stride, pages, nq, nkv, window, keep_first,
-                          (nq / nkv + 7) / 8, scale * 1.4426950408889634f, page_split(page_size), box, stages, error_word};
+                          (nq / nkv + 7) / 8, scale * 1.4426950408889634f, page_split(page_size)};
     const cudaStream_t s = (cudaStream_t)stream;
+    const bool few = nq / nkv <= 4;
     switch (hd) {
-        case 64: return launch_decode<64>(map, a, tokens, blocks, warps, s);
-        case 128: return launch_decode<128>(map, a, tokens, blocks, warps, s);
-        default: return launch_decode<256>(map, a, tokens, blocks, warps, s);
+        case 64: return few ? launch_decode<64, 4>(a, tokens, blocks, warps, s) : launch_decode<64, 8>(a, tokens, blocks, warps, s);
+        case 128: return few ? launch_decode<128, 4>(a, tokens, blocks, warps, s) : launch_decode<128, 8>(a, tokens, blocks, warps, s);
+        default: return few ? launch_decode<256, 4>(a, tokens, blocks, warps, s) : launch_decode<256, 8>(a, tokens, blocks, warps, s);
     }
 }

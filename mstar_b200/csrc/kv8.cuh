@@ -55,17 +55,20 @@ __device__ __forceinline__ void kv8_unpack4(uint32_t w, float* v) {
     v[3] = b.y;
 }
 
-// Division of a non-negative number below 2^31 by a fixed page size: a shift where that is a power of two.
+// Division of a number in [0, 2^31) by a fixed page size d: with s = ceil(log2 d) and m = ceil(2^(31 + s) / d) < 2^32 + 1,
+// m d - 2^(31 + s) < d <= 2^s, so that n m / 2^(31 + s) exceeds n / d by less than 2^-31 n / d < 1 / d and has its floor.
 struct PageSplit {
-    int size, shift;    // shift < 0: no power of two
+    int size;
+    uint32_t magic;
+    int shift;
 };
 static inline PageSplit page_split(int size) {
     int s = 0;
-    while ((1 << s) < size) ++s;
-    return PageSplit{size, (1 << s) == size ? s : -1};
+    while ((1ll << s) < size) ++s;
+    return PageSplit{size, (uint32_t)(((1ull << (31 + s)) + size - 1) / size), 31 + s};
 }
 __device__ __forceinline__ int page_of(const PageSplit& p, int key) {
-    return p.shift >= 0 ? key >> p.shift : key / p.size;
+    return (int)(((uint64_t)(uint32_t)key * p.magic) >> p.shift);
 }
 // The page that a request's table (a row of `width` entries) names for its page `logical`, brought into the cache.
 __device__ __forceinline__ int page_id(const int* table, int logical, int width, int pages) {

@@ -18,7 +18,7 @@ from __future__ import annotations
 
 import torch
 
-from . import _DT, _dt, _error_ptr, _need_cuda, _ptr, _stream, lib, num_sms
+from . import _DT, _dt, _need_cuda, _ptr, _stream, lib, num_sms
 from .lib import KernelError, check
 
 KV8_DTYPE = torch.float8_e4m3fn
@@ -178,20 +178,17 @@ def _float_attention(what, q, out, kv_cache, kv_scales, block_table, indptr, kv_
 KV8_DECODE_HEAD_DIMS = (64, 128, 256)
 
 
-def _rows_fit(kv_cache) -> bool:
-    """Whether the cache's rows can be counted in 31 bits, as the copies by TMA count them."""
-    return kv_cache.numel() // kv_cache.shape[4] < 2 ** 31
-
-
 def kv8_decode_shape(pairs: int, max_keys: int, head_dim: int, sms: int) -> tuple:
-    """(blocks of a cluster, warps of a block, tiles of a warp's ring) that share the keys of each of
-    ``pairs`` (token, kv head, 8 query heads) in the decode kernel."""
-    want = max(1, min(-(-max_keys // 32), -(-8 * sms // max(pairs, 1))))
-    warps = 4 if want <= 64 else 8
+    """(blocks of a cluster, warps of a block) that share the keys of each of ``pairs`` (token, kv head,
+    8 query heads) in the decode kernel: about seven warps an SM, none without a tile of 32 keys; blocks
+    of four warps, of eight where the pairs are few.  (8 x 8, 4 x 4 and 1 x 4 for 8, 64 and 512 pairs took
+    15.3, 9.1 and 18.2 us; half and twice the blocks 22.2 and 23.2, 12.5 and 15.4, - and 24.9.)"""
+    want = max(1, min(-(-max_keys // 32), -(-7 * sms // max(pairs, 1))))
+    warps = 4 if want <= 32 or head_dim == 256 else 8
     blocks = 1
-    while blocks < 16 and blocks * warps < want:
+    while blocks < 8 and blocks * warps < want:
         blocks *= 2
-    return blocks, warps, 3 if head_dim <= 128 else 2
+    return blocks, warps
 
 
 def _most_keys(max_len, max_q, window, keep_first) -> int:
@@ -217,15 +214,14 @@ def paged_decode_attention_kv8(q: torch.Tensor, out: torch.Tensor, kv_cache: tor
     if tokens <= 0:
         return
     if (q.dtype == torch.bfloat16 and head_dim in KV8_DECODE_HEAD_DIMS and page_size % 8 == 0
-            and q.stride(0) % 8 == 0 and (q.data_ptr() | kv_cache.data_ptr()) % 16 == 0 and _rows_fit(kv_cache)):
+            and q.stride(0) % 8 == 0 and (q.data_ptr() | kv_cache.data_ptr()) % 16 == 0 and kv_scales.data_ptr() % 8 == 0):
         most = _most_keys(max_len, 1, window, keep_first)
         pairs = tokens * num_kv_heads * -(-num_heads // num_kv_heads // 8)
-        blocks, warps, stages = kv8_decode_shape(pairs, most, head_dim, num_sms(q.device))
+        blocks, warps = kv8_decode_shape(pairs, most, head_dim, num_sms(q.device))
         check(lib.get("attention_kv8_decode").mstar_kv8_decode(
             q.data_ptr(), q.stride(0), out.data_ptr(), kv_cache.data_ptr(), kv_scales.data_ptr(), kv_cache.shape[0],
             block_table.data_ptr(), block_table.stride(0), token_req.data_ptr(), cache_pos.data_ptr(), tokens, num_heads,
-            num_kv_heads, head_dim, page_size, window, keep_first, scale, blocks, warps, stages, _error_ptr(q),
-            _stream()), what)
+            num_kv_heads, head_dim, page_size, window, keep_first, scale, blocks, warps, _stream()), what)
         return
     _float_attention(what, q, out, kv_cache, kv_scales, block_table, None, None, token_req, cache_pos, 0, tokens, 1,
                      _most_keys(max_len, 1, window, keep_first), num_heads, num_kv_heads, head_dim, page_size, window,

@@ -147,7 +147,7 @@ _SIGNATURES = {
     },
     "attention_kv8_decode": {
         "mstar_kv8_decode": [_vp, _i, _vp, _vp, _vp, _i, _vp, _i, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _f, _i, _i,
-                             _i, _vp, _vp],
+                             _vp],
     },
     "gemm_f32": {
         "mstar_sgemm_nt": [_vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp, _vp],
