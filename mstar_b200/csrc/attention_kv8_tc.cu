@@ -1,0 +1,575 @@
+// Attention of prompt portions over the 8-bit cache (format: kv8.cuh) on the fifth-generation tensor cores, bfloat16,
+// head_dim 64 or 128, up to 128 query heads per kv head, any page size, window and kept first keys.
+//
+// One CTA owns two row tiles of 128 / G whole tokens each (G query heads per kv head; rows are (token, head) pairs) and
+// one kv head, and walks the keys that some of its rows see, 128 at a time.  Its sixteen warps:
+//   * 4 loader warps copy a tile's key codes into the tile that the MMAs read (cp.async), and read its value codes into
+//     registers (the next tile's loads are under way meanwhile), make bfloat16 of them and store the swizzled tile;
+//   * one thread issues the products: S_A = Q_A K^T, S_B = Q_B K^T of the next tile as soon as a tile's weights have been
+//     used, and O_A += P_A V, O_B += P_B V as soon as weights are there, so that the tensor cores work for one row tile
+//     while the other one's softmax runs;
+//   * 4 + 4 softmax warps own a row a thread: they read it from tensor memory, keep the running maximum and sum in
+//     registers, and write the weights as bfloat16 over the scores (tcgen05.st); the output in tensor memory is rescaled
+//     only when a maximum grew by more than 2^8.
+// Tensor memory: S / P 2 x 128 columns, O 2 x head_dim.  Shared memory (head_dim 128): queries 64 KB, two stages of keys
+// of 16 KB and two of values of 32 KB each.
+//
+// The scores' product takes the keys' codes as they are: kind::f8f6f4 at twice the rate of 16-bit operands, and the
+// query in two codes, x = hi + lo, so that the two products cost what one of 16 bits does and the keys need neither
+// conversion nor a second copy.  A row of queries is scaled by a power of two to have its largest number in (224, 448];
+// hi is within 2^-4 of a number, lo leaves 2^-10 at most, 2^-17.8 of the row's largest (a bfloat16 query is within 2^-9
+// of itself to begin with).  The keys' scales are a factor a score, two at a time (mul.f32x2); it is NaN for a row that
+// is held as NaNs, so that who sees it gets NaNs and nobody else.
+//
+// Values become bfloat16 with their row's scale folded in, which is exact for every scale: sign, exponent and mantissa
+// of a code are moved to bfloat16's places (which reads as the code times 2^-120, subnormal codes included), and a
+// product by 2^(120 + e) puts it right (two for e > 7); the even and the odd codes of a word become a pair each, and the
+// output's features are put back in order as they are stored.  (float16 values relative to a common exponent need a
+// third of the instructions, but rows of values 2^20 apart in size lost the smaller ones.)
+//
+// What bounds it: per tile of 128 keys and 256 rows (head_dim 128) the MMAs take 2,048 clocks, the exponentials 2,048 (16
+// a clock and SM), reading operands and storing tiles some 240 KB of shared memory at 128 bytes a clock.
+//
+// Few row tiles and many keys: the tiles are cut into `splits` ranges whose (maximum, sum, output) go to scratch memory
+// and are joined by a second kernel (kv8_merge.cuh).  Row tiles with the most keys are launched first.
+//
+// Every mbarrier wait is bounded; one that runs out sets the error word (31 to 36) and everybody leaves.
+#include "attention_tc_util.cuh"
+#include "kv8_merge.cuh"
+#include "mma_util.cuh"
+#include "tma_util.cuh"
+
+#define K8_ROWS 128
+#define K8_KEYS 128
+#define K8_THREADS 512
+#define K8_SLACK 8.0f
+
+struct Kv8TcArgs {
+    const bf16* q;
+    bf16* out;
+    const uint8_t *codes, *scales;
+    const int *block_table, *qo_indptr, *kv_len;
+    int q_stride, bt_stride, pages, nq, nkv, window, keep_first, first_entry;
+    float scale_log2e;
+    PageSplit page;
+    Kv8Parts parts;
+    int* error_word;
+};
+
+__host__ __device__ constexpr int k8_codes(int hd) { return 128 * hd; }          // a tile of codes: 128 rows
+__host__ __device__ constexpr int k8_values(int hd) { return K8_KEYS * hd * 2; }
+// queries [2 row tiles][hi, lo], two stages of keys and of values, of four tiles each key's row, factor and value factor,
+// the barriers
+__host__ __device__ constexpr int k8_smem(int hd) { return 6 * k8_codes(hd) + 2 * k8_values(hd) + 4 * 128 * 12 + 192; }
+
+__device__ __forceinline__ void k8_sync_loaders() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+template <int R> __device__ __forceinline__ void k8_more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(R)); }
+template <int R> __device__ __forceinline__ void k8_less_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(R)); }
+// Instruction descriptors, D float: kind::f8f6f4 with e4m3 operands, kind::f16 with bfloat16 ones and an MN-major B.
+__host__ __device__ constexpr uint32_t k8_idesc_codes(int m, int n) {
+    return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
+}
+__device__ __forceinline__ void k8_mma_codes(uint32_t tmem_d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(tmem_d), "l"(da), "l"(db), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+// Descriptor of a tile of codes, K-major: rows of 128 bytes with the 128-byte swizzle, or of 64 with the 64-byte one;
+// groups of 8 rows follow one another.
+template <int HD> __device__ __forceinline__ uint64_t k8_desc_codes(uint32_t addr) {
+    return (uint64_t)((addr >> 4) & 0x3FFF) | (1ull << 16) | ((uint64_t)(8 * HD >> 4) << 32) | (1ull << 46) |
+           ((HD == 128 ? 2ull : 4ull) << 61);
+}
+// where a 16-byte run c of row r lies in such a tile
+template <int HD> __device__ __forceinline__ uint32_t k8_code_place(int r, int c) {
+    return (uint32_t)(r * HD + ((HD == 128 ? c ^ (r & 7) : c ^ ((r >> 1) & 3)) << 4));
+}
+__device__ __forceinline__ uint64_t k8_two(uint32_t lo, uint32_t hi) { return (uint64_t)lo | ((uint64_t)hi << 32); }
+__device__ __forceinline__ uint64_t k8_mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t k8_fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t k8_add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ float k8_lo(uint64_t x) { return __uint_as_float((uint32_t)x); }
+__device__ __forceinline__ float k8_hi(uint64_t x) { return __uint_as_float((uint32_t)(x >> 32)); }
+__device__ __forceinline__ uint32_t k8_mul_bf16x2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+// bits 0 .. n - 1
+__device__ __forceinline__ uint32_t k8_below(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }
+// The factors that make a code's bits in bfloat16's places its value for the row's exponent e: 2^min(120 + e, 127) in
+// the low half, 2^max(e - 7, 0) in the high one.
+__device__ __forceinline__ uint32_t k8_value_factors(int e) {
+    return ((uint32_t)(min(120 + e, 127) + 127) << 7) | ((uint32_t)(max(e - 7, 0) + 127) << 23);
+}
+
+template <int HD>
+__global__ void __launch_bounds__(K8_THREADS, 1) kv8_attention_tc_kernel(Kv8TcArgs a) {
+    constexpr int QT = k8_codes(HD), KT = k8_codes(HD), VT = k8_values(HD);
+    extern __shared__ __align__(1024) unsigned char smem[];
+    unsigned char* q_s = smem;                       // [2 row tiles][hi, lo][128 rows x HD codes]
+    unsigned char* k_s = q_s + 4 * QT;               // [2 stages][128 keys x HD codes]
+    unsigned char* v_s = k_s + 2 * KT;               // [2 stages][HD / 64 blocks][128 keys x 128 bytes]
+    uint32_t* row_s = reinterpret_cast<uint32_t*>(v_s + 2 * VT);     // [4][128] rows of the cache
+    float* kf_s = reinterpret_cast<float*>(row_s + 512);             // [4][128] the keys' scales
+    uint32_t* vf_s = row_s + 1024;                                   // [4][128] the values' factors
+    uint64_t* bars = reinterpret_cast<uint64_t*>(vf_s + 512);
+    const uint32_t k_full = tc_smem(bars), v_full = tc_smem(bars + 2), k_empty = tc_smem(bars + 4),
+                   v_empty = tc_smem(bars + 6), s_full = tc_smem(bars + 8), p_ready = tc_smem(bars + 10),
+                   q_ready = tc_smem(bars + 12), o_full = tc_smem(bars + 14);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 16);
+
+    pdl_wait();
+    const int splits = a.parts.splits;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int kvh = blockIdx.x / splits, split = blockIdx.x % splits;
+    const int e = a.first_entry + blockIdx.z;
+    const int G = a.nq / a.nkv, TPT = K8_ROWS / G, RPT = TPT * G;
+    const int q_start = a.qo_indptr[e], q_len = a.qo_indptr[e + 1] - q_start;
+    const int tok0 = (gridDim.y - 1 - blockIdx.y) * 2 * TPT;
+    if (tok0 >= q_len) return;
+    if ((tc_smem(smem) & 1023u) != 0) {              // the swizzled tiles need this alignment
+        if (tid == 0) atomicExch(a.error_word, 31);
+        return;
+    }
+    const int past = a.kv_len[e] - q_len;
+    const bool has_b = tok0 + TPT < q_len;
+    const int last_tok = min(tok0 + 2 * TPT, q_len) - 1;
+    const SeenKeys seen = seen_keys(past + tok0, past + last_tok, a.window, a.keep_first);
+    const int all_tiles = (seen.count + K8_KEYS - 1) / K8_KEYS;
+    const int per_split = (all_tiles + splits - 1) / splits;
+    const int tile0 = split * per_split, ntiles = max(0, min(all_tiles - tile0, per_split));
+
+    if (tid == 0) {
+        for (int i = 0; i < 16; ++i) mbar_init(tc_smem(bars + i), i < 4 || (i >= 10 && i < 14) ? 128 : 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 12) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc_smem(tmem_slot)), "r"(512u)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    pt_fence_before();
+    __syncthreads();
+    pt_fence_after();
+    const uint32_t tmem = *tmem_slot;
+
+    if (warp >= 12) {
+        // ------------------------------------------------------------------------------------- the products
+        k8_less_registers<48>();
+        if (warp == 12 && lane == 0 && ntiles > 0) {
+            constexpr uint32_t idesc_s = k8_idesc_codes(K8_ROWS, K8_KEYS), idesc_o = pt_idesc(K8_ROWS, HD, 1);
+            auto scores = [&](int x, int j) {
+                const uint32_t qa = tc_smem(q_s + x * 2 * QT), ka = tc_smem(k_s + (j & 1) * KT);
+#pragma unroll
+                for (int part = 0; part < 2; ++part)
+#pragma unroll
+                    for (int kk = 0; kk < HD / 32; ++kk)
+                        k8_mma_codes(tmem + x * 128, k8_desc_codes<HD>(qa + part * QT + kk * 32),
+                                     k8_desc_codes<HD>(ka + kk * 32), idesc_s, (part | kk) != 0);
+                pt_commit(s_full + 8 * x);
+            };
+            bool ok = mbar_wait(q_ready, 0) && (!has_b || mbar_wait(q_ready + 8, 0)) && mbar_wait(k_full, 0);
+            if (ok) {
+                pt_fence_after();
+                scores(0, 0);
+                if (has_b) scores(1, 0);
+                pt_commit(k_empty);
+            }
+            for (int j = 0; j < ntiles && ok; ++j) {
+                const uint32_t ph = ((uint32_t)j >> 1) & 1u, ph1 = ((uint32_t)(j + 1) >> 1) & 1u;
+                const int s = j & 1, s1 = s ^ 1;
+                ok = mbar_wait(v_full + 8 * s, ph);
+                for (int x = 0; x < (has_b ? 2 : 1) && ok; ++x) {
+                    ok = mbar_wait(p_ready + 8 * x, (uint32_t)j & 1u);
+                    if (!ok) break;
+                    pt_fence_after();
+                    const uint32_t va = tc_smem(v_s + s * VT);
+#pragma unroll
+                    for (int kk = 0; kk < K8_KEYS / 16; ++kk)
+                        pt_mma_ts(tmem + 256 + x * HD, tmem + x * 128 + kk * 8, pt_desc(va + kk * 16 * 128, K8_KEYS * 128, 1024),
+                                  idesc_o, (j | kk) != 0);
+                    if (x == 1 || !has_b) pt_commit(v_empty + 8 * s);
+                    if (j == ntiles - 1) {
+                        pt_commit(o_full + 8 * x);
+                    } else {
+                        if (x == 0) ok = mbar_wait(k_full + 8 * s1, ph1);
+                        if (!ok) break;
+                        pt_fence_after();
+                        // (over the weights that the product before reads: one thread's products run in their order)
+                        scores(x, j + 1);
+                        if (x == 1 || !has_b) pt_commit(k_empty + 8 * s1);
+                    }
+                }
+            }
+            if (!ok) atomicExch(a.error_word, 32);
+        }
+    } else if (warp >= 8) {
+        // ---------------------------------------------------------------------- keys and values from the pages
+        k8_less_registers<96>();
+        const int ct = tid - 256, w = ct >> 5;
+        const int* bt = a.block_table + (size_t)e * a.bt_stride;
+        const size_t plane = (size_t)a.nkv * a.page.size;
+        constexpr int CPR = HD / 16, NP = CPR, RP = 128 / CPR;   // 16-byte runs a row, passes, rows of a pass
+        // eight neighbouring lanes: two rows' four runs, whose stores then fall into different banks
+        const int run = HD == 128 ? (lane & 3) | ((lane >> 1) & 4) : lane & 3;
+        const int sub = HD == 128 ? ((lane >> 2) & 1) | ((lane >> 3) & 2) : lane >> 2;
+        const int r0 = w * (RP / 4) + sub;
+        auto key_at = [&](int j) { return key_of(seen, min((tile0 + j) * K8_KEYS + ct, seen.count - 1)); };
+        auto entry_of = [&](int j) -> int { return bt[min(page_of(a.page, key_at(j)), a.bt_stride - 1)]; };
+        auto row_of = [&](int j, int entry) -> uint32_t {
+            const int key = key_at(j), page = (int)min((unsigned)entry, (unsigned)(a.pages - 1));
+            return ((uint32_t)page * 2 * a.nkv + kvh) * a.page.size + (uint32_t)(key - page_of(a.page, key) * a.page.size);
+        };
+        // row and factors of tile j from this thread's key; four tiles' places, so that one barrier a tile will do
+        auto stage = [&](int j, uint32_t row, int kb, int vb) {
+            const int at = (j & 3) * 128 + ct;
+            const bool bad = kb == KV8_BAD_BYTE || vb == KV8_BAD_BYTE;
+            row_s[at] = row;
+            kf_s[at] = bad ? __int_as_float(0x7fc00000) : kv8_scale(kb);
+            vf_s[at] = k8_value_factors(bad ? 0 : vb - 127);
+            k8_sync_loaders();
+        };
+        auto copy_keys = [&](int j) {
+            const uint32_t tile = tc_smem(k_s + (j & 1) * KT);
+#pragma unroll
+            for (int i = 0; i < NP; ++i) {
+                const int r = i * RP + r0;
+                cp_async_16(tile + k8_code_place<HD>(r, run), a.codes + (size_t)row_s[(j & 3) * 128 + r] * HD + run * 16, 16);
+            }
+            cp_async_commit();
+        };
+        auto load_values = [&](int j, uint4 (&x)[NP]) {
+#pragma unroll
+            for (int i = 0; i < NP; ++i)
+                x[i] = *reinterpret_cast<const uint4*>(
+                    a.codes + ((size_t)row_s[(j & 3) * 128 + i * RP + r0] + plane) * HD + run * 16);
+        };
+        auto store_values = [&](int j, const uint4 (&x)[NP]) {
+#pragma unroll
+            for (int i = 0; i < NP; ++i) {
+                const int r = i * RP + r0, c = run * 2;
+                const uint32_t f = vf_s[(j & 3) * 128 + r], f1 = __byte_perm(f, f, 0x1010);
+                const uint32_t in[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+                uint32_t out[8];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {       // codes 0 and 2 of a word, then 1 and 3
+                    out[2 * k] = k8_mul_bf16x2(((in[k] << 8) & 0x80008000u) | ((in[k] << 4) & 0x07f007f0u), f1);
+                    out[2 * k + 1] = k8_mul_bf16x2((in[k] & 0x80008000u) | ((in[k] >> 4) & 0x07f007f0u), f1);
+                }
+                if ((f >> 16) != 0x3f80u) {         // values above 2^15
+                    const uint32_t f2 = __byte_perm(f, f, 0x3232);
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) out[k] = k8_mul_bf16x2(out[k], f2);
+                }
+                unsigned char* base = v_s + (j & 1) * VT + (c >> 3) * (128 * 128) + r * 128;
+                *reinterpret_cast<uint4*>(base + (((c & 7) ^ (r & 7)) << 4)) = make_uint4(out[0], out[1], out[2], out[3]);
+                *reinterpret_cast<uint4*>(base + ((((c & 7) + 1) ^ (r & 7)) << 4)) = make_uint4(out[4], out[5], out[6], out[7]);
+            }
+        };
+        if (ntiles > 0) {
+            uint4 vx[NP];
+            bool ok = true;      // (a warp that gives up a wait goes on to meet the others at the loaders' barrier)
+            // table entries are read two tiles ahead of their rows' use, scales one
+            int entry = entry_of(0);
+            uint32_t row = row_of(0, entry);
+            int kb = a.scales[row], vb = a.scales[row + plane];
+            if (ntiles > 1) entry = entry_of(1);
+            stage(0, row, kb, vb);
+            copy_keys(0);
+            load_values(0, vx);
+            if (ntiles > 1) {
+                row = row_of(1, entry);
+                kb = a.scales[row];
+                vb = a.scales[row + plane];
+                if (ntiles > 2) entry = entry_of(2);
+            }
+            cp_async_wait<0>();
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            mbar_arrive(k_full);
+            for (int j = 0; j < ntiles; ++j) {
+                const int s = j & 1, s1 = s ^ 1;
+                const bool more = j + 1 < ntiles;
+                if (more) {
+                    stage(j + 1, row, kb, vb);
+                    // the tile's place is free when the scores of the tile before are done
+                    if (ok && !pt_wait_warp(k_empty + 8 * s1, (((uint32_t)(j + 1) >> 1) & 1u) ^ 1u)) {
+                        if (lane == 0) atomicExch(a.error_word, 33);
+                        ok = false;
+                    }
+                    if (ok) copy_keys(j + 1);
+                    if (j + 2 < ntiles) {
+                        row = row_of(j + 2, entry);
+                        kb = a.scales[row];
+                        vb = a.scales[row + plane];
+                        if (j + 3 < ntiles) entry = entry_of(j + 3);
+                    }
+                }
+                if (ok && !pt_wait_warp(v_empty + 8 * s, (((uint32_t)j >> 1) & 1u) ^ 1u)) {
+                    if (lane == 0) atomicExch(a.error_word, 34);
+                    ok = false;
+                }
+                if (ok) {
+                    store_values(j, vx);
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    mbar_arrive(v_full + 8 * s);
+                }
+                if (more) {
+                    load_values(j + 1, vx);
+                    cp_async_wait<0>();
+                    if (ok) {
+                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                        mbar_arrive(k_full + 8 * s1);
+                    }
+                }
+            }
+        }
+    } else {
+        // ------------------------------------------------------------------------- softmax, a row a thread
+        k8_more_registers<184>();
+        const int x = warp >> 2, r = tid & 127;
+        const int tok = tok0 + x * TPT + min(r, RPT - 1) / G;
+        const bool valid = r < RPT && tok < q_len;
+        const size_t head = (size_t)(q_start + min(tok, q_len - 1)) * a.nq + kvh * G + r % G;
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+        const uint32_t t_s = tmem + lanes + x * 128, t_o = tmem + lanes + 256 + x * HD;
+        float m = -INFINITY, l = 0.f, row_scale = 0.f;
+        bool ok = true;
+        if (x == 0 || has_b) {
+            if (ntiles > 0) {
+                // the query: two codes a number, into the K-major swizzled tiles
+                const bf16* q = a.q + (size_t)(q_start + min(tok, q_len - 1)) * a.q_stride + (size_t)(kvh * G + r % G) * HD;
+                float most = 0.f;
+#pragma unroll 4
+                for (int c = 0; c < HD / 8; ++c) {
+                    float v[8];
+                    load8(q + c * 8, v);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) most = fabsf(v[i]) < INFINITY ? fmaxf(most, fabsf(v[i])) : INFINITY;
+                }
+                const int byte = kv8_scale_byte(most);            // a query that is not finite gives NaNs
+                const float inv = valid && byte != KV8_BAD_BYTE ? kv8_inverse_scale(byte) : 0.f;
+                row_scale = byte != KV8_BAD_BYTE ? kv8_scale(byte) * a.scale_log2e : __int_as_float(0x7fc00000);
+#pragma unroll 2
+                for (int c = 0; c < HD / 16; ++c) {
+                    uint32_t hi[4], lo[4];
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        float v[8];
+                        load8(q + c * 16 + h * 8, v);
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) v[i] = inv != 0.f ? v[i] * inv : 0.f;
+#pragma unroll
+                        for (int k = 0; k < 2; ++k) {
+                            float b[4];
+                            hi[2 * h + k] = kv8_pack4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
+                            kv8_unpack4(hi[2 * h + k], b);
+                            lo[2 * h + k] = kv8_pack4(v[4 * k] - b[0], v[4 * k + 1] - b[1], v[4 * k + 2] - b[2], v[4 * k + 3] - b[3]);
+                        }
+                    }
+                    unsigned char* to = q_s + x * 2 * QT + k8_code_place<HD>(r, c);
+                    *reinterpret_cast<uint4*>(to) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                    *reinterpret_cast<uint4*>(to + QT) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                mbar_arrive(q_ready + 8 * x);
+            }
+            // in counts of seen keys: the newest key of this row and the newest one that its window has passed
+            const int pos = past + min(tok, q_len - 1), shift = seen.kept - seen.lo;
+            const int v_max = pos + shift, v_min = a.window > 0 ? pos - a.window + shift : -1;
+            // of the tile's rows: the least v_max, the largest v_min
+            const int all_max = past + tok0 + x * TPT + shift;
+            const int all_min = a.window > 0 ? past + min(tok0 + x * TPT + TPT, q_len) - 1 - a.window + shift : -1;
+            for (int j = 0; j < ntiles; ++j) {
+                if (!pt_wait_warp(s_full + 8 * x, (uint32_t)j & 1u)) {
+                    if (lane == 0) atomicExch(a.error_word, 35);
+                    ok = false;
+                    break;
+                }
+                pt_fence_after();
+                const float4* kf = reinterpret_cast<const float4*>(kf_s + (j & 3) * 128);
+                const int v0 = (tile0 + j) * K8_KEYS;
+                uint64_t t[64];                         // scores times their key's scale, in pairs
+                {
+                    uint32_t s[2][32];
+                    pt_ld32(t_s, s[0]);
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        pt_wait_ld();
+                        if (c < 3) pt_ld32(t_s + (c + 1) * 32, s[(c + 1) & 1]);
+                        const uint32_t* sc = s[c & 1];
+#pragma unroll
+                        for (int i = 0; i < 32; i += 4) {
+                            const float4 f = kf[c * 8 + (i >> 2)];
+                            t[c * 16 + (i >> 1)] = k8_mul2(k8_two(sc[i], sc[i + 1]),
+                                                           k8_two(__float_as_uint(f.x), __float_as_uint(f.y)));
+                            t[c * 16 + (i >> 1) + 1] = k8_mul2(k8_two(sc[i + 2], sc[i + 3]),
+                                                               k8_two(__float_as_uint(f.z), __float_as_uint(f.w)));
+                        }
+                    }
+                }
+                if (v0 + K8_KEYS - 1 > all_max || v0 <= all_min) {
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        const int b = v0 + c * 32;
+                        const uint32_t seen_bits = k8_below(v_max + 1 - b) & ~(k8_below(v_min + 1 - b) & ~k8_below(a.keep_first - b));
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            uint32_t lo = (uint32_t)t[c * 16 + i], hi = (uint32_t)(t[c * 16 + i] >> 32);
+                            if (!(seen_bits >> (2 * i) & 1u)) lo = 0xff800000u;          // -inf
+                            if (!(seen_bits >> (2 * i + 1) & 1u)) hi = 0xff800000u;
+                            t[c * 16 + i] = k8_two(lo, hi);
+                        }
+                    }
+                }
+                float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) mx[c] = fmaxf(fmaxf(mx[c], k8_lo(t[c * 16 + i])), k8_hi(t[c * 16 + i]));
+                const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * row_scale;
+                float alpha = 1.f;
+                if (top > m + K8_SLACK) {
+                    alpha = pt_ex2(m - top);
+                    m = top;
+                }
+                // a row that has seen nothing yet: weights of exp(-inf) whatever finite number is taken off
+                const float ref = m == -INFINITY ? 0.f : m;
+                const uint64_t ref2 = k8_two(__float_as_uint(-ref), __float_as_uint(-ref));
+                const uint64_t scale2 = k8_two(__float_as_uint(row_scale), __float_as_uint(row_scale));
+                l *= alpha;
+                uint64_t sum[2] = {0ull, 0ull};
+                uint32_t packed[2][32];
+#pragma unroll
+                for (int i = 0; i < 64; ++i) {
+                    const uint64_t d = k8_fma2(t[i], scale2, ref2);
+                    const float p0 = pt_ex2(k8_lo(d)), p1 = pt_ex2(k8_hi(d));
+                    sum[i & 1] = k8_add2(sum[i & 1], k8_two(__float_as_uint(p0), __float_as_uint(p1)));
+                    packed[i >> 5][i & 31] = pack_bf16(p0, p1);
+                }
+                const uint64_t both = k8_add2(sum[0], sum[1]);
+                l += k8_lo(both) + k8_hi(both);
+                if (j > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
+                    // (the scores came after the product before on the tensor cores: the output is at rest)
+#pragma unroll 1
+                    for (int c0 = 0; c0 < HD; c0 += 32) {
+                        uint32_t o[32];
+                        pt_ld32(t_o + c0, o);
+                        pt_wait_ld();
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+                        pt_st32(t_o + c0, o);
+                    }
+                }
+                pt_st32(t_s, packed[0]);
+                pt_st32(t_s + 32, packed[1]);
+                pt_wait_st();
+                pt_fence_before();
+                mbar_arrive(p_ready + 8 * x);
+            }
+            if (ntiles > 0 && ok && !pt_wait_warp(o_full + 8 * x, 0)) {
+                if (lane == 0) atomicExch(a.error_word, 36);
+                ok = false;
+            }
+            pt_fence_after();
+            // ---------------------------------------------------------------- epilogue
+            if (ok) {
+                const size_t at = (head - (size_t)kv8_first_token(a.parts) * a.nq) * splits + split;
+                const float f = splits > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l;
+                if (splits > 1 && valid) {
+                    a.parts.ml[2 * at] = l == 0.f ? -INFINITY : m;
+                    a.parts.ml[2 * at + 1] = l;
+                }
+#pragma unroll 1
+                for (int c0 = 0; c0 < HD && ntiles > 0; c0 += 32) {
+                    uint32_t o[32];
+                    pt_ld32(t_o + c0, o);
+                    pt_wait_ld();
+                    if (valid) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            float v[8];
+#pragma unroll
+                            for (int k = 0; k < 8; ++k)            // (places 1 and 2 of four hold features 2 and 1)
+                                v[k] = __uint_as_float(o[8 * i + ((k & 3) == 1 ? k + 1 : (k & 3) == 2 ? k - 1 : k)]) * f;
+                            if (splits > 1) store8(a.parts.o + at * HD + c0 + 8 * i, v);
+                            else store8(a.out + head * HD + c0 + 8 * i, v);
+                        }
+                    }
+                }
+                if (ntiles == 0 && splits == 1 && valid) {       // rows that see nothing at all
+                    const float none[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+                    for (int c0 = 0; c0 < HD; c0 += 8) store8(a.out + head * HD + c0, none);
+                }
+            }
+        }
+    }
+    pt_fence_before();
+    __syncthreads();
+    pdl_launch_dependents();
+    if (warp == 12) {
+        pt_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+    }
+}
+
+template <int HD> static int launch_kv8_tc(const Kv8TcArgs& a, dim3 grid, cudaStream_t s) {
+    auto kernel = kv8_attention_tc_kernel<HD>;
+    // more than half of an SM's shared memory, so that no second CTA lands there and waits for tensor memory
+    const int smem = k8_smem(HD) > 120 * 1024 ? k8_smem(HD) : 120 * 1024;
+    static bool configured[64] = {false};
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return (int)e;
+    if (dev < 0 || dev >= 64) return -1;
+    if (!configured[dev]) {
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        if (e != cudaSuccess) return (int)e;
+        configured[dev] = true;
+    }
+    e = mstar_launch(kernel, grid, dim3(K8_THREADS), (size_t)smem, s, a);
+    return e != cudaSuccess ? (int)e : launch_status();
+}
+
+// Entries [first_entry, first_entry + count) of at most max_q tokens each.  q rows q_stride apart, 16-byte aligned.
+// `tokens`, `splits`, `part_o` and `part_ml` as in mstar_kv8_attention.  Returns 0, a CUDA error code or -1 (shape
+// refused).
+MSTAR_API int mstar_kv8_attention_tc(const void* q, int q_stride, void* out, const void* codes, const void* scales, int pages,
+                                     const int* block_table, int bt_stride, const int* qo_indptr, const int* kv_len,
+                                     int first_entry, int count, int max_q, int tokens, int nq, int nkv, int hd,
+                                     int page_size, int window, int keep_first, float scale, int splits, float* part_o,
+                                     float* part_ml, int* error_word, void* stream) {
+    if (count <= 0 || max_q <= 0) return 0;
+    if ((hd != 64 && hd != 128) || nkv <= 0 || nq % nkv != 0 || nq / nkv > K8_ROWS || page_size <= 0 || pages <= 0 ||
+        splits < 1 || count > 65535 || error_word == nullptr || !(scale > 0.f) || ((uintptr_t)q & 15) != 0 ||
+        q_stride % 8 != 0 || ((uintptr_t)codes & 15) != 0 || ((uintptr_t)out & 15) != 0 ||
+        (long long)pages * 2 * nkv * page_size > 0xffffffffll)
+        return -1;
+    const Kv8Parts parts{part_o, part_ml, splits, qo_indptr + first_entry, count};
+    const Kv8TcArgs a{(const bf16*)q, (bf16*)out, (const uint8_t*)codes, (const uint8_t*)scales, block_table, qo_indptr,
+                      kv_len, q_stride, bt_stride, pages, nq, nkv, window, keep_first, first_entry,
+                      scale * 1.4426950408889634f, page_split(page_size), parts, error_word};
+    const int per_cta = 2 * (K8_ROWS / (nq / nkv));
+    const long long tiles = ((long long)max_q + per_cta - 1) / per_cta;
+    if (tiles > 65535) return -1;
+    const dim3 grid(nkv * splits, (unsigned)tiles, count);
+    const cudaStream_t s = (cudaStream_t)stream;
+    const int code = hd == 64 ? launch_kv8_tc<64>(a, grid, s) : launch_kv8_tc<128>(a, grid, s);
+    if (code != 0 || splits == 1) return code;
+    return kv8_merge(parts, out, MSTAR_BF16, tokens, nq, hd, s);
+}

@@ -610,7 +610,8 @@ def tcgen05_error_word(device) -> torch.Tensor:
     1-3 tcgen05 GEMM (producer, MMA issuer, epilogue), 4 decode attention copies, 6-12 tcgen05
     prefill attention, 13-14 bulk-copy small-M GEMM, 15-17 swapped-operand tcgen05 GEMM, 18
     delta-rule scan in pieces, 19-21 grouped expert GEMM, 22-27 prompt attention with probabilities
-    in three parts, 28-29 float product by bfloat16 parts; zero otherwise."""
+    in three parts, 28-29 float product by bfloat16 parts, 31-36 attention of portions over an 8-bit
+    cache; zero otherwise."""
     key = torch.device(device).index or 0
     if key not in _tc_error_words:
         _tc_error_words[key] = torch.zeros(1, dtype=torch.int32, device=device)
@@ -643,6 +644,8 @@ WAIT_CODES.update({c: "prompt attention with probabilities in three parts: a wai
                    "ran out" for c in range(22, 28)})
 WAIT_CODES.update({28: "float product by bfloat16 parts: a worker waited for a stage or a sum",
                    29: "float product by bfloat16 parts: the MMA issuer waited for operands"})
+WAIT_CODES.update({c: "attention of portions over an 8-bit cache: a wait on one of its barriers ran out"
+                   for c in range(31, 37)})
 WAIT_CODES.update({c: "tcgen05 prefill attention: a wait on one of its barriers ran out"
                    for c in range(6, 13)})
 

@@ -55,6 +55,7 @@ LIBRARIES = {
     "kv8_cache": ("cuda", ["kv8_cache.cu"], []),
     "attention_kv8": ("cuda", ["attention_kv8.cu"], []),
     "attention_kv8_decode": ("cuda", ["attention_kv8_decode.cu"], []),
+    "attention_kv8_tc": ("cuda", ["attention_kv8_tc.cu"], []),
     "host": ("host", ["host/cache_manager.cpp"], []),
 }
 

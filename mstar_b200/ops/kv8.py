@@ -18,7 +18,7 @@ from __future__ import annotations
 
 import torch
 
-from . import _DT, _dt, _need_cuda, _ptr, _stream, lib, num_sms
+from . import _DT, _dt, _error_ptr, _need_cuda, _ptr, _stream, lib, num_sms
 from .lib import KernelError, check
 
 KV8_DTYPE = torch.float8_e4m3fn
@@ -183,12 +183,21 @@ def kv8_decode_shape(pairs: int, max_keys: int, head_dim: int, sms: int) -> tupl
     8 query heads) in the decode kernel: about seven warps an SM, none without a tile of 32 keys; blocks
     of four warps, of eight where the pairs are few.  (8 x 8, 4 x 4 and 1 x 4 for 8, 64 and 512 pairs took
     15.3, 9.1 and 18.2 us; half and twice the blocks 22.2 and 23.2, 12.5 and 15.4, - and 24.9.)"""
-    want = max(1, min(-(-max_keys // 32), -(-7 * sms // max(pairs, 1))))
+    want = max(1, min(-(-max_keys // 32), 7 * sms // max(pairs, 1)))
     warps = 4 if want <= 32 or head_dim == 256 else 8
     blocks = 1
     while blocks < 8 and blocks * warps < want:
         blocks *= 2
     return blocks, warps
+
+
+KV8_TC_HEAD_DIMS = (64, 128)
+
+
+def kv8_tc_splits(blocks: int, max_keys: int, sms: int) -> int:
+    """Ranges that the keys of ``blocks`` pairs of row tiles are cut into in the tensor-core kernel: a block
+    an SM, ranges of at least two tiles of 128 keys, at most 64."""
+    return max(1, min(64, sms // max(blocks, 1), -(-max_keys // 256)))
 
 
 def _most_keys(max_len, max_q, window, keep_first) -> int:
@@ -248,6 +257,22 @@ def paged_prefill_attention_kv8(q: torch.Tensor, out: torch.Tensor, kv_cache: to
     _check_index(what, block_table, (qo_indptr, last + 1), (kv_len, last))
     _check_device(what, q, out, kv_cache, kv_scales, block_table, qo_indptr, kv_len)
     if entries <= 0 or max_q_len <= 0 or out.shape[0] == 0:
+        return
+    group = num_heads // num_kv_heads
+    if (q.dtype == torch.bfloat16 and head_dim in KV8_TC_HEAD_DIMS and group <= 128 and q.stride(0) % 8 == 0
+            and (q.data_ptr() | kv_cache.data_ptr() | out.data_ptr()) % 16 == 0):
+        tiles = -(-max_q_len // (2 * (128 // group)))
+        most = _most_keys(max_kv_len, max_q_len, window, keep_first)
+        splits = kv8_tc_splits(tiles * num_kv_heads * entries, most, num_sms(q.device))
+        tokens = min(out.shape[0], entries * max_q_len)
+        part, part_o, part_ml = _parts(q, tokens, num_heads, head_dim, splits)
+        check(lib.get("attention_kv8_tc").mstar_kv8_attention_tc(
+            q.data_ptr(), q.stride(0), out.data_ptr(), kv_cache.data_ptr(), kv_scales.data_ptr(), kv_cache.shape[0],
+            block_table.data_ptr(), block_table.stride(0), qo_indptr.data_ptr(), kv_len.data_ptr(), first_entry, entries,
+            max_q_len, tokens, num_heads, num_kv_heads, head_dim, page_size, window, keep_first, scale, splits, part_o,
+            part_ml, _error_ptr(q), _stream()), what)
+        if splits > 1:
+            lib.add_launches(1)                 # the kernel that joins the parts
         return
     _float_attention(what, q, out, kv_cache, kv_scales, block_table, qo_indptr, kv_len, None, None, first_entry, entries,
                      max_q_len, _most_keys(max_kv_len, max_q_len, window, keep_first), num_heads, num_kv_heads, head_dim,

@@ -149,6 +149,10 @@ _SIGNATURES = {
         "mstar_kv8_decode": [_vp, _i, _vp, _vp, _vp, _i, _vp, _i, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _f, _i, _i,
                              _vp],
     },
+    "attention_kv8_tc": {
+        "mstar_kv8_attention_tc": [_vp, _i, _vp, _vp, _vp, _i, _vp, _i, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _i, _i,
+                                   _f, _i, _vp, _vp, _vp, _vp],
+    },
     "gemm_f32": {
         "mstar_sgemm_nt": [_vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp, _vp],
         "mstar_sgemm_parts": [_vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _vp, _vp],
