@@ -257,3 +257,11 @@ MSTAR_API int mstar_kv8_attention(const void* q, int q_stride, void* out, int ac
     if (code != 0 || splits == 1) return code;
     return kv8_merge(parts, out, act_dtype, tokens, nq, hd, s);
 }
+
+MSTAR_API int mstar_kv8_attention_packed(const long long* a) {
+    return mstar_kv8_attention((const void*)a[0], (int)a[1], (void*)a[2], (int)a[3], (const void*)a[4],
+        (const void*)a[5], (int)a[6], (const int*)a[7], (int)a[8], (const int*)a[9], (const int*)a[10],
+        (const int*)a[11], (const int*)a[12], (int)a[13], (int)a[14], (int)a[15], (int)a[16], (int)a[17], (int)a[18],
+        (int)a[19], (int)a[20], (int)a[21], (int)a[22], kv8_packed_float(a[23]), (int)a[24], (float*)a[25],
+        (float*)a[26], (void*)a[27]);
+}

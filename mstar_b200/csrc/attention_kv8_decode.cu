@@ -603,3 +603,10 @@ MSTAR_API int mstar_kv8_decode(const void* q, int q_stride, void* out, const voi
         default: return few ? launch_decode<256, 4>(a, tokens, blocks, warps, s) : launch_decode<256, 8>(a, tokens, blocks, warps, s);
     }
 }
+
+MSTAR_API int mstar_kv8_decode_packed(const long long* a) {
+    return mstar_kv8_decode((const void*)a[0], (int)a[1], (void*)a[2], (const void*)a[3], (const void*)a[4],
+        (int)a[5], (const int*)a[6], (int)a[7], (const int*)a[8], (const int*)a[9], (int)a[10], (int)a[11],
+        (int)a[12], (int)a[13], (int)a[14], (int)a[15], (int)a[16], kv8_packed_float(a[17]), (int)a[18], (int)a[19],
+        (void*)a[20]);
+}

@@ -5,7 +5,7 @@
 // one kv head, and walks the keys that some of its rows see, 128 at a time.  Its sixteen warps:
 //   * 4 loader warps copy a tile's key codes into the tile that the MMAs read (cp.async), and read its value codes into
 //     registers (the next tile's loads are under way meanwhile), make bfloat16 of them and store the swizzled tile;
-//   * one thread issues the products: S_A = Q_A K^T, S_B = Q_B K^T of the next tile as soon as a tile's weights have been
+//   * one warp issues the products: S_A = Q_A K^T, S_B = Q_B K^T of the next tile as soon as a tile's weights have been
 //     used, and O_A += P_A V, O_B += P_B V as soon as weights are there, so that the tensor cores work for one row tile
 //     while the other one's softmax runs;
 //   * 4 + 4 softmax warps own a row a thread: they read it from tensor memory, keep the running maximum and sum in
@@ -69,20 +69,50 @@ template <int R> __device__ __forceinline__ void k8_less_registers() { asm volat
 __host__ __device__ constexpr uint32_t k8_idesc_codes(int m, int n) {
     return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
-__device__ __forceinline__ void k8_mma_codes(uint32_t tmem_d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t accumulate) {
+// The products and their commits, issued by the one lane whose `leader` is not zero.  All lanes run the code around them:
+// operands computed in a branch of one lane are vector registers, and moving them to uniform ones for every product took
+// some 140 clocks a product, twice what the product takes.
+__device__ __forceinline__ uint32_t k8_elect() {
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+    return r;
+}
+// (descriptors as their low words, where the address is, beside high words that do not change)
+__device__ __forceinline__ void k8_mma_codes(uint32_t leader, uint32_t tmem_d, uint32_t da, uint32_t db, uint32_t high,
+                                             uint32_t idesc, uint32_t accumulate) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
-        ::"r"(tmem_d), "l"(da), "l"(db), "r"(idesc), "r"(accumulate)
+        "{\n\t.reg .pred p, q;\n\t.reg .b64 a, b;\n\t"
+        "setp.ne.b32 p, %5, 0;\n\t"
+        "setp.ne.b32 q, %6, 0;\n\t"
+        "mov.b64 a, {%1, %3};\n\t"
+        "mov.b64 b, {%2, %3};\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a, b, %4, p;\n\t}"
+        ::"r"(tmem_d), "r"(da), "r"(db), "r"(high), "r"(idesc), "r"(accumulate), "r"(leader)
         : "memory");
 }
-// Descriptor of a tile of codes, K-major: rows of 128 bytes with the 128-byte swizzle, or of 64 with the 64-byte one;
-// groups of 8 rows follow one another.
-template <int HD> __device__ __forceinline__ uint64_t k8_desc_codes(uint32_t addr) {
-    return (uint64_t)((addr >> 4) & 0x3FFF) | (1ull << 16) | ((uint64_t)(8 * HD >> 4) << 32) | (1ull << 46) |
-           ((HD == 128 ? 2ull : 4ull) << 61);
+__device__ __forceinline__ void k8_mma_weights(uint32_t leader, uint32_t tmem_d, uint32_t tmem_a, uint32_t db, uint32_t high,
+                                               uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t.reg .b64 b;\n\t"
+        "setp.ne.b32 p, %5, 0;\n\t"
+        "setp.ne.b32 q, %6, 0;\n\t"
+        "mov.b64 b, {%2, %3};\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n\t}"
+        ::"r"(tmem_d), "r"(tmem_a), "r"(db), "r"(high), "r"(idesc), "r"(accumulate), "r"(leader)
+        : "memory");
 }
+__device__ __forceinline__ void k8_commit(uint32_t leader, uint32_t bar) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar), "r"(leader)
+        : "memory");
+}
+// High words of the descriptors (stride byte offset, version, swizzle) of a tile of codes, K-major: rows of 128 bytes with
+// the 128-byte swizzle, or of 64 with the 64-byte one, groups of 8 rows after one another; and of a tile of values.
+template <int HD> __host__ __device__ constexpr uint32_t k8_codes_high() {
+    return (uint32_t)(8 * HD >> 4) | (1u << 14) | ((HD == 128 ? 2u : 4u) << 29);
+}
+__host__ __device__ constexpr uint32_t k8_values_high() { return (1024u >> 4) | (1u << 14) | (2u << 29); }
 // where a 16-byte run c of row r lies in such a tile
 template <int HD> __device__ __forceinline__ uint32_t k8_code_place(int r, int c) {
     return (uint32_t)(r * HD + ((HD == 128 ? c ^ (r & 7) : c ^ ((r >> 1) & 3)) << 4));
@@ -171,57 +201,76 @@ __global__ void __launch_bounds__(K8_THREADS, 1) kv8_attention_tc_kernel(Kv8TcAr
 
     if (warp >= 12) {
         // ------------------------------------------------------------------------------------- the products
-        k8_less_registers<48>();
-        if (warp == 12 && lane == 0 && ntiles > 0) {
+        // (the launch's 128 a thread, dealt out again: 2 x 184 + 80 + 64 = 2 x 184 + 88 + 56 = 512; no spills)
+        k8_less_registers<HD == 128 ? 64 : 56>();
+        if (warp == 12 && ntiles > 0) {
             constexpr uint32_t idesc_s = k8_idesc_codes(K8_ROWS, K8_KEYS), idesc_o = pt_idesc(K8_ROWS, HD, 1);
+            const uint32_t leader = k8_elect();
+            // low words: the address in units of 16 bytes (below 2^14 of them), the leading byte offset from bit 16 on
+            const uint32_t q_low = tc_smem(q_s) >> 4 | 1u << 16, k_low = tc_smem(k_s) >> 4 | 1u << 16;
+            const uint32_t v_low = tc_smem(v_s) >> 4 | (uint32_t)(K8_KEYS * 128 >> 4) << 16;
             auto scores = [&](int x, int j) {
-                const uint32_t qa = tc_smem(q_s + x * 2 * QT), ka = tc_smem(k_s + (j & 1) * KT);
+                const uint32_t qa = q_low + (uint32_t)(x * 2 * QT >> 4), ka = k_low + (uint32_t)((j & 1) * KT >> 4);
 #pragma unroll
                 for (int part = 0; part < 2; ++part)
 #pragma unroll
                     for (int kk = 0; kk < HD / 32; ++kk)
-                        k8_mma_codes(tmem + x * 128, k8_desc_codes<HD>(qa + part * QT + kk * 32),
-                                     k8_desc_codes<HD>(ka + kk * 32), idesc_s, (part | kk) != 0);
-                pt_commit(s_full + 8 * x);
+                        k8_mma_codes(leader, tmem + x * 128, qa + (uint32_t)((part * QT + kk * 32) >> 4),
+                                     ka + (uint32_t)(kk * 32 >> 4), k8_codes_high<HD>(), idesc_s, (part | kk) != 0);
+                k8_commit(leader, s_full + 8 * x);
             };
-            bool ok = mbar_wait(q_ready, 0) && (!has_b || mbar_wait(q_ready + 8, 0)) && mbar_wait(k_full, 0);
+            auto output = [&](int x, int j) {
+                const uint32_t va = v_low + (uint32_t)((j & 1) * VT >> 4);
+#pragma unroll
+                for (int kk = 0; kk < K8_KEYS / 16; ++kk)
+                    k8_mma_weights(leader, tmem + 256 + x * HD, tmem + x * 128 + kk * 8, va + (uint32_t)(kk * 16 * 128 >> 4),
+                                   k8_values_high(), idesc_o, (j | kk) != 0);
+            };
+            bool ok = pt_wait_warp(q_ready, 0) && (!has_b || pt_wait_warp(q_ready + 8, 0)) && pt_wait_warp(k_full, 0);
             if (ok) {
                 pt_fence_after();
                 scores(0, 0);
                 if (has_b) scores(1, 0);
-                pt_commit(k_empty);
+                k8_commit(leader, k_empty);
             }
             for (int j = 0; j < ntiles && ok; ++j) {
                 const uint32_t ph = ((uint32_t)j >> 1) & 1u, ph1 = ((uint32_t)(j + 1) >> 1) & 1u;
                 const int s = j & 1, s1 = s ^ 1;
-                ok = mbar_wait(v_full + 8 * s, ph);
-                for (int x = 0; x < (has_b ? 2 : 1) && ok; ++x) {
-                    ok = mbar_wait(p_ready + 8 * x, (uint32_t)j & 1u);
+                const bool more = j + 1 < ntiles;
+                ok = pt_wait_warp(v_full + 8 * s, ph) && pt_wait_warp(p_ready, (uint32_t)j & 1u);
+                if (!ok) break;
+                pt_fence_after();
+                output(0, j);
+                if (!has_b) k8_commit(leader, v_empty + 8 * s);
+                if (more) {
+                    ok = pt_wait_warp(k_full + 8 * s1, ph1);
                     if (!ok) break;
                     pt_fence_after();
-                    const uint32_t va = tc_smem(v_s + s * VT);
-#pragma unroll
-                    for (int kk = 0; kk < K8_KEYS / 16; ++kk)
-                        pt_mma_ts(tmem + 256 + x * HD, tmem + x * 128 + kk * 8, pt_desc(va + kk * 16 * 128, K8_KEYS * 128, 1024),
-                                  idesc_o, (j | kk) != 0);
-                    if (x == 1 || !has_b) pt_commit(v_empty + 8 * s);
-                    if (j == ntiles - 1) {
-                        pt_commit(o_full + 8 * x);
+                    // (over the weights that the product before reads: one thread's products run in their order)
+                    scores(0, j + 1);
+                    if (!has_b) k8_commit(leader, k_empty + 8 * s1);
+                } else {
+                    k8_commit(leader, o_full);
+                }
+                if (has_b) {
+                    ok = pt_wait_warp(p_ready + 8, (uint32_t)j & 1u);
+                    if (!ok) break;
+                    pt_fence_after();
+                    output(1, j);
+                    k8_commit(leader, v_empty + 8 * s);
+                    if (more) {
+                        scores(1, j + 1);
+                        k8_commit(leader, k_empty + 8 * s1);
                     } else {
-                        if (x == 0) ok = mbar_wait(k_full + 8 * s1, ph1);
-                        if (!ok) break;
-                        pt_fence_after();
-                        // (over the weights that the product before reads: one thread's products run in their order)
-                        scores(x, j + 1);
-                        if (x == 1 || !has_b) pt_commit(k_empty + 8 * s1);
+                        k8_commit(leader, o_full + 8);
                     }
                 }
             }
-            if (!ok) atomicExch(a.error_word, 32);
+            if (!ok && lane == 0) atomicExch(a.error_word, 32);
         }
     } else if (warp >= 8) {
         // ---------------------------------------------------------------------- keys and values from the pages
-        k8_less_registers<96>();
+        k8_less_registers<HD == 128 ? 80 : 88>();
         const int ct = tid - 256, w = ct >> 5;
         const int* bt = a.block_table + (size_t)e * a.bt_stride;
         const size_t plane = (size_t)a.nkv * a.page.size;
@@ -572,4 +621,11 @@ MSTAR_API int mstar_kv8_attention_tc(const void* q, int q_stride, void* out, con
     const int code = hd == 64 ? launch_kv8_tc<64>(a, grid, s) : launch_kv8_tc<128>(a, grid, s);
     if (code != 0 || splits == 1) return code;
     return kv8_merge(parts, out, MSTAR_BF16, tokens, nq, hd, s);
+}
+
+MSTAR_API int mstar_kv8_attention_tc_packed(const long long* a) {
+    return mstar_kv8_attention_tc((const void*)a[0], (int)a[1], (void*)a[2], (const void*)a[3], (const void*)a[4],
+        (int)a[5], (const int*)a[6], (int)a[7], (const int*)a[8], (const int*)a[9], (int)a[10], (int)a[11],
+        (int)a[12], (int)a[13], (int)a[14], (int)a[15], (int)a[16], (int)a[17], (int)a[18], (int)a[19],
+        kv8_packed_float(a[20]), (int)a[21], (float*)a[22], (float*)a[23], (int*)a[24], (void*)a[25]);
 }

@@ -18,6 +18,7 @@
 #pragma once
 
 #include <cuda_fp8.h>
+#include <string.h>
 
 #include "common.cuh"
 
@@ -90,4 +91,12 @@ __device__ __forceinline__ SeenKeys seen_keys(int first, int last, int window, i
 __device__ __forceinline__ int key_of(const SeenKeys& s, int v) { return v < s.kept ? v : v - s.kept + s.lo; }
 __device__ __forceinline__ bool sees(int pos, int key, int window, int keep_first) {
     return key <= pos && (window <= 0 || key > pos - window || key < keep_first);
+}
+
+// The entry points also take their arguments as one array of 64-bit numbers, a float as the bits of a double: a call
+// through ctypes converts each argument by itself, 3.6 us for 21 of them against 0.7 for one packed string.
+static inline float kv8_packed_float(long long bits) {
+    double d;
+    memcpy(&d, &bits, sizeof(d));
+    return (float)d;
 }

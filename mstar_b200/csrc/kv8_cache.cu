@@ -22,28 +22,49 @@ struct Kv8WriteArgs {
     PageSplit page;
 };
 
-// 8 of row[d ..] as floats; V: the row is aligned to 8 elements
-template <bool V, typename A> __device__ __forceinline__ void take8(const A* p, float (&x)[8]) {
-    if constexpr (V) {
-        load8(p, x);
-    } else {
+// 8 of a row as they are loaded: one or two 16-byte words
+template <typename A> struct Run8 { uint4 w[sizeof(A) / 2]; };
+__device__ __forceinline__ void numbers(const Run8<bf16>& r, float (&x)[8]) {
+    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&r);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = to_float(p[i]);
+    for (int i = 0; i < 4; ++i) {
+        const float2 f = __bfloat1622float2(h[i]);
+        x[2 * i] = f.x;
+        x[2 * i + 1] = f.y;
     }
+}
+__device__ __forceinline__ void numbers(const Run8<float>& r, float (&x)[8]) {
+    const float* f = reinterpret_cast<const float*>(&r);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = f[i];
 }
 
 // R: the type of the rotation, float or double
 __device__ __forceinline__ void half_turns(float t, float* sn, float* cs) { sincospif(t, sn, cs); }
 __device__ __forceinline__ void half_turns(double t, double* sn, double* cs) { sincospi(t, sn, cs); }
 
-// L: threads of a head, a power of two with 8 L >= hd.  V: pairs, halves and rows in whole aligned groups of 8.
+// L: threads of a head, a power of two with 8 L >= hd.  V: pairs, halves and rows in whole aligned groups of 8; the
+// loads of a thread's next head then go before the work on this one, those of its first before the angles.
 template <typename A, typename R, int L, bool V>
-__global__ void __launch_bounds__(256) rope_kv8_write_kernel(const A* __restrict__ qkv, A* __restrict__ q_out,
-                                                             Kv8WriteArgs a) {
+__global__ void __launch_bounds__(256) rope_kv8_write_kernel(const A* qkv, A* q_out, Kv8WriteArgs a) {
     pdl_launch_dependents();   // a short kernel: the long one after it may be scheduled now
-    qkv = pdl_after(qkv, pdl_wait());
+    pdl_wait();
     __shared__ R tab_sn[128], tab_cs[128];
+    constexpr int PER = 256 / L;
     const int t = blockIdx.x, hd = a.hd, half = a.rot >> 1;
+    const int l = threadIdx.x % L, d0 = l * 8, heads = a.nq + 2 * a.nkv, step = gridDim.y * PER;
+    const bool in = d0 < hd, turned = d0 < a.rot, upper = d0 >= half;
+    const A* row = qkv + (size_t)t * a.in_stride;
+    Run8<A> own, other;
+    auto load = [&](int h) {
+        if (V && in && h < heads) {
+            own = *reinterpret_cast<const Run8<A>*>(row + (size_t)h * hd + d0);
+            if (turned && h < a.nq + a.nkv && !a.interleaved)
+                other = *reinterpret_cast<const Run8<A>*>(row + (size_t)h * hd + (upper ? d0 - half : d0 + half));
+        }
+    };
+    const int h0 = blockIdx.y * PER + threadIdx.x / L;
+    load(h0);
     for (int j = threadIdx.x; j < half; j += blockDim.x) {
         double turns = (double)a.positions[t] * (double)a.inv_freq[j] * 0.31830988618379067154;   // half-turns
         turns -= 2.0 * rint(0.5 * turns);
@@ -56,19 +77,22 @@ __global__ void __launch_bounds__(256) rope_kv8_write_kernel(const A* __restrict
     const int slot = held ? cp - logical * a.page.size : 0;
     __syncthreads();
 
-    constexpr int PER = 256 / L;
-    const int l = threadIdx.x % L, d0 = l * 8;
-    const bool in = d0 < hd;
-    const int heads = a.nq + 2 * a.nkv;
-    const A* row = qkv + (size_t)t * a.in_stride;
-    for (int h = blockIdx.y * PER + threadIdx.x / L; h < heads; h += gridDim.y * PER) {
+    for (int h = h0; h < heads; h += step) {
         float y[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) y[i] = 0.f;
         if (in) {
             const A* src = row + (size_t)h * hd;
-            take8<V>(src + d0, y);
-            if (h < a.nq + a.nkv && d0 < a.rot) {
+            float z[8];
+            if constexpr (V) {
+                numbers(own, y);
+                numbers(other, z);
+                load(h + step);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) y[i] = to_float(src[d0 + i]);
+            }
+            if (h < a.nq + a.nkv && turned) {
                 if (V && a.interleaved) {
 #pragma unroll
                     for (int i = 0; i < 8; i += 2) {
@@ -78,10 +102,7 @@ __global__ void __launch_bounds__(256) rope_kv8_write_kernel(const A* __restrict
                         y[i + 1] = (float)(x1 * cs + x0 * sn);
                     }
                 } else if (V) {
-                    const bool upper = d0 >= half;
                     const int j0 = upper ? d0 - half : d0;
-                    float z[8];
-                    take8<V>(src + (upper ? d0 - half : d0 + half), z);
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
                         const R sn = upper ? tab_sn[j0 + i] : -tab_sn[j0 + i];
@@ -91,11 +112,11 @@ __global__ void __launch_bounds__(256) rope_kv8_write_kernel(const A* __restrict
                     for (int i = 0; i < 8; ++i) {
                         const int d = d0 + i;
                         if (d >= a.rot) break;
-                        const bool upper = a.interleaved ? (d & 1) : d >= half;
-                        const int j = a.interleaved ? d >> 1 : upper ? d - half : d;
-                        const int other = a.interleaved ? d ^ 1 : upper ? d - half : d + half;
-                        const R sn = upper ? tab_sn[j] : -tab_sn[j];
-                        y[i] = (float)((R)y[i] * tab_cs[j] + (R)to_float(src[other]) * sn);
+                        const bool second = a.interleaved ? (d & 1) : d >= half;
+                        const int j = a.interleaved ? d >> 1 : second ? d - half : d;
+                        const int pair = a.interleaved ? d ^ 1 : second ? d - half : d + half;
+                        const R sn = second ? tab_sn[j] : -tab_sn[j];
+                        y[i] = (float)((R)y[i] * tab_cs[j] + (R)to_float(src[pair]) * sn);
                     }
                 }
             }
@@ -177,36 +198,67 @@ MSTAR_API int mstar_rope_kv8_write(const void* qkv, int act_dtype, int in_stride
 }
 
 // ------------------------------------------------------------------------------- rows read back
-// 8 features a thread; a block takes the 2 nkv rows of one token.
-template <typename A>
-__global__ void __launch_bounds__(256)
-kv8_read_rows_kernel(const uint8_t* codes, const uint8_t* scales, const int* block_table, int bt_stride,
-                     const int* token_req, const int* cache_pos, A* out, int rows, int hd, int pages, PageSplit page) {
+// 8 features a thread and U such runs, 256 apart, whose chains of loads (place, table entry, codes) go side by side: a
+// run alone is three latencies for 24 bytes.
+struct Kv8ReadArgs {
+    const uint8_t *codes, *scales;
+    const int *block_table, *token_req, *cache_pos;
+    int bt_stride, rows, hd, pages, runs;
+    PageSplit page, per_row, per_token;      // runs of a row, runs of a token
+};
+template <typename A, int U> __global__ void __launch_bounds__(256) kv8_read_rows_kernel(Kv8ReadArgs a, A* out) {
     pdl_launch_dependents();
     pdl_wait();
-    const int per_row = hd >> 3, per_token = rows * per_row;
-    const int t = blockIdx.x;
-    const int cp = cache_pos[t], logical = cp < 0 ? -1 : page_of(page, cp);
-    int id = -1;
-    if (logical >= 0 && logical < bt_stride) id = block_table[(size_t)token_req[t] * bt_stride + logical];
-    const bool held = id >= 0 && id < pages;
-    const int slot = held ? cp - logical * page.size : 0;
-    for (int i = threadIdx.x; i < per_token; i += blockDim.x) {
-        const int r = i / per_row, d = (i - r * per_row) * 8;
-        float v[8];
+    const int first = blockIdx.x * (256 * U) + threadIdx.x;
+    int t[U], cp[U], id[U], req[U];
+    size_t at[U];
+    int d[U], scale[U];
+    uint2 w[U];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] = 0.f;
-        if (held) {
-            const size_t at = ((size_t)id * rows + r) * page.size + slot;
-            const uint2 w = *reinterpret_cast<const uint2*>(codes + at * hd + d);
-            const float s = kv8_scale(scales[at]);
-            kv8_unpack4(w.x, v);
-            kv8_unpack4(w.y, v + 4);
-#pragma unroll
-            for (int k = 0; k < 8; ++k) v[k] *= s;
-        }
-        store8(out + (size_t)t * rows * hd + (size_t)r * hd + d, v);
+    for (int u = 0; u < U; ++u) {
+        const int run = min(first + u * 256, a.runs - 1);
+        t[u] = page_of(a.per_token, run);
+        cp[u] = a.cache_pos[t[u]];
+        req[u] = a.token_req[t[u]];
+        d[u] = run - t[u] * a.per_token.size;
     }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int logical = cp[u] < 0 ? -1 : page_of(a.page, cp[u]);
+        id[u] = logical >= 0 && logical < a.bt_stride ? a.block_table[(size_t)req[u] * a.bt_stride + logical] : -1;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int r = page_of(a.per_row, d[u]);
+        d[u] = (d[u] - r * a.per_row.size) * 8;
+        const bool held = id[u] >= 0 && id[u] < a.pages;
+        const int slot = held ? cp[u] - page_of(a.page, cp[u]) * a.page.size : 0;
+        at[u] = ((size_t)(held ? id[u] : 0) * a.rows + r) * a.page.size + slot;
+        w[u] = held ? *reinterpret_cast<const uint2*>(a.codes + at[u] * a.hd + d[u]) : make_uint2(0u, 0u);
+        scale[u] = held ? a.scales[at[u]] : 0;
+        at[u] = ((size_t)t[u] * a.rows + r) * a.hd + d[u];
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        if (first + u * 256 >= a.runs) break;
+        const float s = kv8_scale(scale[u]);
+        float v[8];
+        kv8_unpack4(w[u].x, v);
+        kv8_unpack4(w[u].y, v + 4);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] *= s;
+        store8(out + at[u], v);
+    }
+}
+
+template <typename A>
+static cudaError_t launch_read(const Kv8ReadArgs& a, void* out, cudaStream_t s) {
+    // four runs a thread where they still give every SM two blocks (16,000 tokens' 16 rows of 128: 20.8 us, with a block
+    // a token 34.1); one where they are few (11 tokens' rows: 1.4 us)
+    const int blocks = (a.runs + 255) / 256;
+    if (blocks >= 8 * device_sm_count())
+        return mstar_launch((kv8_read_rows_kernel<A, 4>), dim3((blocks + 3) / 4), dim3(256), 0, s, a, (A*)out);
+    return mstar_launch((kv8_read_rows_kernel<A, 1>), dim3(blocks), dim3(256), 0, s, a, (A*)out);
 }
 
 // out [tokens, 2, nkv, hd]: the rows of the given tokens; zeros where the table has no page.  hd a multiple of 8.
@@ -217,16 +269,31 @@ MSTAR_API int mstar_kv8_read_rows(const void* codes, const void* scales, const i
     if (hd <= 0 || hd % 8 != 0 || nkv <= 0 || page_size <= 0 || pages <= 0 || ((uintptr_t)codes & 7) != 0 ||
         ((uintptr_t)out & 15) != 0)
         return -1;
+    const int per_row = hd / 8, rows = 2 * nkv;
     const cudaStream_t s = (cudaStream_t)stream;
-    cudaError_t e;
-    const PageSplit ps = page_split(page_size);
-    if (out_dtype == MSTAR_F32)
-        e = mstar_launch((kv8_read_rows_kernel<float>), dim3(tokens), dim3(256), 0, s, (const uint8_t*)codes,
-                         (const uint8_t*)scales, block_table, bt_stride, token_req, cache_pos, (float*)out,
-                         2 * nkv, hd, pages, ps);
-    else
-        e = mstar_launch((kv8_read_rows_kernel<bf16>), dim3(tokens), dim3(256), 0, s, (const uint8_t*)codes,
-                         (const uint8_t*)scales, block_table, bt_stride, token_req, cache_pos, (bf16*)out,
-                         2 * nkv, hd, pages, ps);
+    // runs are counted in 31 bits: several launches beyond that
+    const int most = (1 << 30) / (rows * per_row);
+    if (most < 1) return -1;
+    cudaError_t e = cudaSuccess;
+    for (long long t0 = 0; t0 < tokens && e == cudaSuccess; t0 += most) {
+        const int n = tokens - t0 < most ? (int)(tokens - t0) : most;
+        const Kv8ReadArgs a{(const uint8_t*)codes, (const uint8_t*)scales, block_table, token_req + t0, cache_pos + t0,
+                            bt_stride, rows, hd, pages, n * rows * per_row, page_split(page_size), page_split(per_row),
+                            page_split(rows * per_row)};
+        const size_t at = (size_t)t0 * rows * hd;
+        e = out_dtype == MSTAR_F32 ? launch_read<float>(a, (float*)out + at, s) : launch_read<bf16>(a, (bf16*)out + at, s);
+    }
     return e != cudaSuccess ? (int)e : launch_status();
+}
+
+MSTAR_API int mstar_rope_kv8_write_packed(const long long* a) {
+    return mstar_rope_kv8_write((const void*)a[0], (int)a[1], (int)a[2], (void*)a[3], (const int*)a[4],
+        (const int*)a[5], (const int*)a[6], (const int*)a[7], (int)a[8], (const float*)a[9], (void*)a[10],
+        (void*)a[11], (int)a[12], (int)a[13], (int)a[14], (int)a[15], (int)a[16], (int)a[17], (int)a[18], (int)a[19],
+        (void*)a[20]);
+}
+MSTAR_API int mstar_kv8_read_rows_packed(const long long* a) {
+    return mstar_kv8_read_rows((const void*)a[0], (const void*)a[1], (const int*)a[2], (int)a[3], (const int*)a[4],
+        (const int*)a[5], (void*)a[6], (int)a[7], (int)a[8], (int)a[9], (int)a[10], (int)a[11], (int)a[12],
+        (void*)a[13]);
 }

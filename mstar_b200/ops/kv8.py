@@ -16,13 +16,33 @@ The reference's caches hold the compute type only (mstar/engine/kv_cache_engine.
 """
 from __future__ import annotations
 
+from struct import Struct
+
 import torch
 
-from . import _DT, _dt, _error_ptr, _need_cuda, _ptr, _stream, lib, num_sms
+from . import _DT, _error_ptr, _need_cuda, _stream, lib, num_sms
 from .lib import KernelError, check
 
 KV8_DTYPE = torch.float8_e4m3fn
 _INT = torch.int32
+_F32, _BF16 = torch.float32, torch.bfloat16
+_device = torch._C._cuda_getDevice
+# the entry points' arguments as one string (csrc/kv8.cuh)
+_pack_write = Struct("=21q").pack
+_pack_read = Struct("=14q").pack
+_pack_float = Struct("=23qd4q").pack
+_pack_decode = Struct("=17qd3q").pack
+_pack_portions = Struct("=20qd5q").pack
+
+
+_sm_counts: dict = {}
+
+
+def _sms(device: int) -> int:
+    n = _sm_counts.get(device)
+    if n is None:
+        n = _sm_counts[device] = num_sms(torch.device("cuda", device))
+    return n
 
 
 def kv8_supported(head_dim: int) -> bool:
@@ -34,9 +54,10 @@ def _refuse(what: str, why: str) -> None:
     raise KernelError(f"{what}: {why}")
 
 
-def _check_cache(what, kv_cache, kv_scales, num_kv_heads, page_size, head_dim) -> None:
+def _check_cache(what, kv_cache, kv_scales, num_kv_heads, page_size, head_dim) -> int:
+    """The cache's pages."""
     shape = kv_cache.shape
-    if kv_cache.dtype != KV8_DTYPE or kv_scales.dtype != torch.uint8:
+    if kv_cache.dtype is not KV8_DTYPE or kv_scales.dtype is not torch.uint8:
         _refuse(what, f"the cache holds {KV8_DTYPE} codes and uint8 scales, got {kv_cache.dtype} and {kv_scales.dtype}")
     if len(shape) != 5 or shape[0] < 1 or shape[1:] != (2, num_kv_heads, page_size, head_dim):
         _refuse(what, f"the cache's shape {tuple(shape)} is not (pages, 2, {num_kv_heads}, {page_size}, {head_dim})")
@@ -44,27 +65,28 @@ def _check_cache(what, kv_cache, kv_scales, num_kv_heads, page_size, head_dim) -
         _refuse(what, f"the scales' shape {tuple(kv_scales.shape)} is not the cache's {tuple(shape[:4])}")
     if not (kv_cache.is_contiguous() and kv_scales.is_contiguous()):
         _refuse(what, "the cache and its scales must be contiguous")
-    if not kv8_supported(head_dim):
+    if head_dim % 8 or not 0 < head_dim <= 256:
         _refuse(what, f"head_dim {head_dim} is not a multiple of 8 up to 256")
+    return shape[0]
 
 
-def _check_index(what, block_table, *arrays) -> None:
-    """``arrays``: (tensor, least number of elements)."""
-    if block_table.dtype != _INT or block_table.dim() != 2 or block_table.stride(1) != 1:
+def _check_table(what, block_table) -> int:
+    """The distance of its rows."""
+    strides = block_table.stride()
+    if block_table.dtype is not _INT or len(strides) != 2 or strides[1] != 1 or strides[0] < 1:
         _refuse(what, "the block table is int32 [entries, pages], its rows without gaps")
-    for t, n in arrays:
-        if t.dtype != _INT or t.dim() != 1 or t.shape[0] < n or (n > 1 and t.stride(0) != 1):
-            _refuse(what, f"index arrays are int32 [at least {n}], got {t.dtype} {tuple(t.shape)}")
+    return strides[0]
 
 
-def _check_device(what, first, *others) -> None:
-    _need_cuda(first, *others)
-    device = first.get_device()
-    for t in others:
-        if t is not None and t.get_device() != device:
-            _refuse(what, "its tensors lie on different devices")
-    if device != torch._C._cuda_getDevice():
-        _refuse(what, f"its tensors lie on cuda:{device}, which is not the current device")
+def _check_index(what, t, n) -> None:
+    if t.dtype is not _INT or not t.is_contiguous() or t.numel() < n:
+        _refuse(what, f"index arrays are contiguous int32 [at least {n}], got {t.dtype} {tuple(t.shape)}")
+
+
+def _refuse_device(what, *tensors) -> None:
+    _need_cuda(*tensors)
+    _refuse(what, "its tensors lie on " + ", ".join(sorted({str(t.device) for t in tensors}))
+            + f", not all on the current device cuda:{_device()}")
 
 
 def rope_kv8_write(qkv: torch.Tensor, positions, cache_pos, token_req, block_table, inv_freq, kv_cache: torch.Tensor,
@@ -75,31 +97,42 @@ def rope_kv8_write(qkv: torch.Tensor, positions, cache_pos, token_req, block_tab
     tensor of their own (``qkv`` stays as it is).  ``inv_freq``: float [rotary_dim / 2], or None when
     rotary_dim == 0.  Two tokens of a call that name the same place of a request leave either's row."""
     what = "rope_kv8_write"
-    _dt(qkv)
-    if qkv.dim() != 2 or qkv.shape[1] != (num_heads + 2 * num_kv_heads) * head_dim or qkv.stride(1) != 1:
-        _refuse(what, f"qkv {tuple(qkv.shape)} is not [tokens, ({num_heads} + 2 * {num_kv_heads}) * {head_dim}] "
+    dtype = _DT.get(qkv.dtype)
+    if dtype is None:
+        _refuse(what, f"dtype {qkv.dtype} is not supported (float32 and bfloat16 are)")
+    shape, strides = qkv.shape, qkv.stride()
+    if len(shape) != 2 or shape[1] != (num_heads + 2 * num_kv_heads) * head_dim or strides[1] != 1:
+        _refuse(what, f"qkv {tuple(shape)} is not [tokens, ({num_heads} + 2 * {num_kv_heads}) * {head_dim}] "
                       "with rows without gaps")
     if num_heads < 1 or num_kv_heads < 1:
         _refuse(what, "there is at least one query head and one kv head")
     if rotary_dim % 2 or not 0 <= rotary_dim <= head_dim:
         _refuse(what, f"rotary_dim {rotary_dim} is not even and in [0, head_dim={head_dim}]")
-    _check_cache(what, kv_cache, kv_scales, num_kv_heads, page_size, head_dim)
-    if rotary_dim and (inv_freq is None or inv_freq.dtype != torch.float32 or inv_freq.numel() != rotary_dim // 2
-                       or not inv_freq.is_contiguous()):
-        _refuse(what, f"inv_freq is float32 [{rotary_dim // 2}]")
-    n = qkv.shape[0]
-    _check_index(what, block_table, (positions, n), (cache_pos, n), (token_req, n))
-    _check_device(what, qkv, positions, cache_pos, token_req, block_table, inv_freq if rotary_dim else None, kv_cache,
-                  kv_scales)
+    pages = _check_cache(what, kv_cache, kv_scales, num_kv_heads, page_size, head_dim)
+    n, freq = shape[0], 0
+    table = _check_table(what, block_table)
+    _check_index(what, positions, n)
+    _check_index(what, cache_pos, n)
+    _check_index(what, token_req, n)
+    device = qkv.get_device()
+    if rotary_dim:
+        if (inv_freq is None or inv_freq.dtype is not _F32 or inv_freq.numel() != rotary_dim // 2
+                or not inv_freq.is_contiguous()):
+            _refuse(what, f"inv_freq is float32 [{rotary_dim // 2}]")
+        if inv_freq.get_device() != device:
+            _refuse_device(what, qkv, inv_freq)
+        freq = inv_freq.data_ptr()
+    if device < 0 or not (
+            device == positions.get_device() == cache_pos.get_device() == token_req.get_device()
+            == block_table.get_device() == kv_cache.get_device() == kv_scales.get_device() == _device()):
+        _refuse_device(what, qkv, positions, cache_pos, token_req, block_table, kv_cache, kv_scales)
     q = qkv.new_empty((n, num_heads * head_dim))
     if n == 0:
         return q
-    code = lib.get("kv8_cache").mstar_rope_kv8_write(
-        qkv.data_ptr(), _DT[qkv.dtype], qkv.stride(0), q.data_ptr(), positions.data_ptr(), cache_pos.data_ptr(),
-        token_req.data_ptr(), block_table.data_ptr(), block_table.stride(0), _ptr(inv_freq if rotary_dim else None),
-        kv_cache.data_ptr(), kv_scales.data_ptr(), kv_cache.shape[0], n, num_heads, num_kv_heads, head_dim, rotary_dim,
-        int(interleaved), page_size, _stream())
-    check(code, what)
+    check(lib.get("kv8_cache").mstar_rope_kv8_write_packed(_pack_write(
+        qkv.data_ptr(), dtype, strides[0], q.data_ptr(), positions.data_ptr(), cache_pos.data_ptr(),
+        token_req.data_ptr(), block_table.data_ptr(), table, freq, kv_cache.data_ptr(), kv_scales.data_ptr(), pages, n,
+        num_heads, num_kv_heads, head_dim, rotary_dim, bool(interleaved), page_size, _stream())), what)
     return q
 
 
@@ -109,38 +142,47 @@ def kv8_read_rows(kv_cache: torch.Tensor, kv_scales: torch.Tensor, block_table, 
     ``dtype``: exactly what the cache holds.  Token t is place ``cache_pos[t]`` of request
     ``token_req[t]``; a place whose page the table does not have gives zeros."""
     what = "kv8_read_rows"
-    if dtype not in _DT:
+    out_type = _DT.get(dtype)
+    if out_type is None:
         _refuse(what, f"rows are read as float32 or bfloat16, not {dtype}")
     if kv_cache.dim() != 5:
         _refuse(what, f"the cache's shape {tuple(kv_cache.shape)} is not (pages, 2, kv_heads, page_size, head_dim)")
-    pages, _, heads, page_size, head_dim = kv_cache.shape
-    _check_cache(what, kv_cache, kv_scales, heads, page_size, head_dim)
-    n = token_req.shape[0]
-    _check_index(what, block_table, (token_req, n), (cache_pos, n))
-    _check_device(what, kv_cache, kv_scales, block_table, token_req, cache_pos)
-    out = torch.empty((n, 2, heads, head_dim), dtype=dtype, device=kv_cache.device)
+    _, _, heads, page_size, head_dim = kv_cache.shape
+    pages = _check_cache(what, kv_cache, kv_scales, heads, page_size, head_dim)
+    table, n = _check_table(what, block_table), token_req.numel()
+    _check_index(what, token_req, n)
+    _check_index(what, cache_pos, n)
+    device = kv_cache.get_device()
+    if device < 0 or not (
+            device == kv_scales.get_device() == block_table.get_device() == token_req.get_device()
+            == cache_pos.get_device() == _device()):
+        _refuse_device(what, kv_cache, kv_scales, block_table, token_req, cache_pos)
+    out = kv_scales.new_empty((n, 2, heads, head_dim), dtype=dtype)
     if n:
-        code = lib.get("kv8_cache").mstar_kv8_read_rows(
-            kv_cache.data_ptr(), kv_scales.data_ptr(), block_table.data_ptr(), block_table.stride(0),
-            token_req.data_ptr(), cache_pos.data_ptr(), out.data_ptr(), _DT[dtype], n, heads, head_dim, pages,
-            page_size, _stream())
-        check(code, what)
+        check(lib.get("kv8_cache").mstar_kv8_read_rows_packed(_pack_read(
+            kv_cache.data_ptr(), kv_scales.data_ptr(), block_table.data_ptr(), table, token_req.data_ptr(),
+            cache_pos.data_ptr(), out.data_ptr(), out_type, n, heads, head_dim, pages, page_size, _stream())), what)
     return out
 
 
-def _check_attention(what, q, out, rows, num_heads, num_kv_heads, head_dim, window, keep_first, scale) -> None:
+def _check_attention(what, q, out, rows, num_heads, num_kv_heads, head_dim, window, keep_first, scale) -> int:
+    """The distance of q's rows."""
     width = num_heads * head_dim
-    _dt(q)
+    if q.dtype is not _BF16 and q.dtype is not _F32:
+        _refuse(what, f"dtype {q.dtype} is not supported (float32 and bfloat16 are)")
     if num_kv_heads < 1 or num_heads < 1 or num_heads % num_kv_heads:
         _refuse(what, f"{num_heads} query heads are no multiple of {num_kv_heads} kv heads")
-    if q.dim() != 2 or q.shape[0] < rows or q.shape[1] < width or q.stride(1) != 1:
-        _refuse(what, f"q {tuple(q.shape)} is not [at least {rows}, at least {width}] with rows without gaps")
-    if out.dtype != q.dtype or out.dim() != 2 or out.shape[0] < rows or out.shape[1] != width or not out.is_contiguous():
-        _refuse(what, f"out is contiguous {q.dtype} [at least {rows}, {width}], got {out.dtype} {tuple(out.shape)}")
-    if window < 0 or keep_first < 0:
-        _refuse(what, f"window {window} and keep_first {keep_first} are not negative")
+    shape, strides = q.shape, q.stride()
+    if len(shape) != 2 or shape[0] < rows or shape[1] < width or strides[1] != 1:
+        _refuse(what, f"q {tuple(shape)} is not [at least {rows}, at least {width}] with rows without gaps")
+    shape = out.shape
+    if out.dtype is not q.dtype or len(shape) != 2 or shape[0] < rows or shape[1] != width or not out.is_contiguous():
+        _refuse(what, f"out is contiguous {q.dtype} [at least {rows}, {width}], got {out.dtype} {tuple(shape)}")
+    if not (0 <= window < 2 ** 31 and 0 <= keep_first < 2 ** 31):
+        _refuse(what, f"window {window} and keep_first {keep_first} are not negative, and fit 31 bits")
     if not scale > 0.0:
         _refuse(what, f"the scale {scale} is not positive")
+    return strides[0]
 
 
 def kv8_splits(blocks: int, max_keys: int, sms: int) -> int:
@@ -154,23 +196,23 @@ def _parts(q, tokens, num_heads, head_dim, splits) -> tuple:
     if splits == 1:
         return None, 0, 0
     rows = tokens * num_heads * splits
-    t = q.new_empty(rows * (head_dim + 2), dtype=torch.float32)
+    t = q.new_empty(rows * (head_dim + 2), dtype=_F32)
     return t, t.data_ptr(), t.data_ptr() + 4 * rows * head_dim
 
 
-def _float_attention(what, q, out, kv_cache, kv_scales, block_table, indptr, kv_len, req, pos, first_entry, count, max_q,
-                     max_keys, num_heads, num_kv_heads, head_dim, page_size, window, keep_first, scale) -> None:
+def _float_attention(what, q, q_stride, out, kv_cache, kv_scales, pages, block_table, table, indptr, kv_len, req, pos,
+                     first_entry, count, max_q, max_keys, num_heads, num_kv_heads, head_dim, page_size, window, keep_first,
+                     scale) -> None:
     """The kernel that takes every shape: portions by (indptr, kv_len), single tokens by (req, pos)."""
     rows = max_q * (num_heads // num_kv_heads)
     tiles = 1 if rows <= 8 else -(-rows // 64)
-    splits = kv8_splits(tiles * num_kv_heads * count, max_keys, num_sms(q.device))
+    splits = kv8_splits(tiles * num_kv_heads * count, max_keys, _sms(q.get_device()))
     tokens = min(out.shape[0], count * max_q)
     part, part_o, part_ml = _parts(q, tokens, num_heads, head_dim, splits)
-    check(lib.get("attention_kv8").mstar_kv8_attention(
-        q.data_ptr(), q.stride(0), out.data_ptr(), _DT[q.dtype], kv_cache.data_ptr(), kv_scales.data_ptr(),
-        kv_cache.shape[0], block_table.data_ptr(), block_table.stride(0), _ptr(indptr), _ptr(kv_len), _ptr(req), _ptr(pos),
-        first_entry, count, max_q, tokens, num_heads, num_kv_heads, head_dim, page_size, window, keep_first, scale,
-        splits, part_o, part_ml, _stream()), what)
+    check(lib.get("attention_kv8").mstar_kv8_attention_packed(_pack_float(
+        q.data_ptr(), q_stride, out.data_ptr(), _DT[q.dtype], kv_cache.data_ptr(), kv_scales.data_ptr(), pages,
+        block_table.data_ptr(), table, indptr, kv_len, req, pos, first_entry, count, max_q, tokens, num_heads,
+        num_kv_heads, head_dim, page_size, window, keep_first, scale, splits, part_o, part_ml, _stream())), what)
     if splits > 1:
         lib.add_launches(1)                     # the kernel that joins the parts
 
@@ -216,24 +258,31 @@ def paged_decode_attention_kv8(q: torch.Tensor, out: torch.Tensor, kv_cache: tor
     request (it decides how the work is cut, not what is computed).  A token at a place below 0 gives
     zeros."""
     what = "paged_decode_attention_kv8"
-    _check_attention(what, q, out, tokens, num_heads, num_kv_heads, head_dim, window, keep_first, scale)
-    _check_cache(what, kv_cache, kv_scales, num_kv_heads, page_size, head_dim)
-    _check_index(what, block_table, (token_req, tokens), (cache_pos, tokens))
-    _check_device(what, q, out, kv_cache, kv_scales, block_table, token_req, cache_pos)
+    q_stride = _check_attention(what, q, out, tokens, num_heads, num_kv_heads, head_dim, window, keep_first, scale)
+    pages = _check_cache(what, kv_cache, kv_scales, num_kv_heads, page_size, head_dim)
+    table = _check_table(what, block_table)
+    _check_index(what, token_req, tokens)
+    _check_index(what, cache_pos, tokens)
+    device = q.get_device()
+    if device < 0 or not (
+            device == out.get_device() == kv_cache.get_device() == kv_scales.get_device()
+            == block_table.get_device() == token_req.get_device() == cache_pos.get_device() == _device()):
+        _refuse_device(what, q, out, kv_cache, kv_scales, block_table, token_req, cache_pos)
     if tokens <= 0:
         return
-    if (q.dtype == torch.bfloat16 and head_dim in KV8_DECODE_HEAD_DIMS and page_size % 8 == 0
-            and q.stride(0) % 8 == 0 and (q.data_ptr() | kv_cache.data_ptr()) % 16 == 0 and kv_scales.data_ptr() % 8 == 0):
-        most = _most_keys(max_len, 1, window, keep_first)
+    most = _most_keys(max_len, 1, window, keep_first)
+    q_ptr, codes, scales = q.data_ptr(), kv_cache.data_ptr(), kv_scales.data_ptr()
+    if (q.dtype is _BF16 and head_dim in KV8_DECODE_HEAD_DIMS and page_size % 8 == 0 and q_stride % 8 == 0
+            and (q_ptr | codes) % 16 == 0 and scales % 8 == 0):
         pairs = tokens * num_kv_heads * -(-num_heads // num_kv_heads // 8)
-        blocks, warps = kv8_decode_shape(pairs, most, head_dim, num_sms(q.device))
-        check(lib.get("attention_kv8_decode").mstar_kv8_decode(
-            q.data_ptr(), q.stride(0), out.data_ptr(), kv_cache.data_ptr(), kv_scales.data_ptr(), kv_cache.shape[0],
-            block_table.data_ptr(), block_table.stride(0), token_req.data_ptr(), cache_pos.data_ptr(), tokens, num_heads,
-            num_kv_heads, head_dim, page_size, window, keep_first, scale, blocks, warps, _stream()), what)
+        blocks, warps = kv8_decode_shape(pairs, most, head_dim, _sms(device))
+        check(lib.get("attention_kv8_decode").mstar_kv8_decode_packed(_pack_decode(
+            q_ptr, q_stride, out.data_ptr(), codes, scales, pages, block_table.data_ptr(), table, token_req.data_ptr(),
+            cache_pos.data_ptr(), tokens, num_heads, num_kv_heads, head_dim, page_size, window, keep_first, scale, blocks,
+            warps, _stream())), what)
         return
-    _float_attention(what, q, out, kv_cache, kv_scales, block_table, None, None, token_req, cache_pos, 0, tokens, 1,
-                     _most_keys(max_len, 1, window, keep_first), num_heads, num_kv_heads, head_dim, page_size, window,
+    _float_attention(what, q, q_stride, out, kv_cache, kv_scales, pages, block_table, table, 0, 0, token_req.data_ptr(),
+                     cache_pos.data_ptr(), 0, tokens, 1, most, num_heads, num_kv_heads, head_dim, page_size, window,
                      keep_first, scale)
 
 
@@ -247,33 +296,40 @@ def paged_prefill_attention_kv8(q: torch.Tensor, out: torch.Tensor, kv_cache: to
     ``paged_decode_attention_kv8``).  ``max_q_len`` bounds the new tokens of these entries, ``max_kv_len``
     their keys.  Rows of other entries are left as they are."""
     what = "paged_prefill_attention_kv8"
-    _check_attention(what, q, out, 0, num_heads, num_kv_heads, head_dim, window, keep_first, scale)
-    _check_cache(what, kv_cache, kv_scales, num_kv_heads, page_size, head_dim)
-    if first_entry < 0 or q.shape[0] < out.shape[0]:
+    q_stride = _check_attention(what, q, out, 0, num_heads, num_kv_heads, head_dim, window, keep_first, scale)
+    pages = _check_cache(what, kv_cache, kv_scales, num_kv_heads, page_size, head_dim)
+    table, rows = _check_table(what, block_table), out.shape[0]
+    if first_entry < 0 or q.shape[0] < rows:
         _refuse(what, "first_entry is not negative, and q has a row for every row of out")
     last = first_entry + max(entries, 0)
     if block_table.shape[0] < last:
         _refuse(what, f"the block table has {block_table.shape[0]} rows and {last} entries are named")
-    _check_index(what, block_table, (qo_indptr, last + 1), (kv_len, last))
-    _check_device(what, q, out, kv_cache, kv_scales, block_table, qo_indptr, kv_len)
-    if entries <= 0 or max_q_len <= 0 or out.shape[0] == 0:
+    _check_index(what, qo_indptr, last + 1)
+    _check_index(what, kv_len, last)
+    device = q.get_device()
+    if device < 0 or not (
+            device == out.get_device() == kv_cache.get_device() == kv_scales.get_device()
+            == block_table.get_device() == qo_indptr.get_device() == kv_len.get_device() == _device()):
+        _refuse_device(what, q, out, kv_cache, kv_scales, block_table, qo_indptr, kv_len)
+    if entries <= 0 or max_q_len <= 0 or rows == 0:
         return
+    max_q_len = min(max_q_len, rows)
     group = num_heads // num_kv_heads
-    if (q.dtype == torch.bfloat16 and head_dim in KV8_TC_HEAD_DIMS and group <= 128 and q.stride(0) % 8 == 0
-            and (q.data_ptr() | kv_cache.data_ptr() | out.data_ptr()) % 16 == 0):
+    most = _most_keys(max_kv_len, max_q_len, window, keep_first)
+    q_ptr, out_ptr, codes = q.data_ptr(), out.data_ptr(), kv_cache.data_ptr()
+    if (q.dtype is _BF16 and head_dim in KV8_TC_HEAD_DIMS and group <= 128 and q_stride % 8 == 0
+            and (q_ptr | codes | out_ptr) % 16 == 0):
         tiles = -(-max_q_len // (2 * (128 // group)))
-        most = _most_keys(max_kv_len, max_q_len, window, keep_first)
-        splits = kv8_tc_splits(tiles * num_kv_heads * entries, most, num_sms(q.device))
-        tokens = min(out.shape[0], entries * max_q_len)
+        splits = kv8_tc_splits(tiles * num_kv_heads * entries, most, _sms(device))
+        tokens = min(rows, entries * max_q_len)
         part, part_o, part_ml = _parts(q, tokens, num_heads, head_dim, splits)
-        check(lib.get("attention_kv8_tc").mstar_kv8_attention_tc(
-            q.data_ptr(), q.stride(0), out.data_ptr(), kv_cache.data_ptr(), kv_scales.data_ptr(), kv_cache.shape[0],
-            block_table.data_ptr(), block_table.stride(0), qo_indptr.data_ptr(), kv_len.data_ptr(), first_entry, entries,
-            max_q_len, tokens, num_heads, num_kv_heads, head_dim, page_size, window, keep_first, scale, splits, part_o,
-            part_ml, _error_ptr(q), _stream()), what)
+        check(lib.get("attention_kv8_tc").mstar_kv8_attention_tc_packed(_pack_portions(
+            q_ptr, q_stride, out_ptr, codes, kv_scales.data_ptr(), pages, block_table.data_ptr(), table,
+            qo_indptr.data_ptr(), kv_len.data_ptr(), first_entry, entries, max_q_len, tokens, num_heads, num_kv_heads,
+            head_dim, page_size, window, keep_first, scale, splits, part_o, part_ml, _error_ptr(q), _stream())), what)
         if splits > 1:
             lib.add_launches(1)                 # the kernel that joins the parts
         return
-    _float_attention(what, q, out, kv_cache, kv_scales, block_table, qo_indptr, kv_len, None, None, first_entry, entries,
-                     max_q_len, _most_keys(max_kv_len, max_q_len, window, keep_first), num_heads, num_kv_heads, head_dim,
+    _float_attention(what, q, q_stride, out, kv_cache, kv_scales, pages, block_table, table, qo_indptr.data_ptr(),
+                     kv_len.data_ptr(), 0, 0, first_entry, entries, max_q_len, most, num_heads, num_kv_heads, head_dim,
                      page_size, window, keep_first, scale)

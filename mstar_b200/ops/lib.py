@@ -136,23 +136,11 @@ _SIGNATURES = {
         "mstar_paged_prefill_attention_tc": [_vp, _vp, _i, _i, _vp, _vp, _i, _vp, _vp, _i, _i, _i,
                                              _i, _i, _i, _i, _f, _vp, _vp],
     },
-    "kv8_cache": {
-        "mstar_rope_kv8_write": [_vp, _i, _i, _vp, _vp, _vp, _vp, _vp, _i, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i,
-                                 _i, _i, _vp],
-        "mstar_kv8_read_rows": [_vp, _vp, _vp, _i, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp],
-    },
-    "attention_kv8": {
-        "mstar_kv8_attention": [_vp, _i, _vp, _i, _vp, _vp, _i, _vp, _i, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i,
-                                _i, _i, _i, _i, _f, _i, _vp, _vp, _vp],
-    },
-    "attention_kv8_decode": {
-        "mstar_kv8_decode": [_vp, _i, _vp, _vp, _vp, _i, _vp, _i, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _f, _i, _i,
-                             _vp],
-    },
-    "attention_kv8_tc": {
-        "mstar_kv8_attention_tc": [_vp, _i, _vp, _vp, _vp, _i, _vp, _i, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _i, _i,
-                                   _f, _i, _vp, _vp, _vp, _vp],
-    },
+    # (arguments packed into one string of 64-bit numbers)
+    "kv8_cache": {"mstar_rope_kv8_write_packed": [_c.c_char_p], "mstar_kv8_read_rows_packed": [_c.c_char_p]},
+    "attention_kv8": {"mstar_kv8_attention_packed": [_c.c_char_p]},
+    "attention_kv8_decode": {"mstar_kv8_decode_packed": [_c.c_char_p]},
+    "attention_kv8_tc": {"mstar_kv8_attention_tc_packed": [_c.c_char_p]},
     "gemm_f32": {
         "mstar_sgemm_nt": [_vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp, _vp],
         "mstar_sgemm_parts": [_vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _vp, _vp],
