@@ -3,14 +3,23 @@
 //
 // One CTA owns two row tiles of 128 / G whole tokens each (G query heads per kv head; rows are (token, head) pairs) and
 // one kv head, and walks the keys that some of its rows see, 128 at a time.  Its sixteen warps:
-//   * 4 loader warps copy a tile's key codes into the tile that the MMAs read (cp.async), and read its value codes into
-//     registers (the next tile's loads are under way meanwhile), make bfloat16 of them and store the swizzled tile;
+//   * 3 warps find a tile's rows through the table (two tiles ahead), and copy its key codes into the tile that the MMAs
+//     read (cp.async);
+//   * 4 warps read its value codes into registers (the next tile's loads are under way meanwhile), make bfloat16 of them
+//     and store the swizzled tile;
 //   * one warp issues the products: S_A = Q_A K^T, S_B = Q_B K^T of the next tile as soon as a tile's weights have been
 //     used, and O_A += P_A V, O_B += P_B V as soon as weights are there, so that the tensor cores work for one row tile
 //     while the other one's softmax runs;
 //   * 4 + 4 softmax warps own a row a thread: they read it from tensor memory, keep the running maximum and sum in
 //     registers, and write the weights as bfloat16 over the scores (tcgen05.st); the output in tensor memory is rescaled
 //     only when a maximum grew by more than 2^8.
+// Where the portions have one row tile only and the keys are many, A and B are the same rows, A with the even and B with
+// the odd tiles of keys, and their outputs two parts to be joined: 1.6 us a tile instead of 2.5, for twice the parts.
+//
+// What else was built: two buffers of 64 keys a row tile in the same tensor memory, so that scores are made ahead (601 us
+// for 2,048 tokens on 14,336 keys; this 565: products of 64 keys read the queries from shared memory twice as often); the
+// same with two threads a row, which take its steps in turn (571: the exponentials are the same); half a row a thread
+// (754: the halves have to meet at every tile).
 // Tensor memory: S / P 2 x 128 columns, O 2 x head_dim.  Shared memory (head_dim 128): queries 64 KB, two stages of keys
 // of 16 KB and two of values of 32 KB each.
 //
@@ -58,11 +67,10 @@ struct Kv8TcArgs {
 
 __host__ __device__ constexpr int k8_codes(int hd) { return 128 * hd; }          // a tile of codes: 128 rows
 __host__ __device__ constexpr int k8_values(int hd) { return K8_KEYS * hd * 2; }
-// queries [2 row tiles][hi, lo], two stages of keys and of values, of four tiles each key's row, factor and value factor,
+// queries [2 row tiles][hi, lo], two stages of keys and of values, of eight tiles each key's row, factor and value factor,
 // the barriers
-__host__ __device__ constexpr int k8_smem(int hd) { return 6 * k8_codes(hd) + 2 * k8_values(hd) + 4 * 128 * 12 + 192; }
+__host__ __device__ constexpr int k8_smem(int hd) { return 6 * k8_codes(hd) + 2 * k8_values(hd) + 8 * 128 * 12 + 256; }
 
-__device__ __forceinline__ void k8_sync_loaders() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
 template <int R> __device__ __forceinline__ void k8_more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(R)); }
 template <int R> __device__ __forceinline__ void k8_less_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(R)); }
 // Instruction descriptors, D float: kind::f8f6f4 with e4m3 operands, kind::f16 with bfloat16 ones and an MN-major B.
@@ -135,6 +143,11 @@ __device__ __forceinline__ uint64_t k8_add2(uint64_t a, uint64_t b) {
 }
 __device__ __forceinline__ float k8_lo(uint64_t x) { return __uint_as_float((uint32_t)x); }
 __device__ __forceinline__ float k8_hi(uint64_t x) { return __uint_as_float((uint32_t)(x >> 32)); }
+__device__ __forceinline__ float k8_max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
 __device__ __forceinline__ uint32_t k8_mul_bf16x2(uint32_t a, uint32_t b) {
     uint32_t r;
     asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
@@ -148,45 +161,50 @@ __device__ __forceinline__ uint32_t k8_value_factors(int e) {
     return ((uint32_t)(min(120 + e, 127) + 127) << 7) | ((uint32_t)(max(e - 7, 0) + 127) << 23);
 }
 
-template <int HD>
+template <int HD, bool PAIR>
 __global__ void __launch_bounds__(K8_THREADS, 1) kv8_attention_tc_kernel(Kv8TcArgs a) {
     constexpr int QT = k8_codes(HD), KT = k8_codes(HD), VT = k8_values(HD);
     extern __shared__ __align__(1024) unsigned char smem[];
     unsigned char* q_s = smem;                       // [2 row tiles][hi, lo][128 rows x HD codes]
     unsigned char* k_s = q_s + 4 * QT;               // [2 stages][128 keys x HD codes]
     unsigned char* v_s = k_s + 2 * KT;               // [2 stages][HD / 64 blocks][128 keys x 128 bytes]
-    uint32_t* row_s = reinterpret_cast<uint32_t*>(v_s + 2 * VT);     // [4][128] rows of the cache
-    float* kf_s = reinterpret_cast<float*>(row_s + 512);             // [4][128] the keys' scales
-    uint32_t* vf_s = row_s + 1024;                                   // [4][128] the values' factors
-    uint64_t* bars = reinterpret_cast<uint64_t*>(vf_s + 512);
+    // what is told of eight tiles' keys: a place is taken again when the scores of the fifth tile after it are done, and
+    // with them, at the latest, the weights of its own
+    uint32_t* row_s = reinterpret_cast<uint32_t*>(v_s + 2 * VT);     // [8][128] rows of the cache
+    float* kf_s = reinterpret_cast<float*>(row_s + 1024);            // [8][128] the keys' scales
+    uint32_t* vf_s = row_s + 2048;                                   // [8][128] the values' factors
+    uint64_t* bars = reinterpret_cast<uint64_t*>(vf_s + 1024);
     const uint32_t k_full = tc_smem(bars), v_full = tc_smem(bars + 2), k_empty = tc_smem(bars + 4),
                    v_empty = tc_smem(bars + 6), s_full = tc_smem(bars + 8), p_ready = tc_smem(bars + 10),
-                   q_ready = tc_smem(bars + 12), o_full = tc_smem(bars + 14);
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 16);
+                   q_ready = tc_smem(bars + 12), o_full = tc_smem(bars + 14), rows_full = tc_smem(bars + 16);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 24);
 
     pdl_wait();
-    const int splits = a.parts.splits;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    // PAIR: one row tile, its even and odd key tiles side by side; `splits` ranges of keys, two parts each
+    const int splits = PAIR ? a.parts.splits >> 1 : a.parts.splits;
+    // (the exchange tells the compiler that a warp has one number: what follows from it need not be kept by every thread)
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
     const int kvh = blockIdx.x / splits, split = blockIdx.x % splits;
     const int e = a.first_entry + blockIdx.z;
     const int G = a.nq / a.nkv, TPT = K8_ROWS / G, RPT = TPT * G;
     const int q_start = a.qo_indptr[e], q_len = a.qo_indptr[e + 1] - q_start;
-    const int tok0 = (gridDim.y - 1 - blockIdx.y) * 2 * TPT;
+    const int tok0 = (gridDim.y - 1 - blockIdx.y) * (PAIR ? 1 : 2) * TPT;
     if (tok0 >= q_len) return;
     if ((tc_smem(smem) & 1023u) != 0) {              // the swizzled tiles need this alignment
         if (tid == 0) atomicExch(a.error_word, 31);
         return;
     }
     const int past = a.kv_len[e] - q_len;
-    const bool has_b = tok0 + TPT < q_len;
-    const int last_tok = min(tok0 + 2 * TPT, q_len) - 1;
+    const bool has_b = PAIR || tok0 + TPT < q_len;
+    const int last_tok = min(tok0 + (PAIR ? 1 : 2) * TPT, q_len) - 1;
     const SeenKeys seen = seen_keys(past + tok0, past + last_tok, a.window, a.keep_first);
     const int all_tiles = (seen.count + K8_KEYS - 1) / K8_KEYS;
     const int per_split = (all_tiles + splits - 1) / splits;
     const int tile0 = split * per_split, ntiles = max(0, min(all_tiles - tile0, per_split));
 
     if (tid == 0) {
-        for (int i = 0; i < 16; ++i) mbar_init(tc_smem(bars + i), i < 4 || (i >= 10 && i < 14) ? 128 : 1);
+        for (int i = 0; i < 24; ++i)
+            mbar_init(tc_smem(bars + i), i < 2 || i >= 16 ? 96 : i < 4 || i == 12 || i == 13 ? 128 : i == 10 || i == 11 ? 4 : 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 12) {
@@ -199,18 +217,105 @@ __global__ void __launch_bounds__(K8_THREADS, 1) kv8_attention_tc_kernel(Kv8TcAr
     pt_fence_after();
     const uint32_t tmem = *tmem_slot;
 
+    // what the loaders share: the keys of a tile by their place in it, and the table
+    const int* bt = a.block_table + (size_t)e * a.bt_stride;
+    const size_t plane = (size_t)a.nkv * a.page.size;
+    constexpr int CPR = HD / 16, RP = 128 / CPR;             // 16-byte runs a row, rows of a pass of 128 threads
     if (warp >= 12) {
-        // ------------------------------------------------------------------------------------- the products
-        // (the launch's 128 a thread, dealt out again: 2 x 184 + 80 + 64 = 2 x 184 + 88 + 56 = 512; no spills)
-        k8_less_registers<HD == 128 ? 64 : 56>();
-        if (warp == 12 && ntiles > 0) {
+        // (the launch's 128 a thread, dealt out again: 2 x 184 + 80 + 64 = 512)
+        k8_less_registers<64>();
+        if (warp > 12) {
+            // ------------------------------------------------------------------ rows, factors, keys
+            const int kt = tid - 13 * 32;                    // 96 threads; the first 32 have a second key of a tile
+            auto entry_of = [&](int j, int c) -> int {
+                const int key = key_of(seen, min((tile0 + j) * K8_KEYS + c, seen.count - 1));
+                return bt[min(page_of(a.page, key), a.bt_stride - 1)];
+            };
+            auto row_of = [&](int j, int c, int entry) -> uint32_t {
+                const int key = key_of(seen, min((tile0 + j) * K8_KEYS + c, seen.count - 1));
+                const int page = (int)min((unsigned)entry, (unsigned)(a.pages - 1));
+                return ((uint32_t)page * 2 * a.nkv + kvh) * a.page.size + (uint32_t)(key - page_of(a.page, key) * a.page.size);
+            };
+            auto keep = [&](int j, int c, uint32_t row, int kb, int vb) {
+                const int at = (j & 7) * 128 + c;
+                const bool bad = kb == KV8_BAD_BYTE || vb == KV8_BAD_BYTE;
+                row_s[at] = row;
+                kf_s[at] = bad ? __int_as_float(0x7fc00000) : kv8_scale(kb);
+                vf_s[at] = k8_value_factors(bad ? 0 : vb - 127);
+            };
+            const bool two = kt < 32;
+            // table entries are read two tiles ahead of their rows' use, scales one (a warp issues in order, and would
+            // stand still at the first use of what it just asked for)
+            int ea = 0, eb = 0, ka = 0, va = 0, kb = 0, vb = 0;
+            uint32_t ra = 0, rb = 0;
+            auto ask_rows = [&](int j) {
+                if (j >= ntiles) return;
+                ra = row_of(j, kt, ea);
+                ka = a.scales[ra];
+                va = a.scales[ra + plane];
+                if (two) {
+                    rb = row_of(j, kt + 96, eb);
+                    kb = a.scales[rb];
+                    vb = a.scales[rb + plane];
+                }
+            };
+            auto ask_entries = [&](int j) {
+                if (j >= ntiles) return;
+                ea = entry_of(j, kt);
+                if (two) eb = entry_of(j, kt + 96);
+            };
+            ask_entries(0);
+            ask_rows(0);
+            ask_entries(1);
+            bool ok = true;
+            for (int j = 0; j < ntiles && ok; ++j) {
+                const int s = j & 1;
+                keep(j, kt, ra, ka, va);
+                if (two) keep(j, kt + 96, rb, kb, vb);
+                mbar_arrive(rows_full + 8 * (j & 7));
+                ask_rows(j + 1);
+                ask_entries(j + 2);
+                // the tile's place is free when the scores of the tile before the last are done
+                if (!pt_wait_warp(rows_full + 8 * (j & 7), ((uint32_t)j >> 3) & 1u) ||
+                    !pt_wait_warp(k_empty + 8 * s, (((uint32_t)j >> 1) & 1u) ^ 1u)) {
+                    if (lane == 0) atomicExch(a.error_word, 33);
+                    ok = false;
+                    break;
+                }
+                const uint32_t tile = tc_smem(k_s + s * KT);
+                constexpr int N = (128 * CPR + 95) / 96;
+                uint32_t rows[N];
+#pragma unroll
+                for (int i = 0; i < N; ++i) rows[i] = row_s[(j & 7) * 128 + min(kt + i * 96, 128 * CPR - 1) / CPR];
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    const int at = kt + i * 96;
+                    if (at < 128 * CPR)
+                        cp_async_16(tile + k8_code_place<HD>(at / CPR, at % CPR), a.codes + (size_t)rows[i] * HD + at % CPR * 16, 16);
+                }
+                cp_async_commit();
+                if (j > 0) {
+                    cp_async_wait<1>();
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    mbar_arrive(k_full + 8 * (s ^ 1));
+                }
+                if (j + 1 == ntiles) {
+                    cp_async_wait<0>();
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    mbar_arrive(k_full + 8 * s);
+                }
+            }
+            cp_async_wait<0>();
+        } else if (ntiles > 0) {
+            // ------------------------------------------------------------------ the products
             constexpr uint32_t idesc_s = k8_idesc_codes(K8_ROWS, K8_KEYS), idesc_o = pt_idesc(K8_ROWS, HD, 1);
             const uint32_t leader = k8_elect();
             // low words: the address in units of 16 bytes (below 2^14 of them), the leading byte offset from bit 16 on
             const uint32_t q_low = tc_smem(q_s) >> 4 | 1u << 16, k_low = tc_smem(k_s) >> 4 | 1u << 16;
             const uint32_t v_low = tc_smem(v_s) >> 4 | (uint32_t)(K8_KEYS * 128 >> 4) << 16;
+            // row tile x with the keys of tile j; its weights with the values of tile j, `first` of its tiles
             auto scores = [&](int x, int j) {
-                const uint32_t qa = q_low + (uint32_t)(x * 2 * QT >> 4), ka = k_low + (uint32_t)((j & 1) * KT >> 4);
+                const uint32_t qa = q_low + (PAIR ? 0u : (uint32_t)(x * 2 * QT >> 4)), ka = k_low + (uint32_t)((j & 1) * KT >> 4);
 #pragma unroll
                 for (int part = 0; part < 2; ++part)
 #pragma unroll
@@ -219,101 +324,109 @@ __global__ void __launch_bounds__(K8_THREADS, 1) kv8_attention_tc_kernel(Kv8TcAr
                                      ka + (uint32_t)(kk * 32 >> 4), k8_codes_high<HD>(), idesc_s, (part | kk) != 0);
                 k8_commit(leader, s_full + 8 * x);
             };
-            auto output = [&](int x, int j) {
+            auto output = [&](int x, int j, bool first) {
                 const uint32_t va = v_low + (uint32_t)((j & 1) * VT >> 4);
 #pragma unroll
                 for (int kk = 0; kk < K8_KEYS / 16; ++kk)
                     k8_mma_weights(leader, tmem + 256 + x * HD, tmem + x * 128 + kk * 8, va + (uint32_t)(kk * 16 * 128 >> 4),
-                                   k8_values_high(), idesc_o, (j | kk) != 0);
+                                   k8_values_high(), idesc_o, !first || kk != 0);
             };
-            bool ok = pt_wait_warp(q_ready, 0) && (!has_b || pt_wait_warp(q_ready + 8, 0)) && pt_wait_warp(k_full, 0);
-            if (ok) {
-                pt_fence_after();
-                scores(0, 0);
-                if (has_b) scores(1, 0);
-                k8_commit(leader, k_empty);
-            }
-            for (int j = 0; j < ntiles && ok; ++j) {
-                const uint32_t ph = ((uint32_t)j >> 1) & 1u, ph1 = ((uint32_t)(j + 1) >> 1) & 1u;
-                const int s = j & 1, s1 = s ^ 1;
-                const bool more = j + 1 < ntiles;
-                ok = pt_wait_warp(v_full + 8 * s, ph) && pt_wait_warp(p_ready, (uint32_t)j & 1u);
-                if (!ok) break;
-                pt_fence_after();
-                output(0, j);
-                if (!has_b) k8_commit(leader, v_empty + 8 * s);
-                if (more) {
-                    ok = pt_wait_warp(k_full + 8 * s1, ph1);
-                    if (!ok) break;
+            bool ok = pt_wait_warp(q_ready, 0) && (PAIR || !has_b || pt_wait_warp(q_ready + 8, 0)) && pt_wait_warp(k_full, 0);
+            // a product that overwrites weights follows the one that reads them: one warp's products run in their order
+            if constexpr (PAIR) {
+                // tile j: row tile j & 1
+                if (ok) {
                     pt_fence_after();
-                    // (over the weights that the product before reads: one thread's products run in their order)
-                    scores(0, j + 1);
-                    if (!has_b) k8_commit(leader, k_empty + 8 * s1);
-                } else {
-                    k8_commit(leader, o_full);
+                    scores(0, 0);
+                    k8_commit(leader, k_empty);
+                    if (ntiles > 1) {
+                        ok = pt_wait_warp(k_full + 8, 0);
+                        pt_fence_after();
+                        if (ok) {
+                            scores(1, 1);
+                            k8_commit(leader, k_empty + 8);
+                        }
+                    }
                 }
-                if (has_b) {
-                    ok = pt_wait_warp(p_ready + 8, (uint32_t)j & 1u);
+                for (int j = 0; j < ntiles && ok; ++j) {
+                    const int s = j & 1;
+                    const uint32_t ph = ((uint32_t)j >> 1) & 1u;
+                    ok = pt_wait_warp(v_full + 8 * s, ph) && pt_wait_warp(p_ready + 8 * s, ph);
                     if (!ok) break;
                     pt_fence_after();
-                    output(1, j);
+                    output(s, j, j < 2);
                     k8_commit(leader, v_empty + 8 * s);
-                    if (more) {
-                        scores(1, j + 1);
-                        k8_commit(leader, k_empty + 8 * s1);
+                    if (j + 2 < ntiles) {
+                        ok = pt_wait_warp(k_full + 8 * s, ph ^ 1u);
+                        if (!ok) break;
+                        pt_fence_after();
+                        scores(s, j + 2);
+                        k8_commit(leader, k_empty + 8 * s);
                     } else {
-                        k8_commit(leader, o_full + 8);
+                        k8_commit(leader, o_full + 8 * s);
+                    }
+                }
+            } else {
+                if (ok) {
+                    pt_fence_after();
+                    scores(0, 0);
+                    if (has_b) scores(1, 0);
+                    k8_commit(leader, k_empty);
+                }
+                for (int j = 0; j < ntiles && ok; ++j) {
+                    const uint32_t ph = ((uint32_t)j >> 1) & 1u, ph1 = ((uint32_t)(j + 1) >> 1) & 1u;
+                    const int s = j & 1, s1 = s ^ 1;
+                    const bool more = j + 1 < ntiles;
+                    ok = pt_wait_warp(v_full + 8 * s, ph) && pt_wait_warp(p_ready, (uint32_t)j & 1u);
+                    if (!ok) break;
+                    pt_fence_after();
+                    output(0, j, j == 0);
+                    if (!has_b) k8_commit(leader, v_empty + 8 * s);
+                    if (more) {
+                        ok = pt_wait_warp(k_full + 8 * s1, ph1);
+                        if (!ok) break;
+                        pt_fence_after();
+                        scores(0, j + 1);
+                        if (!has_b) k8_commit(leader, k_empty + 8 * s1);
+                    } else {
+                        k8_commit(leader, o_full);
+                    }
+                    if (has_b) {
+                        ok = pt_wait_warp(p_ready + 8, (uint32_t)j & 1u);
+                        if (!ok) break;
+                        pt_fence_after();
+                        output(1, j, j == 0);
+                        k8_commit(leader, v_empty + 8 * s);
+                        if (more) {
+                            scores(1, j + 1);
+                            k8_commit(leader, k_empty + 8 * s1);
+                        } else {
+                            k8_commit(leader, o_full + 8);
+                        }
                     }
                 }
             }
             if (!ok && lane == 0) atomicExch(a.error_word, 32);
         }
     } else if (warp >= 8) {
-        // ---------------------------------------------------------------------- keys and values from the pages
-        k8_less_registers<HD == 128 ? 80 : 88>();
-        const int ct = tid - 256, w = ct >> 5;
-        const int* bt = a.block_table + (size_t)e * a.bt_stride;
-        const size_t plane = (size_t)a.nkv * a.page.size;
-        constexpr int CPR = HD / 16, NP = CPR, RP = 128 / CPR;   // 16-byte runs a row, passes, rows of a pass
+        // ---------------------------------------------------------------------- values
+        k8_less_registers<80>();
+        constexpr int NP = CPR;                              // passes
         // eight neighbouring lanes: two rows' four runs, whose stores then fall into different banks
         const int run = HD == 128 ? (lane & 3) | ((lane >> 1) & 4) : lane & 3;
         const int sub = HD == 128 ? ((lane >> 2) & 1) | ((lane >> 3) & 2) : lane >> 2;
-        const int r0 = w * (RP / 4) + sub;
-        auto key_at = [&](int j) { return key_of(seen, min((tile0 + j) * K8_KEYS + ct, seen.count - 1)); };
-        auto entry_of = [&](int j) -> int { return bt[min(page_of(a.page, key_at(j)), a.bt_stride - 1)]; };
-        auto row_of = [&](int j, int entry) -> uint32_t {
-            const int key = key_at(j), page = (int)min((unsigned)entry, (unsigned)(a.pages - 1));
-            return ((uint32_t)page * 2 * a.nkv + kvh) * a.page.size + (uint32_t)(key - page_of(a.page, key) * a.page.size);
-        };
-        // row and factors of tile j from this thread's key; four tiles' places, so that one barrier a tile will do
-        auto stage = [&](int j, uint32_t row, int kb, int vb) {
-            const int at = (j & 3) * 128 + ct;
-            const bool bad = kb == KV8_BAD_BYTE || vb == KV8_BAD_BYTE;
-            row_s[at] = row;
-            kf_s[at] = bad ? __int_as_float(0x7fc00000) : kv8_scale(kb);
-            vf_s[at] = k8_value_factors(bad ? 0 : vb - 127);
-            k8_sync_loaders();
-        };
-        auto copy_keys = [&](int j) {
-            const uint32_t tile = tc_smem(k_s + (j & 1) * KT);
-#pragma unroll
-            for (int i = 0; i < NP; ++i) {
-                const int r = i * RP + r0;
-                cp_async_16(tile + k8_code_place<HD>(r, run), a.codes + (size_t)row_s[(j & 3) * 128 + r] * HD + run * 16, 16);
-            }
-            cp_async_commit();
-        };
+        const int r0 = (warp - 8) * (RP / 4) + sub;
         auto load_values = [&](int j, uint4 (&x)[NP]) {
 #pragma unroll
             for (int i = 0; i < NP; ++i)
                 x[i] = *reinterpret_cast<const uint4*>(
-                    a.codes + ((size_t)row_s[(j & 3) * 128 + i * RP + r0] + plane) * HD + run * 16);
+                    a.codes + ((size_t)row_s[(j & 7) * 128 + i * RP + r0] + plane) * HD + run * 16);
         };
         auto store_values = [&](int j, const uint4 (&x)[NP]) {
 #pragma unroll
             for (int i = 0; i < NP; ++i) {
                 const int r = i * RP + r0, c = run * 2;
-                const uint32_t f = vf_s[(j & 3) * 128 + r], f1 = __byte_perm(f, f, 0x1010);
+                const uint32_t f = vf_s[(j & 7) * 128 + r], f1 = __byte_perm(f, f, 0x1010);
                 const uint32_t in[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
                 uint32_t out[8];
 #pragma unroll
@@ -333,66 +446,27 @@ __global__ void __launch_bounds__(K8_THREADS, 1) kv8_attention_tc_kernel(Kv8TcAr
         };
         if (ntiles > 0) {
             uint4 vx[NP];
-            bool ok = true;      // (a warp that gives up a wait goes on to meet the others at the loaders' barrier)
-            // table entries are read two tiles ahead of their rows' use, scales one
-            int entry = entry_of(0);
-            uint32_t row = row_of(0, entry);
-            int kb = a.scales[row], vb = a.scales[row + plane];
-            if (ntiles > 1) entry = entry_of(1);
-            stage(0, row, kb, vb);
-            copy_keys(0);
-            load_values(0, vx);
-            if (ntiles > 1) {
-                row = row_of(1, entry);
-                kb = a.scales[row];
-                vb = a.scales[row + plane];
-                if (ntiles > 2) entry = entry_of(2);
-            }
-            cp_async_wait<0>();
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            mbar_arrive(k_full);
-            for (int j = 0; j < ntiles; ++j) {
-                const int s = j & 1, s1 = s ^ 1;
-                const bool more = j + 1 < ntiles;
-                if (more) {
-                    stage(j + 1, row, kb, vb);
-                    // the tile's place is free when the scores of the tile before are done
-                    if (ok && !pt_wait_warp(k_empty + 8 * s1, (((uint32_t)(j + 1) >> 1) & 1u) ^ 1u)) {
-                        if (lane == 0) atomicExch(a.error_word, 33);
-                        ok = false;
-                    }
-                    if (ok) copy_keys(j + 1);
-                    if (j + 2 < ntiles) {
-                        row = row_of(j + 2, entry);
-                        kb = a.scales[row];
-                        vb = a.scales[row + plane];
-                        if (j + 3 < ntiles) entry = entry_of(j + 3);
-                    }
-                }
-                if (ok && !pt_wait_warp(v_empty + 8 * s, (((uint32_t)j >> 1) & 1u) ^ 1u)) {
-                    if (lane == 0) atomicExch(a.error_word, 34);
-                    ok = false;
-                }
-                if (ok) {
-                    store_values(j, vx);
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                    mbar_arrive(v_full + 8 * s);
-                }
-                if (more) {
-                    load_values(j + 1, vx);
-                    cp_async_wait<0>();
-                    if (ok) {
-                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                        mbar_arrive(k_full + 8 * s1);
-                    }
+            bool ok = pt_wait_warp(rows_full, 0);
+            if (ok) load_values(0, vx);
+            for (int j = 0; j < ntiles && ok; ++j) {
+                const int s = j & 1;
+                ok = pt_wait_warp(v_empty + 8 * s, (((uint32_t)j >> 1) & 1u) ^ 1u);
+                if (!ok) break;
+                store_values(j, vx);
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                mbar_arrive(v_full + 8 * s);
+                if (j + 1 < ntiles) {
+                    ok = pt_wait_warp(rows_full + 8 * ((j + 1) & 7), ((uint32_t)(j + 1) >> 3) & 1u);
+                    if (ok) load_values(j + 1, vx);
                 }
             }
+            if (!ok && lane == 0) atomicExch(a.error_word, 34);
         }
     } else {
         // ------------------------------------------------------------------------- softmax, a row a thread
         k8_more_registers<184>();
         const int x = warp >> 2, r = tid & 127;
-        const int tok = tok0 + x * TPT + min(r, RPT - 1) / G;
+        const int tok = tok0 + (PAIR ? 0 : x * TPT) + min(r, RPT - 1) / G;
         const bool valid = r < RPT && tok < q_len;
         const size_t head = (size_t)(q_start + min(tok, q_len - 1)) * a.nq + kvh * G + r % G;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
@@ -432,26 +506,29 @@ __global__ void __launch_bounds__(K8_THREADS, 1) kv8_attention_tc_kernel(Kv8TcAr
                         }
                     }
                     unsigned char* to = q_s + x * 2 * QT + k8_code_place<HD>(r, c);
+                    if (PAIR && x == 1) continue;                 // (the same rows as x = 0)
                     *reinterpret_cast<uint4*>(to) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
                     *reinterpret_cast<uint4*>(to + QT) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                mbar_arrive(q_ready + 8 * x);
+                if (!PAIR || x == 0) mbar_arrive(q_ready + 8 * x);
             }
             // in counts of seen keys: the newest key of this row and the newest one that its window has passed
             const int pos = past + min(tok, q_len - 1), shift = seen.kept - seen.lo;
             const int v_max = pos + shift, v_min = a.window > 0 ? pos - a.window + shift : -1;
             // of the tile's rows: the least v_max, the largest v_min
-            const int all_max = past + tok0 + x * TPT + shift;
-            const int all_min = a.window > 0 ? past + min(tok0 + x * TPT + TPT, q_len) - 1 - a.window + shift : -1;
-            for (int j = 0; j < ntiles; ++j) {
-                if (!pt_wait_warp(s_full + 8 * x, (uint32_t)j & 1u)) {
+            const int first_tok = tok0 + (PAIR ? 0 : x * TPT);
+            const int all_max = past + first_tok + shift;
+            const int all_min = a.window > 0 ? past + min(first_tok + TPT, q_len) - 1 - a.window + shift : -1;
+            constexpr int STEP = PAIR ? 2 : 1;
+            for (int j = PAIR ? x : 0; j < ntiles; j += STEP) {
+                if (!pt_wait_warp(s_full + 8 * x, (uint32_t)(j / STEP) & 1u)) {
                     if (lane == 0) atomicExch(a.error_word, 35);
                     ok = false;
                     break;
                 }
                 pt_fence_after();
-                const float4* kf = reinterpret_cast<const float4*>(kf_s + (j & 3) * 128);
+                const float4* kf = reinterpret_cast<const float4*>(kf_s + (j & 7) * 128);
                 const int v0 = (tile0 + j) * K8_KEYS;
                 uint64_t t[64];                         // scores times their key's scale, in pairs
                 {
@@ -513,7 +590,7 @@ __global__ void __launch_bounds__(K8_THREADS, 1) kv8_attention_tc_kernel(Kv8TcAr
                 }
                 const uint64_t both = k8_add2(sum[0], sum[1]);
                 l += k8_lo(both) + k8_hi(both);
-                if (j > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
+                if (j >= STEP && __any_sync(0xffffffffu, alpha != 1.f)) {
                     // (the scores came after the product before on the tensor cores: the output is at rest)
 #pragma unroll 1
                     for (int c0 = 0; c0 < HD; c0 += 32) {
@@ -529,23 +606,26 @@ __global__ void __launch_bounds__(K8_THREADS, 1) kv8_attention_tc_kernel(Kv8TcAr
                 pt_st32(t_s + 32, packed[1]);
                 pt_wait_st();
                 pt_fence_before();
-                mbar_arrive(p_ready + 8 * x);
+                __syncwarp();
+                if (lane == 0) mbar_arrive(p_ready + 8 * x);
             }
-            if (ntiles > 0 && ok && !pt_wait_warp(o_full + 8 * x, 0)) {
+            const bool some = PAIR ? ntiles > x : ntiles > 0;         // whether there is an output
+            if (some && ok && !pt_wait_warp(o_full + 8 * x, 0)) {
                 if (lane == 0) atomicExch(a.error_word, 36);
                 ok = false;
             }
             pt_fence_after();
             // ---------------------------------------------------------------- epilogue
             if (ok) {
-                const size_t at = (head - (size_t)kv8_first_token(a.parts) * a.nq) * splits + split;
-                const float f = splits > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l;
-                if (splits > 1 && valid) {
+                const bool parts = PAIR || splits > 1;
+                const size_t at = (head - (size_t)kv8_first_token(a.parts) * a.nq) * a.parts.splits + (PAIR ? 2 * split + x : split);
+                const float f = parts ? 1.f : l == 0.f ? 0.f : 1.f / l;
+                if (parts && valid) {
                     a.parts.ml[2 * at] = l == 0.f ? -INFINITY : m;
                     a.parts.ml[2 * at + 1] = l;
                 }
 #pragma unroll 1
-                for (int c0 = 0; c0 < HD && ntiles > 0; c0 += 32) {
+                for (int c0 = 0; c0 < HD && some; c0 += 32) {
                     uint32_t o[32];
                     pt_ld32(t_o + c0, o);
                     pt_wait_ld();
@@ -556,12 +636,12 @@ __global__ void __launch_bounds__(K8_THREADS, 1) kv8_attention_tc_kernel(Kv8TcAr
 #pragma unroll
                             for (int k = 0; k < 8; ++k)            // (places 1 and 2 of four hold features 2 and 1)
                                 v[k] = __uint_as_float(o[8 * i + ((k & 3) == 1 ? k + 1 : (k & 3) == 2 ? k - 1 : k)]) * f;
-                            if (splits > 1) store8(a.parts.o + at * HD + c0 + 8 * i, v);
+                            if (parts) store8(a.parts.o + at * HD + c0 + 8 * i, v);
                             else store8(a.out + head * HD + c0 + 8 * i, v);
                         }
                     }
                 }
-                if (ntiles == 0 && splits == 1 && valid) {       // rows that see nothing at all
+                if (!some && !parts && valid) {       // rows that see nothing at all
                     const float none[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
                     for (int c0 = 0; c0 < HD; c0 += 8) store8(a.out + head * HD + c0, none);
                 }
@@ -577,8 +657,8 @@ __global__ void __launch_bounds__(K8_THREADS, 1) kv8_attention_tc_kernel(Kv8TcAr
     }
 }
 
-template <int HD> static int launch_kv8_tc(const Kv8TcArgs& a, dim3 grid, cudaStream_t s) {
-    auto kernel = kv8_attention_tc_kernel<HD>;
+template <int HD, bool PAIR> static int launch_kv8_tc(const Kv8TcArgs& a, dim3 grid, cudaStream_t s) {
+    auto kernel = kv8_attention_tc_kernel<HD, PAIR>;
     // more than half of an SM's shared memory, so that no second CTA lands there and waits for tensor memory
     const int smem = k8_smem(HD) > 120 * 1024 ? k8_smem(HD) : 120 * 1024;
     static bool configured[64] = {false};
@@ -596,13 +676,14 @@ template <int HD> static int launch_kv8_tc(const Kv8TcArgs& a, dim3 grid, cudaSt
 }
 
 // Entries [first_entry, first_entry + count) of at most max_q tokens each.  q rows q_stride apart, 16-byte aligned.
-// `tokens`, `splits`, `part_o` and `part_ml` as in mstar_kv8_attention.  Returns 0, a CUDA error code or -1 (shape
+// `tokens`, `splits`, `part_o` and `part_ml` as in mstar_kv8_attention; `pair`: max_q is at most 128 / G, and a CTA takes
+// the even and the odd key tiles of its one row tile side by side and leaves two of the (an even number of) parts.  Returns 0, a CUDA error code or -1 (shape
 // refused).
 MSTAR_API int mstar_kv8_attention_tc(const void* q, int q_stride, void* out, const void* codes, const void* scales, int pages,
                                      const int* block_table, int bt_stride, const int* qo_indptr, const int* kv_len,
                                      int first_entry, int count, int max_q, int tokens, int nq, int nkv, int hd,
-                                     int page_size, int window, int keep_first, float scale, int splits, float* part_o,
-                                     float* part_ml, int* error_word, void* stream) {
+                                     int page_size, int window, int keep_first, float scale, int splits, int pair,
+                                     float* part_o, float* part_ml, int* error_word, void* stream) {
     if (count <= 0 || max_q <= 0) return 0;
     if ((hd != 64 && hd != 128) || nkv <= 0 || nq % nkv != 0 || nq / nkv > K8_ROWS || page_size <= 0 || pages <= 0 ||
         splits < 1 || count > 65535 || error_word == nullptr || !(scale > 0.f) || ((uintptr_t)q & 15) != 0 ||
@@ -613,12 +694,15 @@ MSTAR_API int mstar_kv8_attention_tc(const void* q, int q_stride, void* out, con
     const Kv8TcArgs a{(const bf16*)q, (bf16*)out, (const uint8_t*)codes, (const uint8_t*)scales, block_table, qo_indptr,
                       kv_len, q_stride, bt_stride, pages, nq, nkv, window, keep_first, first_entry,
                       scale * 1.4426950408889634f, page_split(page_size), parts, error_word};
-    const int per_cta = 2 * (K8_ROWS / (nq / nkv));
-    const long long tiles = ((long long)max_q + per_cta - 1) / per_cta;
+    const int per_tile = K8_ROWS / (nq / nkv);
+    if (pair && (max_q > per_tile || splits % 2 != 0)) return -1;
+    const long long tiles = pair ? 1 : ((long long)max_q + 2 * per_tile - 1) / (2 * per_tile);
     if (tiles > 65535) return -1;
-    const dim3 grid(nkv * splits, (unsigned)tiles, count);
+    const dim3 grid(nkv * (pair ? splits / 2 : splits), (unsigned)tiles, count);
     const cudaStream_t s = (cudaStream_t)stream;
-    const int code = hd == 64 ? launch_kv8_tc<64>(a, grid, s) : launch_kv8_tc<128>(a, grid, s);
+    int code;
+    if (pair) code = hd == 64 ? launch_kv8_tc<64, true>(a, grid, s) : launch_kv8_tc<128, true>(a, grid, s);
+    else code = hd == 64 ? launch_kv8_tc<64, false>(a, grid, s) : launch_kv8_tc<128, false>(a, grid, s);
     if (code != 0 || splits == 1) return code;
     return kv8_merge(parts, out, MSTAR_BF16, tokens, nq, hd, s);
 }
@@ -627,5 +711,5 @@ MSTAR_API int mstar_kv8_attention_tc_packed(const long long* a) {
     return mstar_kv8_attention_tc((const void*)a[0], (int)a[1], (void*)a[2], (const void*)a[3], (const void*)a[4],
         (int)a[5], (const int*)a[6], (int)a[7], (const int*)a[8], (const int*)a[9], (int)a[10], (int)a[11],
         (int)a[12], (int)a[13], (int)a[14], (int)a[15], (int)a[16], (int)a[17], (int)a[18], (int)a[19],
-        kv8_packed_float(a[20]), (int)a[21], (float*)a[22], (float*)a[23], (int*)a[24], (void*)a[25]);
+        kv8_packed_float(a[20]), (int)a[21], (int)a[22], (float*)a[23], (float*)a[24], (int*)a[25], (void*)a[26]);
 }

@@ -32,7 +32,7 @@ _pack_write = Struct("=21q").pack
 _pack_read = Struct("=14q").pack
 _pack_float = Struct("=23qd4q").pack
 _pack_decode = Struct("=17qd3q").pack
-_pack_portions = Struct("=20qd5q").pack
+_pack_portions = Struct("=20qd6q").pack
 
 
 _sm_counts: dict = {}
@@ -236,10 +236,14 @@ def kv8_decode_shape(pairs: int, max_keys: int, head_dim: int, sms: int) -> tupl
 KV8_TC_HEAD_DIMS = (64, 128)
 
 
-def kv8_tc_splits(blocks: int, max_keys: int, sms: int) -> int:
-    """Ranges that the keys of ``blocks`` pairs of row tiles are cut into in the tensor-core kernel: a block
-    an SM, ranges of at least two tiles of 128 keys, at most 64."""
-    return max(1, min(64, sms // max(blocks, 1), -(-max_keys // 256)))
+def kv8_tc_splits(blocks: int, max_keys: int, sms: int, one_tile: bool) -> tuple:
+    """(parts that the keys of ``blocks`` blocks of row tiles are cut into in the tensor-core kernel, whether a
+    block makes two of them): a block an SM, at least two tiles of 128 keys each, at most 64 parts.  With
+    one row tile a block takes two key tiles side by side from ten tiles on: two portions of 17 tokens on
+    20,000 / 10,000 / 5,000 keys took 49.7 / 35.2 / 26.9 us so, and 56.3 / 34.8 / 23.9 one after another."""
+    ranges = max(1, min(32, sms // max(blocks, 1), -(-max_keys // 256)))
+    pair = one_tile and max_keys >= ranges * 1280
+    return (2 * ranges if pair else ranges), pair
 
 
 def _most_keys(max_len, max_q, window, keep_first) -> int:
@@ -319,14 +323,16 @@ def paged_prefill_attention_kv8(q: torch.Tensor, out: torch.Tensor, kv_cache: to
     q_ptr, out_ptr, codes = q.data_ptr(), out.data_ptr(), kv_cache.data_ptr()
     if (q.dtype is _BF16 and head_dim in KV8_TC_HEAD_DIMS and group <= 128 and q_stride % 8 == 0
             and (q_ptr | codes | out_ptr) % 16 == 0):
-        tiles = -(-max_q_len // (2 * (128 // group)))
-        splits = kv8_tc_splits(tiles * num_kv_heads * entries, most, _sms(device))
+        per_tile = 128 // group
+        tiles = -(-max_q_len // (2 * per_tile))
+        splits, pair = kv8_tc_splits(tiles * num_kv_heads * entries, most, _sms(device), max_q_len <= per_tile)
         tokens = min(rows, entries * max_q_len)
         part, part_o, part_ml = _parts(q, tokens, num_heads, head_dim, splits)
         check(lib.get("attention_kv8_tc").mstar_kv8_attention_tc_packed(_pack_portions(
             q_ptr, q_stride, out_ptr, codes, kv_scales.data_ptr(), pages, block_table.data_ptr(), table,
             qo_indptr.data_ptr(), kv_len.data_ptr(), first_entry, entries, max_q_len, tokens, num_heads, num_kv_heads,
-            head_dim, page_size, window, keep_first, scale, splits, part_o, part_ml, _error_ptr(q), _stream())), what)
+            head_dim, page_size, window, keep_first, scale, splits, pair, part_o, part_ml, _error_ptr(q),
+            _stream())), what)
         if splits > 1:
             lib.add_launches(1)                 # the kernel that joins the parts
         return

@@ -193,6 +193,18 @@ def test_one_long_request(act, hd):
     c.check(c.prefill())
 
 
+@pytest.mark.parametrize("hd,window,keep", [(64, 0, 0), (128, 0, 0), (64, 1400, 2)])
+def test_few_rows_on_many_keys_side_by_side(hd, window, keep):
+    """Portions of one row tile in so many requests that a block walks ten key tiles and more: two at a time."""
+    from mstar_b200 import ops
+    from mstar_b200.ops.kv8 import kv8_tc_splits
+
+    lens_q, lens_kv = [3] * 19, [3, 4, 60, 128, 129, 256, 257, 1500] + [70] * 11
+    assert kv8_tc_splits(8 * 19, 1500, ops.num_sms(), True) == (2, True)
+    c = Case(lens_q, lens_kv, 8, 8, hd, 16, BF16, seed=17, window=window, keep=keep)
+    c.check(c.prefill(max_len=1500))
+
+
 @pytest.mark.parametrize("act", [F32, BF16])
 @pytest.mark.parametrize("hd", [64, 128])
 def test_bounds_only_cut_the_work(act, hd):
