@@ -22,49 +22,28 @@ struct Kv8WriteArgs {
     PageSplit page;
 };
 
-// 8 of a row as they are loaded: one or two 16-byte words
-template <typename A> struct Run8 { uint4 w[sizeof(A) / 2]; };
-__device__ __forceinline__ void numbers(const Run8<bf16>& r, float (&x)[8]) {
-    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&r);
+// 8 of row[d ..] as floats; V: the row is aligned to 8 elements
+template <bool V, typename A> __device__ __forceinline__ void take8(const A* p, float (&x)[8]) {
+    if constexpr (V) {
+        load8(p, x);
+    } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float2 f = __bfloat1622float2(h[i]);
-        x[2 * i] = f.x;
-        x[2 * i + 1] = f.y;
+        for (int i = 0; i < 8; ++i) x[i] = to_float(p[i]);
     }
-}
-__device__ __forceinline__ void numbers(const Run8<float>& r, float (&x)[8]) {
-    const float* f = reinterpret_cast<const float*>(&r);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = f[i];
 }
 
 // R: the type of the rotation, float or double
 __device__ __forceinline__ void half_turns(float t, float* sn, float* cs) { sincospif(t, sn, cs); }
 __device__ __forceinline__ void half_turns(double t, double* sn, double* cs) { sincospi(t, sn, cs); }
 
-// L: threads of a head, a power of two with 8 L >= hd.  V: pairs, halves and rows in whole aligned groups of 8; the
-// loads of a thread's next head then go before the work on this one, those of its first before the angles.
+// L: threads of a head, a power of two with 8 L >= hd.  V: pairs, halves and rows in whole aligned groups of 8.
 template <typename A, typename R, int L, bool V>
-__global__ void __launch_bounds__(256) rope_kv8_write_kernel(const A* qkv, A* q_out, Kv8WriteArgs a) {
+__global__ void __launch_bounds__(256) rope_kv8_write_kernel(const A* __restrict__ qkv, A* __restrict__ q_out,
+                                                             Kv8WriteArgs a) {
     pdl_launch_dependents();   // a short kernel: the long one after it may be scheduled now
-    pdl_wait();
+    qkv = pdl_after(qkv, pdl_wait());
     __shared__ R tab_sn[128], tab_cs[128];
-    constexpr int PER = 256 / L;
     const int t = blockIdx.x, hd = a.hd, half = a.rot >> 1;
-    const int l = threadIdx.x % L, d0 = l * 8, heads = a.nq + 2 * a.nkv, step = gridDim.y * PER;
-    const bool in = d0 < hd, turned = d0 < a.rot, upper = d0 >= half;
-    const A* row = qkv + (size_t)t * a.in_stride;
-    Run8<A> own, other;
-    auto load = [&](int h) {
-        if (V && in && h < heads) {
-            own = *reinterpret_cast<const Run8<A>*>(row + (size_t)h * hd + d0);
-            if (turned && h < a.nq + a.nkv && !a.interleaved)
-                other = *reinterpret_cast<const Run8<A>*>(row + (size_t)h * hd + (upper ? d0 - half : d0 + half));
-        }
-    };
-    const int h0 = blockIdx.y * PER + threadIdx.x / L;
-    load(h0);
     for (int j = threadIdx.x; j < half; j += blockDim.x) {
         double turns = (double)a.positions[t] * (double)a.inv_freq[j] * 0.31830988618379067154;   // half-turns
         turns -= 2.0 * rint(0.5 * turns);
@@ -77,22 +56,19 @@ __global__ void __launch_bounds__(256) rope_kv8_write_kernel(const A* qkv, A* q_
     const int slot = held ? cp - logical * a.page.size : 0;
     __syncthreads();
 
-    for (int h = h0; h < heads; h += step) {
+    constexpr int PER = 256 / L;
+    const int l = threadIdx.x % L, d0 = l * 8;
+    const bool in = d0 < hd;
+    const int heads = a.nq + 2 * a.nkv;
+    const A* row = qkv + (size_t)t * a.in_stride;
+    for (int h = blockIdx.y * PER + threadIdx.x / L; h < heads; h += gridDim.y * PER) {
         float y[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) y[i] = 0.f;
         if (in) {
             const A* src = row + (size_t)h * hd;
-            float z[8];
-            if constexpr (V) {
-                numbers(own, y);
-                numbers(other, z);
-                load(h + step);
-            } else {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) y[i] = to_float(src[d0 + i]);
-            }
-            if (h < a.nq + a.nkv && turned) {
+            take8<V>(src + d0, y);
+            if (h < a.nq + a.nkv && d0 < a.rot) {
                 if (V && a.interleaved) {
 #pragma unroll
                     for (int i = 0; i < 8; i += 2) {
@@ -102,7 +78,10 @@ __global__ void __launch_bounds__(256) rope_kv8_write_kernel(const A* qkv, A* q_
                         y[i + 1] = (float)(x1 * cs + x0 * sn);
                     }
                 } else if (V) {
+                    const bool upper = d0 >= half;
                     const int j0 = upper ? d0 - half : d0;
+                    float z[8];
+                    take8<V>(src + (upper ? d0 - half : d0 + half), z);
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
                         const R sn = upper ? tab_sn[j0 + i] : -tab_sn[j0 + i];
@@ -112,11 +91,11 @@ __global__ void __launch_bounds__(256) rope_kv8_write_kernel(const A* qkv, A* q_
                     for (int i = 0; i < 8; ++i) {
                         const int d = d0 + i;
                         if (d >= a.rot) break;
-                        const bool second = a.interleaved ? (d & 1) : d >= half;
-                        const int j = a.interleaved ? d >> 1 : second ? d - half : d;
-                        const int pair = a.interleaved ? d ^ 1 : second ? d - half : d + half;
-                        const R sn = second ? tab_sn[j] : -tab_sn[j];
-                        y[i] = (float)((R)y[i] * tab_cs[j] + (R)to_float(src[pair]) * sn);
+                        const bool upper = a.interleaved ? (d & 1) : d >= half;
+                        const int j = a.interleaved ? d >> 1 : upper ? d - half : d;
+                        const int other = a.interleaved ? d ^ 1 : upper ? d - half : d + half;
+                        const R sn = upper ? tab_sn[j] : -tab_sn[j];
+                        y[i] = (float)((R)y[i] * tab_cs[j] + (R)to_float(src[other]) * sn);
                     }
                 }
             }
