@@ -1,16 +1,19 @@
-// Grouped-query attention over the 8-bit cache (format: kv8.cuh) in float arithmetic on CUDA cores: prompt portions
-// and single tokens, both activation types, any head size that is a multiple of 8 up to 256, any group of query
-// heads, any page size.  It is the attention of the 32-bit mode and of the shapes that the tensor-core kernels do not
-// take.
+// Grouped-query attention over the 8-bit cache (format: kv8.cuh) for the 32-bit mode and for what the other kernels do not
+// take: prompt portions and single tokens, both activation types, any group of query heads, any page size.  Two kernels:
+// head sizes 64, 128 and 256 on the tensor cores (second half of this file), others that are multiples of 8 up to 256 in
+// float arithmetic on CUDA cores.
 //
-// A row is (token, query head of the group); R rows of one request and kv head make a block, which walks the keys
+// On CUDA cores: a row is (token, query head of the group); R rows of one request and kv head make a block, which walks the keys
 // that some of its rows see (kept first keys, then the window) in tiles of 64: codes become floats times their row's
 // scale in shared memory (keys transposed), S = Q K^T and O += P V by outer products in registers, softmax statistics
 // per row in registers.  R = 64 for portions (4 x 4 scores a thread), 8 for single tokens (a warp a row).  Where there
 // are few row tiles the keys are cut into `splits` parts whose (maximum, sum, output) go to scratch memory.
 //
 // Semantics are those of attention_generic.cu; a row that sees no key gives zeros.
+#include <cuda_fp16.h>
+
 #include "kv8_merge.cuh"
+#include "mma_util.cuh"
 
 struct Kv8AttnArgs {
     const void* q;
@@ -201,7 +204,7 @@ __global__ void __launch_bounds__(256) kv8_attention_kernel(Kv8AttnArgs a) {
 #pragma unroll
             for (int c = 0; c < DT; ++c)
                 if (tx + c * TX < hd) ((A*)a.out)[head * hd + tx + c * TX] = from_float<A>(acc[r][c] * inv);
-        } else {
+        } else if (kv8_has_room(a.parts, first_token + row / G)) {
             const size_t at = (head - (size_t)kv8_first_token(a.parts) * a.nq) * a.parts.splits + split;
 #pragma unroll
             for (int c = 0; c < DT; ++c)
@@ -217,20 +220,447 @@ __global__ void __launch_bounds__(256) kv8_attention_kernel(Kv8AttnArgs a) {
 template <typename A, int R> static int launch_simt(const Kv8AttnArgs& a, dim3 grid, cudaStream_t s) {
     const int smem = (a.hd * (R + 4) + a.hd * 68 + 64 * (R + 4)) * (int)sizeof(float);
     auto kernel = kv8_attention_kernel<A, R>;
-    static int configured = 0;
-    if (smem > configured) {
-        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 224 * 1024);
+    static bool configured[64] = {false};
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return (int)e;
+    if (dev < 0 || dev >= 64) return -1;
+    if (!configured[dev]) {
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 224 * 1024);
         if (e != cudaSuccess) return (int)e;
-        configured = 224 * 1024;
+        configured[dev] = true;
     }
-    const cudaError_t e = mstar_launch(kernel, grid, dim3(256), (size_t)smem, s, a);
+    e = mstar_launch(kernel, grid, dim3(256), (size_t)smem, s, a);
     return e != cudaSuccess ? (int)e : launch_status();
+}
+
+// ---------------------------------------------------------------------------------------- on the tensor cores
+// m16n8k16 products of float16 with float sums.  e4m3 is exact in float16, so the codes of keys and values are converted
+// in registers, and only queries and weights are rounded: in the 32-bit mode (PARTS 2) each is two float16, x = hi + lo,
+// 22 bits, with a product each.  A row of queries is first scaled by a power of two to have its largest number in [2^13,
+// 2^14), so that the parts are not subnormal.  The rows' scales are put on the scores as in attention_kv8_decode.cu: the
+// values' weights are 2^(s_j + e_j - m'), in [0, 2^8], with a maximum of their own.
+//
+// A warp owns 16 rows (token, query head of the group) and, of every tile of 64 keys, 8 NT: with NT 8 a block's four
+// warps have 64 rows, with NT 2 (16 rows or fewer) they share a tile's keys and leave a part each.  Tiles of codes come by
+// cp.async, one tile ahead (three with few rows), into swizzled shared memory; which features and keys the fragments'
+// elements are is chosen as in the decode kernel, and the queries lie in shared memory in that order.
+//
+// Bound by instructions: about 1,000 of a warp for a tile of 64 keys of 64 features in the 32-bit mode, of which the
+// products fill the tensor pipe for 800 of some 1,600 clocks.  Two portions of 251 tokens, 32 heads of 64 over 8, a window
+// of 200 take 15.8 us (on CUDA cores 108), two of 512 on 6,000 cached 327 us (123 TFLOP/s, half of what the pipe does);
+// single tokens of 8 requests on 2,048 keys 18 us.
+__device__ __forceinline__ uint32_t f16x2_of_codes(uint32_t two) {
+    uint32_t r;
+    asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t}" : "=r"(r) : "r"(two));
+    return r;
+}
+__device__ __forceinline__ uint32_t f16x2_of_codes_hi(uint32_t two) {
+    uint32_t r;
+    asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, hi;\n\t}" : "=r"(r) : "r"(two));
+    return r;
+}
+__device__ __forceinline__ void mma_f16_16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ float exp2_approx(float x) {
+    float y;
+    asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t f16x2(float lo, float hi) {
+    const __half2 v = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ float2 floats_of(uint32_t two) { return __half22float2(*reinterpret_cast<const __half2*>(&two)); }
+
+#define KM_SLACK 8.f
+template <int HD> __host__ __device__ constexpr int km_tile() { return 64 * HD; }
+// tiles of which a block holds copies, on the way or there: with few rows a tile is soon worked off
+template <int NT> __host__ __device__ constexpr int km_stages() { return NT == 8 ? 2 : 4; }
+template <int HD, int PARTS, int NT> __host__ __device__ constexpr int km_smem() {
+    return km_stages<NT>() * (2 * km_tile<HD>() + 64 * 12) + PARTS * (NT == 8 ? 64 : 16) * (HD * 2 + 16) + 64 * 4;
+}
+
+template <typename A, int HD, int PARTS, int NT>
+__global__ void __launch_bounds__(128) kv8_attention_mma_kernel(Kv8AttnArgs a) {
+    constexpr int ROWS = NT == 8 ? 64 : 16, RB = HD < 128 ? HD : 128, KC = HD / 64, VW = HD / 32, MT = HD / 8, NB = NT < 4 ? NT : 4;
+    constexpr int QP = HD * 2 + 16;                      // bytes of a row of queries in shared memory
+    constexpr int S = km_stages<NT>();
+    extern __shared__ __align__(128) unsigned char smem_m[];
+    unsigned char* k_s = smem_m;                         // [S][64 keys x HD codes], then values
+    unsigned char* v_s = k_s + S * km_tile<HD>();
+    unsigned char* q_s = v_s + S * km_tile<HD>();        // [PARTS][ROWS][QP]
+    float2* sc_s = reinterpret_cast<float2*>(q_s + PARTS * ROWS * QP);     // [S][64] 2^e of the key, e of the value
+    uint32_t* row_s = reinterpret_cast<uint32_t*>(sc_s + S * 64);         // [S][64]
+    float* qscale_s = reinterpret_cast<float*>(row_s + S * 64);           // [ROWS]
+    pdl_wait();
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3, G = a.nq / a.nkv;
+    const int ranges = NT == 8 ? a.parts.splits : max(1, a.parts.splits / 4);      // ranges of keys; a part a warp, or one
+    const int kvh = blockIdx.x / ranges, range = blockIdx.x % ranges;
+    int first_token, q_len, past, table_row;
+    if (a.token_req != nullptr) {
+        first_token = blockIdx.z;
+        q_len = 1;
+        past = a.cache_pos[first_token];
+        table_row = a.token_req[first_token];
+    } else {
+        table_row = a.first_entry + blockIdx.z;
+        first_token = a.qo_indptr[table_row];
+        q_len = a.qo_indptr[table_row + 1] - first_token;
+        past = a.kv_len[table_row] - q_len;
+    }
+    const int row0 = blockIdx.y * ROWS, rows = q_len * G;
+    if (row0 >= rows) return;
+    const int last_row = min(row0 + ROWS, rows) - 1;
+    const int* bt = a.block_table + (size_t)table_row * a.bt_stride;
+    const SeenKeys seen = seen_keys(past + row0 / G, past + last_row / G, a.window, a.keep_first);
+    const int all = (seen.count + 63) >> 6, per = (all + ranges - 1) / ranges;
+    const int tile0 = range * per, tiles = max(0, min(per, all - tile0));
+    const size_t plane = (size_t)a.nkv * a.page.size;
+
+    // ---- queries: LR lanes a row, four features a lane and load, NQ loads a turn.  The first turn's go before all else.
+    constexpr int LR = HD < 128 ? HD / 4 : 32, NL = HD / 4 / LR, NQ = NT == 8 ? 8 : 4 * NL * LR / 32;
+    constexpr int RT = NQ / NL * (32 / LR), TURNS = ROWS / 4 / RT;           // rows of a turn of a warp
+    const bool wide = a.q_stride % 4 == 0 && ((uintptr_t)a.q & 15) == 0;
+    float qv[NQ][4];
+    auto q_row = [&](int turn, int i) { return warp * (ROWS / 4) + turn * RT + i / NL * (32 / LR) + lane / LR; };
+    auto q_feature = [&](int i) { return i % NL * 128 + lane % LR * 4; };
+    auto load_q = [&](int turn) {
+#pragma unroll
+        for (int i = 0; i < NQ; ++i) {
+            const int row = row0 + q_row(turn, i);
+            const A* q = (const A*)a.q + (size_t)(first_token + min(row, last_row) / G) * a.q_stride +
+                         (size_t)(kvh * G + min(row, last_row) % G) * HD + q_feature(i);
+            if (wide) {
+                load4(q, qv[i]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) qv[i][j] = to_float(q[j]);
+            }
+        }
+    };
+    // row r's feature d at the place that the fragments want: of 64 features, 16 t + 4 s + e is k-step s, element
+    // 2 t + e % 2 + 8 (e / 2)
+    auto keep_q = [&](int turn) {
+#pragma unroll
+        for (int i0 = 0; i0 < NQ; i0 += NL) {
+            float most = 0.f;
+#pragma unroll
+            for (int i = i0; i < i0 + NL; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) most = fabsf(qv[i][j]) < INFINITY ? fmaxf(most, fabsf(qv[i][j])) : INFINITY;
+#pragma unroll
+            for (int o = LR / 2; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+            // (one below 2^-113 is taken as that large, so that the factors are normal numbers)
+            const uint32_t e = max(__float_as_uint(most) >> 23, 14u);
+            const float down = e < 255u ? __uint_as_float((267u - e) << 23) : 0.f;
+            const int r = q_row(turn, i0);
+            if (lane % LR == 0)
+                qscale_s[r] = e < 255u ? __uint_as_float((e - 13u) << 23) * a.scale * 1.4426950408889634f : __int_as_float(0x7fc00000);
+#pragma unroll
+            for (int i = i0; i < i0 + NL; ++i) {
+                const int d = q_feature(i), x = d & 63;
+                unsigned char* to = q_s + r * QP + ((d & ~63) + ((x >> 2) & 3) * 16 + 2 * (x >> 4)) * 2;
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const float y0 = e < 255u ? qv[i][2 * j] * down : 0.f, y1 = e < 255u ? qv[i][2 * j + 1] * down : 0.f;
+                    const uint32_t hi = f16x2(y0, y1);
+                    *reinterpret_cast<uint32_t*>(to + 16 * j) = hi;
+                    if constexpr (PARTS == 2) {
+                        const float2 b = floats_of(hi);
+                        *reinterpret_cast<uint32_t*>(to + ROWS * QP + 16 * j) = f16x2(y0 - b.x, y1 - b.y);
+                    }
+                }
+            }
+        }
+    };
+    load_q(0);
+
+    // ---- rows, scales and copies of tiles; the table's entries are read a tile ahead of the rows, the scales a tile
+    // ahead of their use
+    auto key_at = [&](int i) { return key_of(seen, min((tile0 + i) * 64 + tid, seen.count - 1)); };
+    int entry[S], ks = 0, vs = 0;
+    auto ask_entry = [&](int i, int& to) {
+        if (tid < 64 && i < tiles) to = bt[min(page_of(a.page, key_at(i)), a.bt_stride - 1)];
+    };
+    auto keep_row = [&](int i, int from) {
+        if (tid < 64 && i < tiles) {
+            const int key = key_at(i), page = (int)min((unsigned)from, (unsigned)(a.pages - 1));
+            const uint32_t row = ((uint32_t)page * 2 * a.nkv + kvh) * a.page.size + (uint32_t)(key - page_of(a.page, key) * a.page.size);
+            row_s[i % S * 64 + tid] = row;
+            ks = a.scales[row];
+            vs = a.scales[row + plane];
+        }
+    };
+    auto keep_scales = [&](int i) {
+        if (tid < 64 && i < tiles) {
+            const bool bad = ks == KV8_BAD_BYTE || vs == KV8_BAD_BYTE;
+            sc_s[i % S * 64 + tid] = make_float2(bad ? __int_as_float(0x7fc00000) : kv8_scale(ks), (float)(vs - 127));
+        }
+    };
+    // where a 16-byte run c of row r lies in a block of a tile: the swizzle of 128- or 64-byte rows
+    auto at = [](int r, int c) { return r * RB + ((RB == 128 ? c ^ (r & 7) : c ^ ((r >> 1) & 3)) << 4); };
+    auto copy = [&](int i) {
+        if (i < tiles) {
+            constexpr int CPR = HD / 16;
+#pragma unroll
+            for (int k = 0; k < CPR / 2; ++k) {
+                const int r = (k * 128 + tid) / CPR, run = tid % CPR;
+                const uint8_t* src = a.codes + (size_t)row_s[i % S * 64 + r] * HD + run * 16;
+                const uint32_t to = smem_u32(k_s) + i % S * km_tile<HD>() + (run >> 3) * (64 * RB) + at(r, run & 7);
+                cp_async_16(to, src, 16);
+                cp_async_16(to + S * km_tile<HD>(), src + plane * HD, 16);
+            }
+        }
+        cp_async_commit();
+    };
+#pragma unroll
+    for (int i = 0; i < S; ++i) ask_entry(i, entry[i]);
+#pragma unroll
+    for (int i = 0; i < S - 1; ++i) {
+        if (i > 0) keep_scales(i - 1);
+        keep_row(i, entry[i]);
+    }
+    entry[0] = entry[S - 1];
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < S - 1; ++i) copy(i);
+#pragma unroll
+    for (int i = 0; i < TURNS; ++i) {
+        if (i > 0) load_q(i);
+        keep_q(i);
+    }
+    __syncthreads();
+    const int wr = NT == 8 ? warp * 16 : 0, n0 = NT == 8 ? 0 : warp * NT;      // the warp's rows, its first 8 keys of a tile
+    const float qs[2] = {qscale_s[wr + g], qscale_s[wr + g + 8]};
+    // which of the keys in sight (counted as in SeenKeys) a row sees: those up to `last`, of these from `first` on or
+    // before `kept`.  A row sees all keys below a block's last `first` and above its first `last`.
+    const int shift = seen.kept - seen.lo, kept = max(seen.kept, a.keep_first + shift);
+    auto last_of = [&](int row) { return past + row / G + shift; };
+    auto first_of = [&](int row) { return a.window > 0 ? last_of(row) - a.window + 1 : 0; };
+    int last[2], first[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        last[h] = last_of(min(row0 + wr + g + 8 * h, last_row));
+        first[h] = first_of(min(row0 + wr + g + 8 * h, last_row));
+    }
+
+    float o[MT][4], m[2] = {-INFINITY, -INFINITY}, w[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < MT; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+    const int kg = (g & 1) ? g ^ 4 : g, kt = (2 * t + 1) ^ 4;      // a product's row or key i is key i, or i ^ 4 where i is odd
+    const uint32_t q_at = smem_u32(q_s) + (wr + (lane & 15)) * QP + (lane >> 4) * 16;
+
+    for (int i = 0; i < tiles; ++i) {
+        keep_scales(i + S - 2);
+        keep_row(i + S - 1, entry[0]);
+        ask_entry(i + S, entry[0]);
+        cp_async_wait<S - 2>();
+        __syncthreads();                                 // this tile is there, the next rows are, the last tile's place is free
+        copy(i + S - 1);
+        const unsigned char* kt_s = k_s + i % S * km_tile<HD>();
+        const unsigned char* vt_s = v_s + i % S * km_tile<HD>();
+        const float2* sc = sc_s + i % S * 64;
+        const int v0 = (tile0 + i) * 64;
+        // ---- scores: s[n][2h + k], row g + 8h, keys 8 (n0 + n) + 2t and + kt
+        float s[NT][4];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+#pragma unroll
+        for (int c = 0; c < KC; ++c) {
+            uint32_t qf[PARTS][4][4];
+#pragma unroll
+            for (int p = 0; p < PARTS; ++p)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) ldmatrix_x4(qf[p][k], q_at + p * ROWS * QP + (c * 4 + k) * 32);
+#pragma unroll
+            for (int n = 0; n < NT; n += NB) {             // NB products side by side: one waits for the last into its sum
+                uint32_t b[NB][4];
+#pragma unroll
+                for (int y = 0; y < NB; ++y) {
+                    const uint4 x = *reinterpret_cast<const uint4*>(kt_s + (c >> 1) * (64 * RB) + at((n0 + n + y) * 8 + kg, t + 4 * (c & 1)));
+                    b[y][0] = x.x; b[y][1] = x.y; b[y][2] = x.z; b[y][3] = x.w;
+                }
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+#pragma unroll
+                    for (int p = 0; p < PARTS; ++p)
+#pragma unroll
+                        for (int y = 0; y < NB; ++y)
+                            mma_f16_16816(s[n + y], qf[p][k], f16x2_of_codes(b[y][k]), f16x2_of_codes_hi(b[y][k]));
+            }
+        }
+        // ---- weights.  s becomes the scores; the exponents of the values' weights are s + ev
+        float top[2] = {-INFINITY, -INFINITY}, vtop[2] = {-INFINITY, -INFINITY}, ev[NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const float2 f = sc[(n0 + n) * 8 + (k ? kt : 2 * t)];
+                ev[n][k] = f.y;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) s[n][2 * h + k] *= f.x * qs[h];
+            }
+        if (v0 + 63 > last_of(row0) || (v0 < first_of(last_row) && v0 + 63 >= kept)) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const int v = v0 + (n0 + n) * 8 + (k ? kt : 2 * t);
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+                        if (v > last[h] || (v < first[h] && v >= kept)) s[n][2 * h + k] = -INFINITY;
+                }
+        }
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                top[j >> 1] = fmaxf(top[j >> 1], s[n][j]);
+                vtop[j >> 1] = fmaxf(vtop[j >> 1], s[n][j] + ev[n][j & 1]);
+            }
+        if (__any_sync(0xffffffffu, (top[0] > m[0] + KM_SLACK) | (top[1] > m[1] + KM_SLACK) | (vtop[0] > w[0] + KM_SLACK) |
+                                        (vtop[1] > w[1] + KM_SLACK))) {
+            float up[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                for (int d = 1; d < 4; d <<= 1) {
+                    top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], d));
+                    vtop[h] = fmaxf(vtop[h], __shfl_xor_sync(0xffffffffu, vtop[h], d));
+                }
+                top[h] = fmaxf(top[h], m[h]);
+                vtop[h] = fmaxf(vtop[h], w[h]);
+                if (m[h] != -INFINITY) l[h] *= exp2_approx(m[h] - top[h]);
+                up[h] = w[h] == -INFINITY ? 0.f : exp2_approx(w[h] - vtop[h]);
+                m[h] = top[h];
+                w[h] = vtop[h];
+            }
+#pragma unroll
+            for (int k = 0; k < MT; ++k) {
+                o[k][0] *= up[0];
+                o[k][1] *= up[0];
+                o[k][2] *= up[1];
+                o[k][3] *= up[1];
+            }
+        }
+        const float mr[2] = {m[0] == -INFINITY ? 0.f : m[0], m[1] == -INFINITY ? 0.f : m[1]};
+        const float wr2[2] = {w[0] == -INFINITY ? 0.f : w[0], w[1] == -INFINITY ? 0.f : w[1]};
+        // ---- values, 16 keys at a time
+#pragma unroll
+        for (int u = 0; u < NT / 2; ++u) {
+            uint32_t pf[PARTS][4];
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int n = 2 * u + x;
+                    l[h] += exp2_approx(s[n][2 * h] - mr[h]) + exp2_approx(s[n][2 * h + 1] - mr[h]);
+                    const float p0 = exp2_approx(s[n][2 * h] + ev[n][0] - wr2[h]), p1 = exp2_approx(s[n][2 * h + 1] + ev[n][1] - wr2[h]);
+                    const uint32_t hi = f16x2(p0, p1);
+                    pf[0][2 * x + h] = hi;
+                    if constexpr (PARTS == 2) {
+                        const float2 b = floats_of(hi);
+                        pf[PARTS - 1][2 * x + h] = f16x2(p0 - b.x, p1 - b.y);
+                    }
+                }
+            uint32_t v[4][VW];
+            const int key0 = (n0 + 2 * u) * 8;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int r = key0 + 8 * (k >> 1) + ((k & 1) ? kt : 2 * t);
+                if constexpr (HD == 64) {
+                    const uint2 x = *reinterpret_cast<const uint2*>(vt_s + at(r, g >> 1) + (g & 1) * 8);
+                    v[k][0] = x.x;
+                    v[k][1] = x.y;
+                } else {
+#pragma unroll
+                    for (int c = 0; c < VW / 4; ++c) {
+                        const int run = g * (VW / 4) + c;
+                        const uint4 x = *reinterpret_cast<const uint4*>(vt_s + (run >> 3) * (64 * RB) + at(r, run & 7));
+                        v[k][4 * c] = x.x; v[k][4 * c + 1] = x.y; v[k][4 * c + 2] = x.z; v[k][4 * c + 3] = x.w;
+                    }
+                }
+            }
+            // block 4 j + e of 8 features: feature 4 j + e of every lane group's run of HD / 8
+#pragma unroll
+            for (int j = 0; j < VW; ++j) {
+                const uint32_t a01 = __byte_perm(v[0][j], v[1][j], 0x5140), a23 = __byte_perm(v[0][j], v[1][j], 0x7362);
+                const uint32_t b01 = __byte_perm(v[2][j], v[3][j], 0x5140), b23 = __byte_perm(v[2][j], v[3][j], 0x7362);
+                const uint32_t lo[4] = {f16x2_of_codes(a01), f16x2_of_codes_hi(a01), f16x2_of_codes(a23), f16x2_of_codes_hi(a23)};
+                const uint32_t hi[4] = {f16x2_of_codes(b01), f16x2_of_codes_hi(b01), f16x2_of_codes(b23), f16x2_of_codes_hi(b23)};
+#pragma unroll
+                for (int p = 0; p < PARTS; ++p)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) mma_f16_16816(o[4 * j + e], pf[p], lo[e], hi[e]);
+            }
+        }
+    }
+    cp_async_wait<0>();
+    pdl_launch_dependents();
+    // ---- the rows' sums, and the outputs: o[k][2h + e], row g + 8h, feature k of the runs of lane groups 2t + e
+    const int part = NT == 8 ? range : range * 4 + warp;
+    const bool parts = NT == 2 || a.parts.splits > 1;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+        for (int d = 1; d < 4; d <<= 1) l[h] += __shfl_xor_sync(0xffffffffu, l[h], d);
+        const int row = row0 + wr + g + 8 * h;
+        if (row >= rows || (parts && !kv8_has_room(a.parts, first_token + row / G))) continue;
+        const size_t head = (size_t)(first_token + row / G) * a.nq + kvh * G + row % G;
+        // 2^(m' - m): the two maxima differ by the values' exponents and the slack at most
+        const float back = w[h] == -INFINITY ? 0.f : exp2_approx(w[h] - m[h]);
+        const float f = parts ? back : l[h] == 0.f ? 0.f : back / l[h];
+        const size_t at_part = (head - (size_t)kv8_first_token(a.parts) * a.nq) * a.parts.splits + part;
+        if (parts && t == 0) {
+            a.parts.ml[2 * at_part] = m[h];
+            a.parts.ml[2 * at_part + 1] = l[h];
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+#pragma unroll
+            for (int k = 0; k < MT; k += 4) {
+                const float x[4] = {o[k][2 * h + e] * f, o[k + 1][2 * h + e] * f, o[k + 2][2 * h + e] * f, o[k + 3][2 * h + e] * f};
+                const int d = (2 * t + e) * (HD / 8) + k;
+                if (parts) store4(a.parts.o + at_part * HD + d, x);
+                else store4((A*)a.out + head * HD + d, x);
+            }
+    }
+}
+
+template <typename A, int HD, int PARTS, int NT>
+static int launch_mma(const Kv8AttnArgs& a, dim3 grid, cudaStream_t s) {
+    auto kernel = kv8_attention_mma_kernel<A, HD, PARTS, NT>;
+    constexpr int smem = km_smem<HD, PARTS, NT>();
+    static bool configured[64] = {false};
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return (int)e;
+    if (dev < 0 || dev >= 64) return -1;
+    if (!configured[dev]) {
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        if (e != cudaSuccess) return (int)e;
+        configured[dev] = true;
+    }
+    e = mstar_launch(kernel, grid, dim3(128), (size_t)smem, s, a);
+    return e != cudaSuccess ? (int)e : launch_status();
+}
+template <typename A, int PARTS, int NT> static int launch_mma_hd(const Kv8AttnArgs& a, dim3 grid, cudaStream_t s) {
+    switch (a.hd) {
+        case 64: return launch_mma<A, 64, PARTS, NT>(a, grid, s);
+        case 128: return launch_mma<A, 128, PARTS, NT>(a, grid, s);
+        default: return launch_mma<A, 256, PARTS, NT>(a, grid, s);
+    }
 }
 
 // Portions (token_req null): entries [first_entry, first_entry + count) of at most max_q tokens.  Single tokens:
 // tokens [0, count).  `tokens`: at least as many as the call covers, at most what `out` has.  splits > 1: the keys of a
-// row tile are shared by that many blocks, `part_o` (tokens * nq * splits * hd floats) and `part_ml` (2 each) hold their
-// parts and a second kernel joins them.  Returns 0, a CUDA error code or -1 (shape refused).
+// row tile are cut into that many parts, `part_o` (tokens * nq * splits * hd floats) and `part_ml` (2 each) hold their
+// parts and a second kernel joins them; a multiple of 4 where rows are 16 or fewer and hd is 64, 128 or 256 (a part a
+// warp).  Returns 0, a CUDA error code or -1 (shape refused).
 MSTAR_API int mstar_kv8_attention(const void* q, int q_stride, void* out, int act_dtype, const void* codes,
                                   const void* scales, int pages, const int* block_table, int bt_stride,
                                   const int* qo_indptr, const int* kv_len, const int* token_req, const int* cache_pos,
@@ -241,21 +671,33 @@ MSTAR_API int mstar_kv8_attention(const void* q, int q_stride, void* out, int ac
     if (hd <= 0 || hd % 8 != 0 || hd > 256 || nkv <= 0 || nq % nkv != 0 || page_size <= 0 || pages <= 0 || splits < 1 ||
         count > 65535 || ((uintptr_t)codes & 7) != 0)
         return -1;
-    const Kv8Parts parts{part_o, part_ml, splits, token_req == nullptr ? qo_indptr + first_entry : nullptr, count};
+    const Kv8Parts parts{part_o, part_ml, splits, token_req == nullptr ? qo_indptr + first_entry : nullptr, count, tokens};
     const Kv8AttnArgs a{q, out, (const uint8_t*)codes, (const uint8_t*)scales, block_table, qo_indptr, kv_len, token_req,
                         cache_pos, q_stride, bt_stride, pages, nq, nkv, hd, window, keep_first, first_entry, scale,
                         page_split(page_size), parts};
     const long long rows = (long long)max_q * (nq / nkv);
-    const int R = rows <= 8 ? 8 : 64;
-    const long long tiles = (rows + R - 1) / R;
-    if (tiles > 65535) return -1;
-    const dim3 grid(nkv * splits, (unsigned)tiles, count);
     const cudaStream_t s = (cudaStream_t)stream;
     int code;
-    if (act_dtype == MSTAR_F32) code = R == 8 ? launch_simt<float, 8>(a, grid, s) : launch_simt<float, 64>(a, grid, s);
-    else code = R == 8 ? launch_simt<bf16, 8>(a, grid, s) : launch_simt<bf16, 64>(a, grid, s);
+    // (the copies want runs of 16 bytes, which any cache of these head sizes has; the output is stored four at a time)
+    if ((hd == 64 || hd == 128 || hd == 256) && ((uintptr_t)codes & 15) == 0 && ((uintptr_t)out & 15) == 0 &&
+        (long long)pages * 2 * nkv * page_size <= 0xffffffffll) {
+        const bool few = rows <= 16;
+        if (few && splits % 4 != 0) return -1;
+        const long long tiles = few ? 1 : (rows + 63) / 64;
+        if (tiles > 65535) return -1;
+        const dim3 grid(nkv * (few ? splits / 4 : splits), (unsigned)tiles, count);
+        if (act_dtype == MSTAR_F32) code = few ? launch_mma_hd<float, 2, 2>(a, grid, s) : launch_mma_hd<float, 2, 8>(a, grid, s);
+        else code = few ? launch_mma_hd<bf16, 1, 2>(a, grid, s) : launch_mma_hd<bf16, 1, 8>(a, grid, s);
+    } else {
+        const int R = rows <= 8 ? 8 : 64;
+        const long long tiles = (rows + R - 1) / R;
+        if (tiles > 65535) return -1;
+        const dim3 grid(nkv * splits, (unsigned)tiles, count);
+        if (act_dtype == MSTAR_F32) code = R == 8 ? launch_simt<float, 8>(a, grid, s) : launch_simt<float, 64>(a, grid, s);
+        else code = R == 8 ? launch_simt<bf16, 8>(a, grid, s) : launch_simt<bf16, 64>(a, grid, s);
+    }
     if (code != 0 || splits == 1) return code;
-    return kv8_merge(parts, out, act_dtype, tokens, nq, hd, s);
+    return kv8_merge(parts, out, act_dtype, nq, hd, s);
 }
 
 MSTAR_API int mstar_kv8_attention_packed(const long long* a) {

@@ -617,10 +617,10 @@ __global__ void __launch_bounds__(K8_THREADS, 1) kv8_attention_tc_kernel(Kv8TcAr
             pt_fence_after();
             // ---------------------------------------------------------------- epilogue
             if (ok) {
-                const bool parts = PAIR || splits > 1;
+                const bool parts = PAIR || splits > 1, stored = valid && (!parts || kv8_has_room(a.parts, (int)(head / a.nq)));
                 const size_t at = (head - (size_t)kv8_first_token(a.parts) * a.nq) * a.parts.splits + (PAIR ? 2 * split + x : split);
                 const float f = parts ? 1.f : l == 0.f ? 0.f : 1.f / l;
-                if (parts && valid) {
+                if (parts && stored) {
                     a.parts.ml[2 * at] = l == 0.f ? -INFINITY : m;
                     a.parts.ml[2 * at + 1] = l;
                 }
@@ -629,7 +629,7 @@ __global__ void __launch_bounds__(K8_THREADS, 1) kv8_attention_tc_kernel(Kv8TcAr
                     uint32_t o[32];
                     pt_ld32(t_o + c0, o);
                     pt_wait_ld();
-                    if (valid) {
+                    if (stored) {
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             float v[8];
@@ -690,7 +690,7 @@ MSTAR_API int mstar_kv8_attention_tc(const void* q, int q_stride, void* out, con
         q_stride % 8 != 0 || ((uintptr_t)codes & 15) != 0 || ((uintptr_t)out & 15) != 0 ||
         (long long)pages * 2 * nkv * page_size > 0xffffffffll)
         return -1;
-    const Kv8Parts parts{part_o, part_ml, splits, qo_indptr + first_entry, count};
+    const Kv8Parts parts{part_o, part_ml, splits, qo_indptr + first_entry, count, tokens};
     const Kv8TcArgs a{(const bf16*)q, (bf16*)out, (const uint8_t*)codes, (const uint8_t*)scales, block_table, qo_indptr,
                       kv_len, q_stride, bt_stride, pages, nq, nkv, window, keep_first, first_entry,
                       scale * 1.4426950408889634f, page_split(page_size), parts, error_word};
@@ -704,7 +704,7 @@ MSTAR_API int mstar_kv8_attention_tc(const void* q, int q_stride, void* out, con
     if (pair) code = hd == 64 ? launch_kv8_tc<64, true>(a, grid, s) : launch_kv8_tc<128, true>(a, grid, s);
     else code = hd == 64 ? launch_kv8_tc<64, false>(a, grid, s) : launch_kv8_tc<128, false>(a, grid, s);
     if (code != 0 || splits == 1) return code;
-    return kv8_merge(parts, out, MSTAR_BF16, tokens, nq, hd, s);
+    return kv8_merge(parts, out, MSTAR_BF16, nq, hd, s);
 }
 
 MSTAR_API int mstar_kv8_attention_tc_packed(const long long* a) {

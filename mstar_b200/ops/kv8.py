@@ -191,6 +191,17 @@ def kv8_splits(blocks: int, max_keys: int, sms: int) -> int:
     return max(1, min(64, -(-2 * sms // max(blocks, 1)), -(-max_keys // 128)))
 
 
+def kv8_mma_splits(blocks: int, max_keys: int, sms: int, few: bool) -> int:
+    """The same for the kernel of the 32-bit mode.  64 rows: two blocks an SM, parts of at least 256 keys.
+    (256 blocks on 220 keys, 152 on 1,000, 512 on 6,500 took 15.7, 59.3, 326 us uncut and 19.4, 55.9, 314 in two
+    parts.)  16 rows or fewer: a block's four warps leave a part each; three blocks on two SMs, 64 keys a warp
+    at least.  (8 pairs of a token and a kv head on 16,384 keys, 64 on 2,048 and 512 on 1,028 took 32, 18 and
+    40 us so, 42, 26 and 36 with a quarter, half and twice as many.)"""
+    if few:
+        return 4 * max(1, min(64, -(-3 * sms // (2 * max(blocks, 1))), -(-max_keys // 256)))
+    return max(1, min(64, -(-2 * sms // max(blocks, 1)), -(-max_keys // 256)))
+
+
 def _parts(q, tokens, num_heads, head_dim, splits) -> tuple:
     """(the tensor, addresses of the outputs' and of the statistics' parts)."""
     if splits == 1:
@@ -201,12 +212,19 @@ def _parts(q, tokens, num_heads, head_dim, splits) -> tuple:
 
 
 def _float_attention(what, q, q_stride, out, kv_cache, kv_scales, pages, block_table, table, indptr, kv_len, req, pos,
-                     first_entry, count, max_q, max_keys, num_heads, num_kv_heads, head_dim, page_size, window, keep_first,
+                     first_entry, count, max_q, max_len, num_heads, num_kv_heads, head_dim, page_size, window, keep_first,
                      scale) -> None:
     """The kernel that takes every shape: portions by (indptr, kv_len), single tokens by (req, pos)."""
-    rows = max_q * (num_heads // num_kv_heads)
-    tiles = 1 if rows <= 8 else -(-rows // 64)
-    splits = kv8_splits(tiles * num_kv_heads * count, max_keys, _sms(q.get_device()))
+    group, sms = num_heads // num_kv_heads, _sms(q.get_device())
+    rows = max_q * group
+    if head_dim in KV8_DECODE_HEAD_DIMS and (kv_cache.data_ptr() | out.data_ptr()) % 16 == 0:
+        few = rows <= 16
+        splits = kv8_mma_splits((1 if few else -(-rows // 64)) * num_kv_heads * count,
+                                _most_keys(max_len, max_q if few else min(max_q, 63 // group + 2), window, keep_first),
+                                sms, few)
+    else:
+        splits = kv8_splits((1 if rows <= 8 else -(-rows // 64)) * num_kv_heads * count,
+                            _most_keys(max_len, max_q, window, keep_first), sms)
     tokens = min(out.shape[0], count * max_q)
     part, part_o, part_ml = _parts(q, tokens, num_heads, head_dim, splits)
     check(lib.get("attention_kv8").mstar_kv8_attention_packed(_pack_float(
@@ -286,7 +304,7 @@ def paged_decode_attention_kv8(q: torch.Tensor, out: torch.Tensor, kv_cache: tor
             warps, _stream())), what)
         return
     _float_attention(what, q, q_stride, out, kv_cache, kv_scales, pages, block_table, table, 0, 0, token_req.data_ptr(),
-                     cache_pos.data_ptr(), 0, tokens, 1, most, num_heads, num_kv_heads, head_dim, page_size, window,
+                     cache_pos.data_ptr(), 0, tokens, 1, max_len, num_heads, num_kv_heads, head_dim, page_size, window,
                      keep_first, scale)
 
 
@@ -337,5 +355,5 @@ def paged_prefill_attention_kv8(q: torch.Tensor, out: torch.Tensor, kv_cache: to
             lib.add_launches(1)                 # the kernel that joins the parts
         return
     _float_attention(what, q, q_stride, out, kv_cache, kv_scales, pages, block_table, table, qo_indptr.data_ptr(),
-                     kv_len.data_ptr(), 0, 0, first_entry, entries, max_q_len, most, num_heads, num_kv_heads, head_dim,
-                     page_size, window, keep_first, scale)
+                     kv_len.data_ptr(), 0, 0, first_entry, entries, max_q_len, max_kv_len, num_heads, num_kv_heads,
+                     head_dim, page_size, window, keep_first, scale)
