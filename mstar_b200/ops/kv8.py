@@ -257,10 +257,11 @@ KV8_TC_HEAD_DIMS = (64, 128)
 def kv8_tc_splits(blocks: int, max_keys: int, sms: int, one_tile: bool) -> tuple:
     """(parts that the keys of ``blocks`` blocks of row tiles are cut into in the tensor-core kernel, whether a
     block makes two of them): a block an SM, at least two tiles of 128 keys each, at most 64 parts.  With
-    one row tile a block takes two key tiles side by side from ten tiles on: two portions of 17 tokens on
-    20,000 / 10,000 / 5,000 keys took 49.7 / 35.2 / 26.9 us so, and 56.3 / 34.8 / 23.9 one after another."""
+    one row tile a block takes two key tiles side by side from four tiles on: two portions of 17 tokens on
+    20,000 / 10,000 / 5,000 keys took 41.0 / 27.3 / 21.5 us so, and 49.4 / 31.2 / 22.9 one after another; one
+    on 5,000 keys (two tiles a block) 20.6 and 19.8."""
     ranges = max(1, min(32, sms // max(blocks, 1), -(-max_keys // 256)))
-    pair = one_tile and max_keys >= ranges * 1280
+    pair = one_tile and max_keys >= ranges * 512
     return (2 * ranges if pair else ranges), pair
 
 
