@@ -22,7 +22,7 @@ struct Kv8AttnArgs {
     const int *block_table;
     // portions: first token and end of every entry, keys of every entry; single tokens: request and place of each
     const int *qo_indptr, *kv_len, *token_req, *cache_pos;
-    int q_stride, bt_stride, pages, nq, nkv, hd, window, keep_first, first_entry;
+    int q_stride, bt_stride, bt_width, pages, nq, nkv, hd, window, keep_first, first_entry;
     float scale;
     PageSplit page;
     Kv8Parts parts;
@@ -97,7 +97,7 @@ __global__ void __launch_bounds__(256) kv8_attention_kernel(Kv8AttnArgs a) {
                 for (int k = 0; k < 8; ++k) v[k] = 0.f;
                 if (j < n) {
                     const int key = key_of(seen, v0 + j), logical = page_of(a.page, key);
-                    const size_t at = ((size_t)page_id(bt, logical, a.bt_stride, a.pages) * 2 + which) * plane +
+                    const size_t at = ((size_t)page_id(bt, logical, a.bt_width, a.pages) * 2 + which) * plane +
                                       (size_t)kvh * a.page.size + (key - logical * a.page.size);
                     const uint2 w = *reinterpret_cast<const uint2*>(a.codes + at * hd + d);
                     const int byte = a.scales[at];
@@ -384,7 +384,7 @@ __global__ void __launch_bounds__(128) kv8_attention_mma_kernel(Kv8AttnArgs a) {
     auto key_at = [&](int i) { return key_of(seen, min((tile0 + i) * 64 + tid, seen.count - 1)); };
     int entry[S], ks = 0, vs = 0;
     auto ask_entry = [&](int i, int& to) {
-        if (tid < 64 && i < tiles) to = bt[min(page_of(a.page, key_at(i)), a.bt_stride - 1)];
+        if (tid < 64 && i < tiles) to = bt[min(page_of(a.page, key_at(i)), a.bt_width - 1)];
     };
     auto keep_row = [&](int i, int from) {
         if (tid < 64 && i < tiles) {
@@ -662,24 +662,24 @@ template <typename A, int PARTS, int NT> static int launch_mma_hd(const Kv8AttnA
 // parts and a second kernel joins them; a multiple of 4 where rows are 16 or fewer and hd is 64, 128 or 256 (a part a
 // warp).  Returns 0, a CUDA error code or -1 (shape refused).
 MSTAR_API int mstar_kv8_attention(const void* q, int q_stride, void* out, int act_dtype, const void* codes,
-                                  const void* scales, int pages, const int* block_table, int bt_stride,
+                                  const void* scales, int pages, const int* block_table, int bt_stride, int bt_width,
                                   const int* qo_indptr, const int* kv_len, const int* token_req, const int* cache_pos,
                                   int first_entry, int count, int max_q, int tokens, int nq, int nkv, int hd,
                                   int page_size, int window, int keep_first, float scale, int splits, float* part_o,
                                   float* part_ml, void* stream) {
     if (count <= 0 || max_q <= 0) return 0;
-    if (hd <= 0 || hd % 8 != 0 || hd > 256 || nkv <= 0 || nq % nkv != 0 || page_size <= 0 || pages <= 0 || splits < 1 ||
-        count > 65535 || ((uintptr_t)codes & 7) != 0)
+    if (hd <= 0 || hd % 8 != 0 || hd > 256 || nkv <= 0 || nq % nkv != 0 || page_size <= 0 || pages <= 0 || bt_width <= 0 ||
+        splits < 1 || count > 65535 || ((uintptr_t)codes & 7) != 0 || ((uintptr_t)out & 15) != 0)
         return -1;
     const Kv8Parts parts{part_o, part_ml, splits, token_req == nullptr ? qo_indptr + first_entry : nullptr, count, tokens};
     const Kv8AttnArgs a{q, out, (const uint8_t*)codes, (const uint8_t*)scales, block_table, qo_indptr, kv_len, token_req,
-                        cache_pos, q_stride, bt_stride, pages, nq, nkv, hd, window, keep_first, first_entry, scale,
+                        cache_pos, q_stride, bt_stride, bt_width, pages, nq, nkv, hd, window, keep_first, first_entry, scale,
                         page_split(page_size), parts};
     const long long rows = (long long)max_q * (nq / nkv);
     const cudaStream_t s = (cudaStream_t)stream;
     int code;
-    // (the copies want runs of 16 bytes, which any cache of these head sizes has; the output is stored four at a time)
-    if ((hd == 64 || hd == 128 || hd == 256) && ((uintptr_t)codes & 15) == 0 && ((uintptr_t)out & 15) == 0 &&
+    // (the copies want runs of 16 bytes)
+    if ((hd == 64 || hd == 128 || hd == 256) && ((uintptr_t)codes & 15) == 0 &&
         (long long)pages * 2 * nkv * page_size <= 0xffffffffll) {
         const bool few = rows <= 16;
         if (few && splits % 4 != 0) return -1;
@@ -702,8 +702,8 @@ MSTAR_API int mstar_kv8_attention(const void* q, int q_stride, void* out, int ac
 
 MSTAR_API int mstar_kv8_attention_packed(const long long* a) {
     return mstar_kv8_attention((const void*)a[0], (int)a[1], (void*)a[2], (int)a[3], (const void*)a[4],
-        (const void*)a[5], (int)a[6], (const int*)a[7], (int)a[8], (const int*)a[9], (const int*)a[10],
-        (const int*)a[11], (const int*)a[12], (int)a[13], (int)a[14], (int)a[15], (int)a[16], (int)a[17], (int)a[18],
-        (int)a[19], (int)a[20], (int)a[21], (int)a[22], kv8_packed_float(a[23]), (int)a[24], (float*)a[25],
-        (float*)a[26], (void*)a[27]);
+        (const void*)a[5], (int)a[6], (const int*)a[7], (int)a[8], (int)a[9], (const int*)a[10], (const int*)a[11],
+        (const int*)a[12], (const int*)a[13], (int)a[14], (int)a[15], (int)a[16], (int)a[17], (int)a[18], (int)a[19],
+        (int)a[20], (int)a[21], (int)a[22], (int)a[23], kv8_packed_float(a[24]), (int)a[25], (float*)a[26],
+        (float*)a[27], (void*)a[28]);
 }

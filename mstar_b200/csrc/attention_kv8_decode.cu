@@ -49,7 +49,7 @@ struct Kv8DecodeArgs {
     bf16* out;
     const uint8_t *codes, *scales;
     const int *block_table, *token_req, *cache_pos;
-    int q_stride, bt_stride, pages, nq, nkv, window, keep_first, head_groups;
+    int q_stride, bt_stride, bt_width, pages, nq, nkv, window, keep_first, head_groups;
     float scale_log2e;
     PageSplit page;
 };
@@ -159,7 +159,7 @@ kv8_decode_kernel(Kv8DecodeArgs a) {
     // The row (of the cache as a matrix of D bytes a row) of this lane's key of a tile, from the table's entry for it.
     // What lies past the table or on pages that are not there is brought into the cache and masked.  (Two steps: a warp
     // issues in order, and would stand still at the first use of an entry just asked for.)
-    auto entry_of = [&](int i) -> int { return bt[min(page_of(a.page, key0_of(i) + lane), a.bt_stride - 1)]; };
+    auto entry_of = [&](int i) -> int { return bt[min(page_of(a.page, key0_of(i) + lane), a.bt_width - 1)]; };
     auto row_of = [&](int i, int entry) -> uint32_t {
         const int key = key0_of(i) + lane, page = (int)min((unsigned)entry, (unsigned)(a.pages - 1));
         return ((uint32_t)page * 2 * a.nkv + kvh) * a.page.size + (uint32_t)(key - page_of(a.page, key) * a.page.size);
@@ -329,7 +329,7 @@ kv8_decode_kernel(Kv8DecodeArgs a) {
             for (int k = 0; k < E; ++k) {
                 const int j = 16 * u + 8 * k + kmine;
                 const float2 f = sc[j];
-                float b0 = s[u][2 * k] * f.x * hs0, b1 = s[u][2 * k + 1] * f.x * hs1;
+                float b0 = s[u][2 * k] * (f.x * hs0), b1 = s[u][2 * k + 1] * (f.x * hs1);
                 if (!whole) {
                     const int key = key0 + j;
                     if (key > pos || (key < lo && key >= a.keep_first)) b0 = b1 = -INFINITY;
@@ -583,17 +583,18 @@ static int launch_decode(const Kv8DecodeArgs& a, int tokens, int blocks, int war
 // 8 or 16, a cluster) of `warps` warps share the keys of a (token, kv head, 8 query heads, or up to 4 where a kv head has
 // no more).  page_size: a multiple of 8.  Returns 0, a CUDA error code or -1 (shape refused).
 MSTAR_API int mstar_kv8_decode(const void* q, int q_stride, void* out, const void* codes, const void* scales, int pages,
-                               const int* block_table, int bt_stride, const int* token_req, const int* cache_pos,
+                               const int* block_table, int bt_stride, int bt_width, const int* token_req, const int* cache_pos,
                                int tokens, int nq, int nkv, int hd, int page_size, int window, int keep_first, float scale,
                                int blocks, int warps, void* stream) {
     if (tokens <= 0) return 0;
-    if (nkv <= 0 || nq % nkv != 0 || page_size <= 0 || page_size % 8 != 0 || pages <= 0 || tokens > 65535 || blocks < 1 ||
+    if (nkv <= 0 || nq % nkv != 0 || page_size <= 0 || page_size % 8 != 0 || pages <= 0 || bt_width <= 0 ||
+        tokens > 65535 || blocks < 1 ||
         blocks > 16 || (blocks & (blocks - 1)) != 0 || ((uintptr_t)q & 15) != 0 || q_stride % 8 != 0 ||
         ((uintptr_t)codes & 15) != 0 || ((uintptr_t)scales & 7) != 0 || ((uintptr_t)out & 7) != 0 ||
         (long long)pages * 2 * nkv * page_size > 0xffffffffll || (hd != 64 && hd != 128 && hd != 256))
         return -1;
     const Kv8DecodeArgs a{(const bf16*)q, (bf16*)out, (const uint8_t*)codes, (const uint8_t*)scales, block_table,
-                          token_req, cache_pos, q_stride, bt_stride, pages, nq, nkv, window, keep_first,
+                          token_req, cache_pos, q_stride, bt_stride, bt_width, pages, nq, nkv, window, keep_first,
                           (nq / nkv + 7) / 8, scale * 1.4426950408889634f, page_split(page_size)};
     const cudaStream_t s = (cudaStream_t)stream;
     const bool few = nq / nkv <= 4;
@@ -606,7 +607,7 @@ MSTAR_API int mstar_kv8_decode(const void* q, int q_stride, void* out, const voi
 
 MSTAR_API int mstar_kv8_decode_packed(const long long* a) {
     return mstar_kv8_decode((const void*)a[0], (int)a[1], (void*)a[2], (const void*)a[3], (const void*)a[4],
-        (int)a[5], (const int*)a[6], (int)a[7], (const int*)a[8], (const int*)a[9], (int)a[10], (int)a[11],
-        (int)a[12], (int)a[13], (int)a[14], (int)a[15], (int)a[16], kv8_packed_float(a[17]), (int)a[18], (int)a[19],
-        (void*)a[20]);
+        (int)a[5], (const int*)a[6], (int)a[7], (int)a[8], (const int*)a[9], (const int*)a[10], (int)a[11], (int)a[12],
+        (int)a[13], (int)a[14], (int)a[15], (int)a[16], (int)a[17], kv8_packed_float(a[18]), (int)a[19], (int)a[20],
+        (void*)a[21]);
 }

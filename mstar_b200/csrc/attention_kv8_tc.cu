@@ -65,7 +65,7 @@ struct Kv8TcArgs {
     bf16* out;
     const uint8_t *codes, *scales;
     const int *block_table, *qo_indptr, *kv_len;
-    int q_stride, bt_stride, pages, nq, nkv, window, keep_first, first_entry;
+    int q_stride, bt_stride, bt_width, pages, nq, nkv, window, keep_first, first_entry;
     float scale_log2e;
     PageSplit page;
     Kv8Parts parts;
@@ -239,7 +239,7 @@ __global__ void __launch_bounds__(K8_THREADS, 1) kv8_attention_tc_kernel(Kv8TcAr
             const int kt = tid - 13 * 32;                    // 96 threads; the first 32 have a second key of a tile
             auto entry_of = [&](int j, int c) -> int {
                 const int key = key_of(seen, min((tile0 + j) * K8_KEYS + c, seen.count - 1));
-                return bt[min(page_of(a.page, key), a.bt_stride - 1)];
+                return bt[min(page_of(a.page, key), a.bt_width - 1)];
             };
             auto row_of = [&](int j, int c, int entry) -> uint32_t {
                 const int key = key_of(seen, min((tile0 + j) * K8_KEYS + c, seen.count - 1));
@@ -771,19 +771,19 @@ template <int HD, bool PAIR> static int launch_kv8_tc(const Kv8TcArgs& a, dim3 g
 // the even and the odd key tiles of its one row tile side by side and leaves two of the (an even number of) parts.  Returns 0, a CUDA error code or -1 (shape
 // refused).
 MSTAR_API int mstar_kv8_attention_tc(const void* q, int q_stride, void* out, const void* codes, const void* scales, int pages,
-                                     const int* block_table, int bt_stride, const int* qo_indptr, const int* kv_len,
+                                     const int* block_table, int bt_stride, int bt_width, const int* qo_indptr, const int* kv_len,
                                      int first_entry, int count, int max_q, int tokens, int nq, int nkv, int hd,
                                      int page_size, int window, int keep_first, float scale, int splits, int pair,
                                      float* part_o, float* part_ml, int* error_word, void* stream) {
     if (count <= 0 || max_q <= 0) return 0;
-    if ((hd != 64 && hd != 128) || nkv <= 0 || nq % nkv != 0 || nq / nkv > K8_ROWS || page_size <= 0 || pages <= 0 ||
-        splits < 1 || count > 65535 || error_word == nullptr || !(scale > 0.f) || ((uintptr_t)q & 15) != 0 ||
+    if ((hd != 64 && hd != 128) || nkv <= 0 || nq % nkv != 0 || nq / nkv > K8_ROWS || page_size <= 0 ||
+        pages <= 0 || bt_width <= 0 || splits < 1 || count > 65535 || error_word == nullptr || !(scale > 0.f) || ((uintptr_t)q & 15) != 0 ||
         q_stride % 8 != 0 || ((uintptr_t)codes & 15) != 0 || ((uintptr_t)out & 15) != 0 ||
         (long long)pages * 2 * nkv * page_size > 0xffffffffll)
         return -1;
     const Kv8Parts parts{part_o, part_ml, splits, qo_indptr + first_entry, count, tokens};
     const Kv8TcArgs a{(const bf16*)q, (bf16*)out, (const uint8_t*)codes, (const uint8_t*)scales, block_table, qo_indptr,
-                      kv_len, q_stride, bt_stride, pages, nq, nkv, window, keep_first, first_entry,
+                      kv_len, q_stride, bt_stride, bt_width, pages, nq, nkv, window, keep_first, first_entry,
                       scale * 1.4426950408889634f, page_split(page_size), parts, error_word};
     const int per_tile = K8_ROWS / (nq / nkv);
     if (pair && (max_q > per_tile || splits % 2 != 0)) return -1;
@@ -800,7 +800,7 @@ MSTAR_API int mstar_kv8_attention_tc(const void* q, int q_stride, void* out, con
 
 MSTAR_API int mstar_kv8_attention_tc_packed(const long long* a) {
     return mstar_kv8_attention_tc((const void*)a[0], (int)a[1], (void*)a[2], (const void*)a[3], (const void*)a[4],
-        (int)a[5], (const int*)a[6], (int)a[7], (const int*)a[8], (const int*)a[9], (int)a[10], (int)a[11],
-        (int)a[12], (int)a[13], (int)a[14], (int)a[15], (int)a[16], (int)a[17], (int)a[18], (int)a[19],
-        kv8_packed_float(a[20]), (int)a[21], (int)a[22], (float*)a[23], (float*)a[24], (int*)a[25], (void*)a[26]);
+        (int)a[5], (const int*)a[6], (int)a[7], (int)a[8], (const int*)a[9], (const int*)a[10], (int)a[11], (int)a[12],
+        (int)a[13], (int)a[14], (int)a[15], (int)a[16], (int)a[17], (int)a[18], (int)a[19], (int)a[20],
+        kv8_packed_float(a[21]), (int)a[22], (int)a[23], (float*)a[24], (float*)a[25], (int*)a[26], (void*)a[27]);
 }

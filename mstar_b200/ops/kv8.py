@@ -28,11 +28,11 @@ _INT = torch.int32
 _F32, _BF16 = torch.float32, torch.bfloat16
 _device = torch._C._cuda_getDevice
 # the entry points' arguments as one string (csrc/kv8.cuh)
-_pack_write = Struct("=21q").pack
-_pack_read = Struct("=14q").pack
-_pack_float = Struct("=23qd4q").pack
-_pack_decode = Struct("=17qd3q").pack
-_pack_portions = Struct("=20qd6q").pack
+_pack_write = Struct("=22q").pack
+_pack_read = Struct("=15q").pack
+_pack_float = Struct("=24qd4q").pack
+_pack_decode = Struct("=18qd3q").pack
+_pack_portions = Struct("=21qd6q").pack
 
 
 _sm_counts: dict = {}
@@ -70,12 +70,15 @@ def _check_cache(what, kv_cache, kv_scales, num_kv_heads, page_size, head_dim) -
     return shape[0]
 
 
-def _check_table(what, block_table) -> int:
-    """The distance of its rows."""
+def _check_table(what, block_table, read=False) -> tuple:
+    """The distance of its rows and their entries."""
     strides = block_table.stride()
     if block_table.dtype is not _INT or len(strides) != 2 or strides[1] != 1 or strides[0] < 1:
         _refuse(what, "the block table is int32 [entries, pages], its rows without gaps")
-    return strides[0]
+    width = block_table.shape[1]
+    if read and width < 1:
+        _refuse(what, "the block table has no pages")
+    return strides[0], width
 
 
 def _check_index(what, t, n) -> None:
@@ -95,7 +98,8 @@ def rope_kv8_write(qkv: torch.Tensor, positions, cache_pos, token_req, block_tab
     """Rotate queries and keys of ``qkv`` [tokens, (num_heads + 2 num_kv_heads) * head_dim], quantise keys
     and values into their pages, and return the rotated queries [tokens, num_heads * head_dim] in a
     tensor of their own (``qkv`` stays as it is).  ``inv_freq``: float [rotary_dim / 2], or None when
-    rotary_dim == 0.  Two tokens of a call that name the same place of a request leave either's row."""
+    rotary_dim == 0.  The tokens of a call name different places: of two with the same one, what is
+    left is a mixture."""
     what = "rope_kv8_write"
     dtype = _DT.get(qkv.dtype)
     if dtype is None:
@@ -131,7 +135,7 @@ def rope_kv8_write(qkv: torch.Tensor, positions, cache_pos, token_req, block_tab
         return q
     check(lib.get("kv8_cache").mstar_rope_kv8_write_packed(_pack_write(
         qkv.data_ptr(), dtype, strides[0], q.data_ptr(), positions.data_ptr(), cache_pos.data_ptr(),
-        token_req.data_ptr(), block_table.data_ptr(), table, freq, kv_cache.data_ptr(), kv_scales.data_ptr(), pages, n,
+        token_req.data_ptr(), block_table.data_ptr(), *table, freq, kv_cache.data_ptr(), kv_scales.data_ptr(), pages, n,
         num_heads, num_kv_heads, head_dim, rotary_dim, bool(interleaved), page_size, _stream())), what)
     return q
 
@@ -160,7 +164,7 @@ def kv8_read_rows(kv_cache: torch.Tensor, kv_scales: torch.Tensor, block_table, 
     out = kv_scales.new_empty((n, 2, heads, head_dim), dtype=dtype)
     if n:
         check(lib.get("kv8_cache").mstar_kv8_read_rows_packed(_pack_read(
-            kv_cache.data_ptr(), kv_scales.data_ptr(), block_table.data_ptr(), table, token_req.data_ptr(),
+            kv_cache.data_ptr(), kv_scales.data_ptr(), block_table.data_ptr(), *table, token_req.data_ptr(),
             cache_pos.data_ptr(), out.data_ptr(), out_type, n, heads, head_dim, pages, page_size, _stream())), what)
     return out
 
@@ -178,6 +182,8 @@ def _check_attention(what, q, out, rows, num_heads, num_kv_heads, head_dim, wind
     shape = out.shape
     if out.dtype is not q.dtype or len(shape) != 2 or shape[0] < rows or shape[1] != width or not out.is_contiguous():
         _refuse(what, f"out is contiguous {q.dtype} [at least {rows}, {width}], got {out.dtype} {tuple(shape)}")
+    if out.data_ptr() % 16:
+        _refuse(what, "out does not start on a 16-byte boundary")
     if not (0 <= window < 2 ** 31 and 0 <= keep_first < 2 ** 31):
         _refuse(what, f"window {window} and keep_first {keep_first} are not negative, and fit 31 bits")
     if not scale > 0.0:
@@ -217,7 +223,7 @@ def _float_attention(what, q, q_stride, out, kv_cache, kv_scales, pages, block_t
     """The kernel that takes every shape: portions by (indptr, kv_len), single tokens by (req, pos)."""
     group, sms = num_heads // num_kv_heads, _sms(q.get_device())
     rows = max_q * group
-    if head_dim in KV8_DECODE_HEAD_DIMS and (kv_cache.data_ptr() | out.data_ptr()) % 16 == 0:
+    if head_dim in KV8_DECODE_HEAD_DIMS and kv_cache.data_ptr() % 16 == 0:
         few = rows <= 16
         splits = kv8_mma_splits((1 if few else -(-rows // 64)) * num_kv_heads * count,
                                 _most_keys(max_len, max_q if few else min(max_q, 63 // group + 2), window, keep_first),
@@ -229,7 +235,7 @@ def _float_attention(what, q, q_stride, out, kv_cache, kv_scales, pages, block_t
     part, part_o, part_ml = _parts(q, tokens, num_heads, head_dim, splits)
     check(lib.get("attention_kv8").mstar_kv8_attention_packed(_pack_float(
         q.data_ptr(), q_stride, out.data_ptr(), _DT[q.dtype], kv_cache.data_ptr(), kv_scales.data_ptr(), pages,
-        block_table.data_ptr(), table, indptr, kv_len, req, pos, first_entry, count, max_q, tokens, num_heads,
+        block_table.data_ptr(), *table, indptr, kv_len, req, pos, first_entry, count, max_q, tokens, num_heads,
         num_kv_heads, head_dim, page_size, window, keep_first, scale, splits, part_o, part_ml, _stream())), what)
     if splits > 1:
         lib.add_launches(1)                     # the kernel that joins the parts
@@ -277,13 +283,13 @@ def paged_decode_attention_kv8(q: torch.Tensor, out: torch.Tensor, kv_cache: tor
     """Attention of ``tokens`` single-query rows (row i of q, out, token_req and cache_pos) over an 8-bit
     cache: the token at place p of its request sees the keys up to p; with ``window`` W > 0 the keys
     p - W + 1 .. p and those below ``keep_first``.  q [tokens, at least num_heads * head_dim], out
-    contiguous [tokens, num_heads * head_dim], both float32 or bfloat16; ``max_len`` bounds the keys of any
-    request (it decides how the work is cut, not what is computed).  A token at a place below 0 gives
-    zeros."""
+    contiguous [tokens, num_heads * head_dim] on a 16-byte boundary, both float32 or bfloat16;
+    ``max_len`` bounds the keys of any request (it decides how the work is cut, not what is computed).
+    A token at a place below 0 gives zeros."""
     what = "paged_decode_attention_kv8"
     q_stride = _check_attention(what, q, out, tokens, num_heads, num_kv_heads, head_dim, window, keep_first, scale)
     pages = _check_cache(what, kv_cache, kv_scales, num_kv_heads, page_size, head_dim)
-    table = _check_table(what, block_table)
+    table = _check_table(what, block_table, read=True)
     _check_index(what, token_req, tokens)
     _check_index(what, cache_pos, tokens)
     device = q.get_device()
@@ -300,7 +306,7 @@ def paged_decode_attention_kv8(q: torch.Tensor, out: torch.Tensor, kv_cache: tor
         pairs = tokens * num_kv_heads * -(-num_heads // num_kv_heads // 8)
         blocks, warps = kv8_decode_shape(pairs, most, head_dim, _sms(device))
         check(lib.get("attention_kv8_decode").mstar_kv8_decode_packed(_pack_decode(
-            q_ptr, q_stride, out.data_ptr(), codes, scales, pages, block_table.data_ptr(), table, token_req.data_ptr(),
+            q_ptr, q_stride, out.data_ptr(), codes, scales, pages, block_table.data_ptr(), *table, token_req.data_ptr(),
             cache_pos.data_ptr(), tokens, num_heads, num_kv_heads, head_dim, page_size, window, keep_first, scale, blocks,
             warps, _stream())), what)
         return
@@ -321,7 +327,7 @@ def paged_prefill_attention_kv8(q: torch.Tensor, out: torch.Tensor, kv_cache: to
     what = "paged_prefill_attention_kv8"
     q_stride = _check_attention(what, q, out, 0, num_heads, num_kv_heads, head_dim, window, keep_first, scale)
     pages = _check_cache(what, kv_cache, kv_scales, num_kv_heads, page_size, head_dim)
-    table, rows = _check_table(what, block_table), out.shape[0]
+    table, rows = _check_table(what, block_table, read=True), out.shape[0]
     if first_entry < 0 or q.shape[0] < rows:
         _refuse(what, "first_entry is not negative, and q has a row for every row of out")
     last = first_entry + max(entries, 0)
@@ -341,14 +347,14 @@ def paged_prefill_attention_kv8(q: torch.Tensor, out: torch.Tensor, kv_cache: to
     most = _most_keys(max_kv_len, max_q_len, window, keep_first)
     q_ptr, out_ptr, codes = q.data_ptr(), out.data_ptr(), kv_cache.data_ptr()
     if (q.dtype is _BF16 and head_dim in KV8_TC_HEAD_DIMS and group <= 128 and q_stride % 8 == 0
-            and (q_ptr | codes | out_ptr) % 16 == 0):
+            and (q_ptr | codes) % 16 == 0):
         per_tile = 128 // group
         tiles = -(-max_q_len // (2 * per_tile))
         splits, pair = kv8_tc_splits(tiles * num_kv_heads * entries, most, _sms(device), max_q_len <= per_tile)
         tokens = min(rows, entries * max_q_len)
         part, part_o, part_ml = _parts(q, tokens, num_heads, head_dim, splits)
         check(lib.get("attention_kv8_tc").mstar_kv8_attention_tc_packed(_pack_portions(
-            q_ptr, q_stride, out_ptr, codes, kv_scales.data_ptr(), pages, block_table.data_ptr(), table,
+            q_ptr, q_stride, out_ptr, codes, kv_scales.data_ptr(), pages, block_table.data_ptr(), *table,
             qo_indptr.data_ptr(), kv_len.data_ptr(), first_entry, entries, max_q_len, tokens, num_heads, num_kv_heads,
             head_dim, page_size, window, keep_first, scale, splits, pair, part_o, part_ml, _error_ptr(q),
             _stream())), what)

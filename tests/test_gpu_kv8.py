@@ -90,6 +90,36 @@ def test_write_and_read_back(act, nq, nkv, hd, rot, inter, page, start):
     assert (codes == 0x55).all() and (scales == 99).all()
 
 
+@pytest.mark.parametrize("act", [F32, BF16])
+@pytest.mark.parametrize("inter", [False, True])
+def test_rotated_keys_get_their_nearest_codes(act, inter):
+    """Four million numbers, some of them next to the border of two codes.  The rotation is off by half a step of a
+    float of the result (2^-24) and 2^-38 of the two products; what is held is then the nearest code's value: off by half
+    a code's step of the exact result, and by that much."""
+    from mstar_b200 import ops
+
+    T, nkv, hd, page = 4096, 8, 128, 64
+    g = torch.Generator(device=DEV).manual_seed(5)
+    qkv = torch.randn(T, (1 + 2 * nkv) * hd, generator=g, device=DEV).to(act)
+    pos, at, req = i32(range(90_000, 90_000 + T)), i32(range(T)), i32([0] * T)
+    codes = torch.zeros(T // page, 2, nkv, page, hd, dtype=torch.uint8, device=DEV).view(torch.float8_e4m3fn)
+    scales = torch.zeros(T // page, 2, nkv, page, dtype=torch.uint8, device=DEV)
+    table = i32([list(range(T // page))])
+    ops.rope_kv8_write(qkv, pos, at, req, table, freqs(hd), codes, scales, 1, nkv, hd, hd, inter, page)
+    got = ops.kv8_read_rows(codes, scales, table, req, at, F32)[:, 0].double()
+    x = qkv[:, hd:(1 + nkv) * hd].double().view(T, nkv, hd)
+    angle = (pos.double()[:, None] * freqs(hd).double())[:, None]
+    lo, hi = (slice(0, hd, 2), slice(1, hd, 2)) if inter else (slice(0, hd // 2), slice(hd // 2, hd))
+    want, size = torch.empty_like(x), torch.empty_like(x)
+    want[..., lo] = x[..., lo] * angle.cos() - x[..., hi] * angle.sin()
+    want[..., hi] = x[..., hi] * angle.cos() + x[..., lo] * angle.sin()
+    size[..., lo] = size[..., hi] = x[..., lo].abs() + x[..., hi].abs()
+    unit = torch.exp2(scales[:, 0].permute(0, 2, 1).reshape(T, nkv, 1).double() - 127.0)
+    step = unit * torch.exp2((want.abs() / unit).clamp(min=2.0 ** -6).log2().floor() - 3)
+    off = (got - want).abs() - step / 2
+    assert (off <= 2.0 ** -24 * want.abs() + 2.0 ** -38 * size).all()
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("nkv,hd,page", [(2, 64, 16), (3, 24, 7), (1, 256, 64), (8, 128, 1)])
 def test_read_rows(dtype, nkv, hd, page):
@@ -369,6 +399,65 @@ def test_the_same_call_twice_gives_the_same_bits(act):
     assert torch.equal(c.decode(), c.decode())
     c = Case([30, 90], [2000, 900], 8, 2, 128, 16, act, seed=16)
     assert torch.equal(c.prefill(), c.prefill())
+
+
+@pytest.mark.parametrize("act", [F32, BF16])
+@pytest.mark.parametrize("hd", [48, 64, 128])
+def test_tables_that_are_part_of_wider_ones(act, hd):
+    """A view of some columns: what lies beside them belongs to somebody else, and is neither written nor read."""
+    from mstar_b200 import ops
+
+    nq, nkv, page = 4, 2, 16
+    c = Case([1, 1, 20], [30, 47, 60], nq, nkv, hd, page, act, seed=31)
+    wide = torch.full((3, c.table.shape[1] + 3), 0, dtype=torch.int32)
+    wide[:, 2:-1] = c.table
+    view = wide.to(DEV)[:, 2:-1]
+    codes, scales = c.cache()
+    out = torch.full((22, nq * hd), 7.0, dtype=act, device=DEV)
+    q = c.q.to(DEV)
+    ops.paged_decode_attention_kv8(q, out, codes, scales, view, c.i32(c.req), c.i32(c.pos), 2, nq, nkv, hd, page, 0, 0,
+                                   c.scale, 60)
+    ops.paged_prefill_attention_kv8(q, out, codes, scales, view, c.i32(c.indptr), c.i32(c.lens_kv), 2, 1, 20, nq, nkv, hd,
+                                    page, 0, 0, c.scale, 60)
+    c.check(out)
+    # places behind the view's last page: its neighbour in the wide table names page 0
+    before = codes.view(torch.uint8).clone(), scales.clone()
+    past = view.shape[1] * page
+    ops.rope_kv8_write(torch.randn(2, (nq + 2 * nkv) * hd, device=DEV).to(act), i32([0, 1]), i32([past, past + 1]), i32([0, 2]),
+                       view, None, codes, scales, nq, nkv, hd, 0, False, page)
+    assert torch.equal(codes.view(torch.uint8), before[0]) and torch.equal(scales, before[1])
+    assert not ops.kv8_read_rows(codes, scales, view, i32([0, 2]), i32([past, past + 1]), act).any()
+
+
+@pytest.mark.parametrize("act", [F32, BF16])
+@pytest.mark.parametrize("hd", [48, 64, 128])
+@pytest.mark.parametrize("max_q", [1, 30])
+def test_portions_longer_than_their_bound_stay_inside_the_parts(monkeypatch, act, hd, max_q):
+    """``max_q_len`` below the tokens that an entry has: those beyond are not computed, and nothing is written behind
+    the memory for the parts or into other rows."""
+    from mstar_b200 import ops
+    from mstar_b200.ops import kv8
+
+    made = []
+
+    def parts(q, tokens, heads, dim, splits):
+        assert splits > 1
+        n = tokens * heads * splits
+        t = torch.full((n * (dim + 2) + 500_000,), 7.0, dtype=F32, device=DEV)
+        made.append((t, n * (dim + 2)))
+        return t, t.data_ptr(), t.data_ptr() + 4 * n * dim
+
+    c = Case([40, 40], [900, 800], 4, 1, hd, 16, act, seed=33)
+    monkeypatch.setattr(kv8, "_parts", parts)
+    out = torch.full((80 + 3, 4 * hd), 3.0, dtype=act, device=DEV)
+    q = torch.cat([c.q, torch.zeros(3, 4 * hd, dtype=act)]).to(DEV)
+    c.prefill(out=out, q=q, max_q=max_q)
+    torch.cuda.synchronize()
+    assert made and all((t[n:] == 7).all() for t, n in made)
+    assert (out[80:] == 3).all()
+    want, bound = c.plain()
+    good = (out[:max_q].double().cpu() - want[:max_q]).abs() <= bound[:max_q]
+    assert good.all()
 
 
 def test_nothing_to_do():

@@ -126,6 +126,25 @@ def test_refusals(name, changes, match):
         getattr(ops, name)(**args(name, **changes))
 
 
+@pytest.mark.parametrize("name", ["paged_decode_attention_kv8", "paged_prefill_attention_kv8"])
+def test_refuses_outputs_off_the_boundary_and_tables_without_pages(name):
+    out = Z(3 * 256 + 1)[1:].view(3, 256)
+    with pytest.raises(ops.KernelError, match="16-byte"):
+        getattr(ops, name)(**args(name, out=out))
+    with pytest.raises(ops.KernelError, match="no pages"):
+        getattr(ops, name)(**args(name, block_table=Z(2, 0, dtype=torch.int32)))
+
+
+def test_splits_of_the_tensor_core_kernels():
+    from mstar_b200.ops.kv8 import kv8_mma_splits, kv8_tc_splits
+
+    assert kv8_mma_splits(256, 220, 148, False) == 1 and kv8_mma_splits(152, 1000, 148, False) == 2
+    assert kv8_mma_splits(8, 10 ** 6, 148, True) == 4 * 28 and kv8_mma_splits(8, 100, 148, True) == 4
+    assert kv8_mma_splits(1, 10 ** 6, 148, False) == 64 and kv8_mma_splits(1, 10 ** 6, 148, True) == 256
+    assert kv8_tc_splits(16, 20017, 148, True) == (18, True) and kv8_tc_splits(16, 20017, 148, False) == (9, False)
+    assert kv8_tc_splits(16, 4000, 148, True) == (9, False) and kv8_tc_splits(200, 511, 148, True) == (1, False)
+
+
 def test_refuses_head_sizes_that_have_no_form():
     for hd in (12, 264):
         assert not ops.kv8_supported(hd)
