@@ -35,6 +35,11 @@
 // one barrier; reading it from there took 4,100 clocks, a wait for every block in turn): one launch, no scratch
 // memory, sums in a fixed order.
 //
+// A warp's ring is two tiles, so that twelve warps of head_dim 128 fit an SM instead of eight (sixteen of 64): its
+// instructions, issued in order and each waiting for the last, bound it, not the copies.  64 requests on 2,048 keys,
+// 8 kv heads of 128: 42 us (47 with three tiles; 30 at the copy bandwidth), one on 16,384: 15.2, 64 on windows of 1,024
+// keys of 64: 17.5.
+//
 // Semantics are those of attention_generic.cu.
 #include <cooperative_groups.h>
 #include <cuda_fp16.h>
@@ -98,7 +103,7 @@ __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.w
 __device__ __forceinline__ float ratio(float a, float b) { return a == -INFINITY ? 0.f : ex2(a - b); }
 
 #define DEC8_KEYS 32     // keys of a tile
-#define DEC8_STAGES 3    // tiles of a warp's ring
+#define DEC8_STAGES 2    // tiles of a warp's ring
 #define DEC8_SLACK 8.f   // how far (in powers of two) scores may exceed the maxima
 // Shared memory of a warp: tiles of keys and of values (blocks of [32 rows x at most 128 bytes], swizzled), then a scale
 // pair a key, then each tile's scale bytes; the outputs that the warps leave at the end lie over the tiles.
@@ -107,8 +112,8 @@ template <int D> __host__ __device__ constexpr int dec8_stage() { return 2 * dec
 template <int D> __host__ __device__ constexpr int dec8_ring() { return DEC8_STAGES * dec8_stage<D>() + DEC8_KEYS * 8; }
 // Of a block: the warps' statistics, the blocks' statistics [16][H][4], and a place for the parts of all blocks of what
 // this block joins, [C][H][D / C].
-template <int D> __host__ __device__ constexpr int dec8_smem(int warps) {
-    return warps * dec8_ring<D>() + (warps * 32 + 16 * 32 + 8 * D) * 4;
+template <int D, int H> __host__ __device__ constexpr int dec8_smem(int warps, int blocks) {
+    return warps * dec8_ring<D>() + (warps * 32 + (blocks > 1 ? 16 * 32 + H * D : 0)) * 4;
 }
 template <int D> __host__ __device__ constexpr int dec8_most_warps() { return D == 64 ? 16 : D == 128 ? 8 : 4; }
 
@@ -545,7 +550,7 @@ kv8_decode_kernel(Kv8DecodeArgs a) {
 template <int D, int H>
 static int launch_decode(const Kv8DecodeArgs& a, int tokens, int blocks, int warps, cudaStream_t s) {
     auto kernel = kv8_decode_kernel<D, H>;
-    const int smem = dec8_smem<D>(warps);
+    int smem = dec8_smem<D, H>(warps, blocks);
     if (warps < 1 || warps > dec8_most_warps<D>() || smem > 227 * 1024) return -1;
     static bool configured[64] = {false};
     int dev = 0;
@@ -563,6 +568,11 @@ static int launch_decode(const Kv8DecodeArgs& a, int tokens, int blocks, int war
     }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(blocks * a.nkv * a.head_groups, tokens);
+    // No more blocks an SM than an even share: with room for more, some SMs take them and others none (256 blocks of four
+    // warps: 10.6 us, 9.1 so).  Clusters do not fill a group of SMs to the last place: the larger, the more is left free.
+    const long long all = (long long)cfg.gridDim.x * tokens * (blocks >= 8 ? 13 : blocks == 4 ? 11 : 10) / 10;
+    const long long share = (all + device_sm_count() - 1) / device_sm_count();
+    smem = max(smem, (int)min(227ll * 1024, 228 * 1024 / (share + 1) - 896));
     cfg.blockDim = dim3(32 * warps);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;

@@ -16,6 +16,7 @@ The reference's caches hold the compute type only (mstar/engine/kv_cache_engine.
 """
 from __future__ import annotations
 
+import functools
 from struct import Struct
 
 import torch
@@ -244,17 +245,34 @@ def _float_attention(what, q, q_stride, out, kv_cache, kv_scales, pages, block_t
 KV8_DECODE_HEAD_DIMS = (64, 128, 256)
 
 
-def kv8_decode_shape(pairs: int, max_keys: int, head_dim: int, sms: int) -> tuple:
-    """(blocks of a cluster, warps of a block) that share the keys of each of ``pairs`` (token, kv head,
-    8 query heads) in the decode kernel: about seven warps an SM, none without a tile of 32 keys; blocks
-    of four warps, of eight where the pairs are few.  (8 x 8, 4 x 4 and 1 x 4 for 8, 64 and 512 pairs took
-    15.3, 9.1 and 18.2 us; half and twice the blocks 22.2 and 23.2, 12.5 and 15.4, - and 24.9.)"""
-    want = max(1, min(-(-max_keys // 32), 7 * sms // max(pairs, 1)))
-    warps = 4 if want <= 32 or head_dim == 256 else 8
-    blocks = 1
-    while blocks < 8 and blocks * warps < want:
-        blocks *= 2
-    return blocks, warps
+@functools.lru_cache(maxsize=4096)
+def kv8_decode_shape(pairs: int, max_keys: int, head_dim: int, few: bool, sms: int) -> tuple:
+    """(blocks of a cluster, warps of a block) that share the keys of each of ``pairs`` (token, kv head, 8
+    query heads; ``few``: 4) in the decode kernel.  All blocks run at once (larger clusters leave SMs
+    free), with the smallest share of a pair's keys on the SM that has most; among those clusters of two
+    at most where that does, and then as many warps as fit.  Where no shape runs at once: single blocks of
+    four.  (Heads of 128, 3 a kv head, 2,048 keys, measured with 16 shapes each: 8, 24, 64, 128, 256, 400, 512
+    pairs take 5.7 with 8 x 8, 6.9 with 4 x 8, 9.6 with 2 x 8, 15.7 with 2 x 6, 23.5 with 1 x 6, 32.8 with 1 x 4,
+    42.2 with 1 x 3, which is the best or within 0.4 us of it; 1 x 4 takes 18.3, 22.3, 26.5, 32.8 and 47.1 for
+    the last five.)"""
+    heads = 4 if few else 8
+    # a warp's two tiles of 32 keys and values with their scales; warps that the registers allow an SM
+    ring, most = 2 * 64 * (head_dim + 1) + 256, 16 if head_dim == 64 or (few and head_dim == 128) else 8
+    tiles = max(1, -(-max_keys // 32))
+    best = None
+    for blocks in (1, 2, 4, 8):
+        if blocks > tiles:
+            break
+        for warps in ((8, 6, 4, 3) if most == 16 and head_dim == 128 else (8, 4) if head_dim < 256 else (4,)):
+            warps = min(warps, -(-tiles // blocks))
+            smem = warps * (ring + 128) + (4 * (512 + heads * head_dim) if blocks > 1 else 0) + 1024
+            room = min(most // warps, 228 * 1024 // smem)
+            if pairs * blocks * max(1.0, 1 + 0.05 * (blocks - 2) / room) > room * sms:
+                continue
+            key = (-(-pairs * blocks // sms) / blocks, max(blocks, 2), -blocks * warps, blocks)
+            if best is None or key < best[0]:
+                best = key, (blocks, warps)
+    return best[1] if best else (1, min(4, tiles))
 
 
 KV8_TC_HEAD_DIMS = (64, 128)
@@ -304,7 +322,7 @@ def paged_decode_attention_kv8(q: torch.Tensor, out: torch.Tensor, kv_cache: tor
     if (q.dtype is _BF16 and head_dim in KV8_DECODE_HEAD_DIMS and page_size % 8 == 0 and q_stride % 8 == 0
             and (q_ptr | codes) % 16 == 0 and scales % 8 == 0):
         pairs = tokens * num_kv_heads * -(-num_heads // num_kv_heads // 8)
-        blocks, warps = kv8_decode_shape(pairs, most, head_dim, _sms(device))
+        blocks, warps = kv8_decode_shape(pairs, most, head_dim, num_heads <= 4 * num_kv_heads, _sms(device))
         check(lib.get("attention_kv8_decode").mstar_kv8_decode_packed(_pack_decode(
             q_ptr, q_stride, out.data_ptr(), codes, scales, pages, block_table.data_ptr(), *table, token_req.data_ptr(),
             cache_pos.data_ptr(), tokens, num_heads, num_kv_heads, head_dim, page_size, window, keep_first, scale, blocks,

@@ -135,6 +135,23 @@ def test_refuses_outputs_off_the_boundary_and_tables_without_pages(name):
         getattr(ops, name)(**args(name, block_table=Z(2, 0, dtype=torch.int32)))
 
 
+def test_shapes_of_the_decode_kernel():
+    """Blocks of a pair times pairs fit the GPU at once wherever some shape does, and no warp is without a tile."""
+    from mstar_b200.ops.kv8 import kv8_decode_shape
+
+    for hd in (64, 128, 256):
+        for few in (True, False):
+            for keys in (1, 31, 33, 100, 1000, 100_000):
+                for pairs in (1, 2, 7, 8, 16, 64, 100, 148, 149, 296, 500, 1000, 10 ** 5):
+                    blocks, warps = kv8_decode_shape(pairs, keys, hd, few, 148)
+                    tiles = -(-keys // 32)
+                    assert blocks in (1, 2, 4, 8) and 1 <= warps <= (4 if hd == 256 else 8)
+                    assert blocks <= tiles and (blocks - 1) * warps < tiles
+                    assert pairs > 148 or pairs * blocks <= 148 * 4
+    assert kv8_decode_shape(8, 16384, 128, True, 148) == (8, 8)
+    assert kv8_decode_shape(512, 2048, 128, True, 148) == (1, 3)
+
+
 def test_splits_of_the_tensor_core_kernels():
     from mstar_b200.ops.kv8 import kv8_mma_splits, kv8_tc_splits
 
