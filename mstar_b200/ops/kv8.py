@@ -257,13 +257,13 @@ def kv8_decode_shape(pairs: int, max_keys: int, head_dim: int, few: bool, sms: i
     the last five.)"""
     heads = 4 if few else 8
     # a warp's two tiles of 32 keys and values with their scales; warps that the registers allow an SM
-    ring, most = 2 * 64 * (head_dim + 1) + 256, 16 if head_dim == 64 or (few and head_dim == 128) else 8
+    ring, most = 2 * 64 * (head_dim + 1) + 256, 16 if head_dim == 64 else 12 if few and head_dim == 128 else 8
     tiles = max(1, -(-max_keys // 32))
     best = None
     for blocks in (1, 2, 4, 8):
         if blocks > tiles:
             break
-        for warps in ((8, 6, 4, 3) if most == 16 and head_dim == 128 else (8, 4) if head_dim < 256 else (4,)):
+        for warps in ((8, 6, 4, 3) if most == 12 else (8, 4) if head_dim < 256 else (4,)):
             warps = min(warps, -(-tiles // blocks))
             smem = warps * (ring + 128) + (4 * (512 + heads * head_dim) if blocks > 1 else 0) + 1024
             room = min(most // warps, 228 * 1024 // smem)
