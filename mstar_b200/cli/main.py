@@ -55,6 +55,12 @@ def _prompts(args) -> list:
     return prompts
 
 
+def _deployed_kv_dtype(kv: dict):
+    """The ``dtype`` of a deployment's ``kv_cache`` section; a compute type's name says what is so anyway."""
+    dtype = kv.get("dtype")
+    return None if dtype in ("bfloat16", "float16", "float32") else dtype
+
+
 def _generate(args) -> None:
     if args.gpus is not None:
         os.environ["CUDA_VISIBLE_DEVICES"] = args.gpus
@@ -73,7 +79,7 @@ def _generate(args) -> None:
               max_concurrent_requests=args.max_concurrent_requests
               or deploy.get("max_concurrent_requests", 64),
               log_stats=args.log_stats or bool(args.log_stats_file),
-              kv_cache_dtype=args.kv_cache_dtype or kv.get("dtype"))
+              kv_cache_dtype=args.kv_cache_dtype or _deployed_kv_dtype(kv))
     d = GenerationDefaults.from_folder(args.model)
 
     def pick(value, default):

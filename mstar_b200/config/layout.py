@@ -141,7 +141,6 @@ class AttentionSpec:
                 and self.chunk is None and self.weights == "softmax" and not self.score_bias
                 and self.value_mix is None)
 
-
     @property
     def eight_bit(self) -> bool:
         """Whether its keys and values can be kept in 8 bits: the plain attention, which may keep

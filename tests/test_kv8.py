@@ -176,6 +176,13 @@ def test_splits_fill_the_gpu_and_keep_parts_long():
     assert ops.kv8_splits(1, 100, 148) == 1 and ops.kv8_splits(1, 10 ** 6, 148) == 64
 
 
+def test_deployment_may_name_the_type():
+    from mstar_b200.cli.main import _deployed_kv_dtype
+
+    assert _deployed_kv_dtype({}) is None and _deployed_kv_dtype({"dtype": "bfloat16"}) is None
+    assert _deployed_kv_dtype({"dtype": "float8_e4m3"}) == "float8_e4m3"
+
+
 def test_command_line_takes_the_type():
     from mstar_b200.cli.main import build_parser
 
