@@ -5,9 +5,9 @@
 // a byte and head.  So the kernel is built around having copies in flight: every warp has a ring of tiles of 32 keys
 // of its own in shared memory, filled by asynchronous copies of 16 bytes a thread with the tiles after the one it works
 // on, and no warp waits for another before the end.  (TMA boxes of a page's rows took some 700 clocks a tile to issue
-// from one thread and 800 from several, against 350: 18.0 us for one token on 16,384 keys where these take 15.7.  Loads
+// from one thread and 800 from several, against 350: 18.0 us for one token on 16,384 keys where these take 15.2.  Loads
 // into registers a step ahead are waited for where the registers are handed on: 52 us for 64 requests with a window of
-// 1,024 keys against 18.6.)  The products run on the tensor cores with the keys as rows, since 16 rows of queries would be mostly padding:
+// 1,024 keys against 17.6.)  The products run on the tensor cores with the keys as rows, since 16 rows of queries would be mostly padding:
 //   S^T [16 keys x 8 heads] += K [16 x 16] Q^T [16 x 8],   O^T [16 features x 8 heads] += V^T [16 x 16 keys] P^T.
 // Which feature or key a fragment's element stands for is free as long as both operands agree.  So a thread's operands
 // are runs of 16 bytes of a row: of K the features [16 t, 16 t + 16) and every 64 after them, of V [D/8 g, D/8 (g + 1))

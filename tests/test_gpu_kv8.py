@@ -460,6 +460,35 @@ def test_portions_longer_than_their_bound_stay_inside_the_parts(monkeypatch, act
     assert good.all()
 
 
+@pytest.mark.parametrize("act", [F32, BF16])
+@pytest.mark.parametrize("hd,page", [(128, 64), (48, 64), (256, 4)])
+def test_pages_more_than_four_gigabytes_apart(act, hd, page):
+    """The same rows on the first and on the last pages of a cache of 4.5 GB: written, read back and attended to alike."""
+    from mstar_b200 import ops
+
+    nq, nkv, n, width = 8, 4, 130, -(-130 // page)
+    pages = int(4.5e9) // (2 * nkv * page * hd)
+    codes = torch.zeros(pages, 2, nkv, page, hd, dtype=torch.uint8, device=DEV).view(torch.float8_e4m3fn)
+    scales = torch.zeros(pages, 2, nkv, page, dtype=torch.uint8, device=DEV)
+    table = i32([list(range(width)), list(range(pages - width, pages))])
+    assert int(table[1, 0]) * 2 * nkv * page * hd > 2 ** 32
+    g = torch.Generator(device=DEV).manual_seed(3)
+    qkv = torch.randn(n, (nq + 2 * nkv) * hd, generator=g, device=DEV).to(act)
+    pos, rows, got = i32(range(n)), [], []
+    for r in range(2):
+        q = ops.rope_kv8_write(qkv, pos, pos, i32([r] * n), table, freqs(hd), codes, scales, nq, nkv, hd, hd, False, page)
+        rows.append(ops.kv8_read_rows(codes, scales, table, i32([r] * n), pos, act))
+        one, all_ = torch.empty(1, nq * hd, dtype=act, device=DEV), torch.empty(n, nq * hd, dtype=act, device=DEV)
+        ops.paged_decode_attention_kv8(q[-1:], one, codes, scales, table, i32([r]), pos[-1:], 1, nq, nkv, hd, page, 0, 0,
+                                       hd ** -0.5, n)
+        ops.paged_prefill_attention_kv8(q, all_, codes, scales, table[r:r + 1], i32([0, n]), i32([n]), 0, 1, n, nq, nkv, hd,
+                                        page, 0, 0, hd ** -0.5, n)
+        got.append((one, all_))
+    assert rows[0].abs().max() > 1 and torch.equal(*rows)
+    assert torch.equal(got[0][0], got[1][0]) and torch.equal(got[0][1], got[1][1])
+    assert torch.isfinite(got[0][1]).all()
+
+
 def test_nothing_to_do():
     from mstar_b200 import ops
 
