@@ -13,9 +13,9 @@
 // is done in pairs of floats: c = c_hi + c_lo with 16 bits in c_hi, so that its product with a bfloat16 is exact, the two
 // products are added with the sum's rounding error (Knuth's two-sum), and the small parts are added to that.
 //
-// 2,048 tokens of 24 + 16 heads of 128 take 12.0 us for 38 MB (5.8 at the copy bandwidth), 999 float tokens of 48 heads of
-// 64 5.0: bound by the latency of a block's chain (position, sines in double, rotation, largest number), of which three
-// blocks an SM run at a time.  Threads with 8 features that read their partners' too, heads one after another, took 11.2
+// 2,048 tokens of 24 + 16 heads of 128 take 11.2 us for 38 MB (5.8 at the copy bandwidth), 999 float tokens of 48 heads of
+// 64 5.0: bound by the latency of a block's chain (position, sines in double, rotation, largest number), of which few
+// an SM run at a time.  Threads with 8 features that read their partners' too, heads one after another, took 11.2
 // with a rotation in float, 14.9 with the keys' in double; the next head's loads ahead, 13.3.
 //
 // The reference's cache has no 8-bit form (mstar/engine/kv_cache_engine.py:132-136).
@@ -238,9 +238,11 @@ __global__ void __launch_bounds__(512) rope_kv8_write_kernel(const A* qkv, A* q_
 
 template <typename A, int L>
 static int launch_write(const void* qkv, void* q_out, const Kv8WriteArgs& a, int tokens, bool vec, cudaStream_t s) {
-    // a token's heads in one block, so that its angles are made once; with few tokens in blocks of 128 threads
-    const long long all = (long long)(a.nq + 2 * a.nkv) * L;
-    const int threads = tokens < 256 ? 128 : (int)min(512ll, (all + 31) / 32 * 32);
+    // A token's heads in one block in the 32-bit mode, so that its angles are made once; in two in the 16-bit mode, which
+    // leaves more blocks whose chains overlap (2,048 and 512 tokens of 40 heads of 128: 11.2 and 3.7 us, 12.5 and 5.1 in one,
+    // 12.2 and 4.4 in three; 999 float tokens 5.0 in one and 5.6 in two).  With few tokens in blocks of 128 threads.
+    const long long all = (long long)(a.nq + 2 * a.nkv) * L, part = sizeof(A) == 2 ? (all + 1) / 2 : all;
+    const int threads = tokens < 256 ? 128 : (int)min(512ll, (part + 31) / 32 * 32);
     const long long slices = (all + threads - 1) / threads;
     if (slices > 65535) return -1;
     const dim3 grid(tokens, (unsigned)slices);
