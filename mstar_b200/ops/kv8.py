@@ -24,9 +24,16 @@ import torch
 from . import _DT, _error_ptr, _need_cuda, _stream, lib, num_sms
 from .lib import KernelError, check
 
+try:
+    # (size, stride, dtype) on the current device: 0.7 us a call, where Tensor.new_empty takes 1.8
+    from torch._C._dynamo.guards import _empty_strided_cuda as _empty
+except ImportError:
+    def _empty(size, stride, dtype):
+        return torch.empty_strided(size, stride, dtype=dtype, device=torch.device("cuda", _device()))
+
 KV8_DTYPE = torch.float8_e4m3fn
 _INT = torch.int32
-_F32, _BF16 = torch.float32, torch.bfloat16
+_F32, _BF16, _BYTE = torch.float32, torch.bfloat16, torch.uint8
 _device = torch._C._cuda_getDevice
 # the entry points' arguments as one string (csrc/kv8.cuh)
 _pack_write = Struct("=22q").pack
@@ -57,18 +64,19 @@ def _refuse(what: str, why: str) -> None:
 
 def _check_cache(what, kv_cache, kv_scales, num_kv_heads, page_size, head_dim) -> int:
     """The cache's pages."""
-    shape = kv_cache.shape
-    if kv_cache.dtype is not KV8_DTYPE or kv_scales.dtype is not torch.uint8:
+    if kv_cache.dtype is not KV8_DTYPE or kv_scales.dtype is not _BYTE:
         _refuse(what, f"the cache holds {KV8_DTYPE} codes and uint8 scales, got {kv_cache.dtype} and {kv_scales.dtype}")
-    if len(shape) != 5 or shape[0] < 1 or shape[1:] != (2, num_kv_heads, page_size, head_dim):
+    shape = kv_cache.shape
+    pages = shape[0] if shape else 0
+    if pages < 1 or shape != (pages, 2, num_kv_heads, page_size, head_dim):
         _refuse(what, f"the cache's shape {tuple(shape)} is not (pages, 2, {num_kv_heads}, {page_size}, {head_dim})")
-    if kv_scales.shape != shape[:4]:
+    if kv_scales.shape != (pages, 2, num_kv_heads, page_size):
         _refuse(what, f"the scales' shape {tuple(kv_scales.shape)} is not the cache's {tuple(shape[:4])}")
     if not (kv_cache.is_contiguous() and kv_scales.is_contiguous()):
         _refuse(what, "the cache and its scales must be contiguous")
     if head_dim % 8 or not 0 < head_dim <= 256:
         _refuse(what, f"head_dim {head_dim} is not a multiple of 8 up to 256")
-    return shape[0]
+    return pages
 
 
 def _check_table(what, block_table, read=False) -> tuple:
@@ -131,7 +139,7 @@ def rope_kv8_write(qkv: torch.Tensor, positions, cache_pos, token_req, block_tab
             device == positions.get_device() == cache_pos.get_device() == token_req.get_device()
             == block_table.get_device() == kv_cache.get_device() == kv_scales.get_device() == _device()):
         _refuse_device(what, qkv, positions, cache_pos, token_req, block_table, kv_cache, kv_scales)
-    q = qkv.new_empty((n, num_heads * head_dim))
+    q = _empty((n, num_heads * head_dim), (num_heads * head_dim, 1), qkv.dtype)
     if n == 0:
         return q
     check(lib.get("kv8_cache").mstar_rope_kv8_write_packed(_pack_write(
@@ -162,7 +170,8 @@ def kv8_read_rows(kv_cache: torch.Tensor, kv_scales: torch.Tensor, block_table, 
             device == kv_scales.get_device() == block_table.get_device() == token_req.get_device()
             == cache_pos.get_device() == _device()):
         _refuse_device(what, kv_cache, kv_scales, block_table, token_req, cache_pos)
-    out = kv_scales.new_empty((n, 2, heads, head_dim), dtype=dtype)
+    row = heads * head_dim
+    out = _empty((n, 2, heads, head_dim), (2 * row, row, head_dim, 1), dtype)
     if n:
         check(lib.get("kv8_cache").mstar_kv8_read_rows_packed(_pack_read(
             kv_cache.data_ptr(), kv_scales.data_ptr(), block_table.data_ptr(), *table, token_req.data_ptr(),
@@ -214,7 +223,7 @@ def _parts(q, tokens, num_heads, head_dim, splits) -> tuple:
     if splits == 1:
         return None, 0, 0
     rows = tokens * num_heads * splits
-    t = q.new_empty(rows * (head_dim + 2), dtype=_F32)
+    t = _empty((rows * (head_dim + 2),), (1,), _F32)
     return t, t.data_ptr(), t.data_ptr() + 4 * rows * head_dim
 
 
