@@ -212,6 +212,17 @@ def test_portions(act, nq, nkv, hd, page, window, keep):
 
 
 @pytest.mark.parametrize("act", [F32, BF16])
+@pytest.mark.parametrize("nq,nkv,hd,page", [(6, 2, 128, 4), (3, 1, 64, 5), (140, 1, 64, 16), (130, 1, 128, 7), (9, 3, 256, 1)])
+@pytest.mark.parametrize("window,keep", [(0, 0), (40, 2)])
+def test_odd_pages_and_many_heads_a_kv_head(act, nq, nkv, hd, page, window, keep):
+    """Pages that groups of eight keys cross, and more query heads a kv head than a tile of the portions' kernel has rows."""
+    c = Case([1, 1, 1], [1, 67, 300], nq, nkv, hd, page, act, seed=41, window=window, keep=keep)
+    c.check(c.decode())
+    c = Case([3, 1, 30], [3, 67, 150], nq, nkv, hd, page, act, seed=42, window=window, keep=keep)
+    c.check(c.prefill())
+
+
+@pytest.mark.parametrize("act", [F32, BF16])
 @pytest.mark.parametrize("hd", [64, 128])
 def test_one_long_request(act, hd):
     """Few rows on many keys: the keys are shared out over blocks and joined."""
