@@ -3,8 +3,8 @@
 // head sizes 64, 128 and 256 on the tensor cores (second half of this file), others that are multiples of 8 up to 256 in
 // float arithmetic on CUDA cores.
 //
-// On CUDA cores: a row is (token, query head of the group); R rows of one request and kv head make a block, which walks the keys
-// that some of its rows see (kept first keys, then the window) in tiles of 64: codes become floats times their row's
+// On CUDA cores: a row is (token, query head of the group); R rows of one request and kv head make a block, which walks the
+// keys that some of its rows see (kept first keys, then the window) in tiles of 64: codes become floats times their row's
 // scale in shared memory (keys transposed), S = Q K^T and O += P V by outer products in registers, softmax statistics
 // per row in registers.  R = 64 for portions (4 x 4 scores a thread), 8 for single tokens (a warp a row).  Where there
 // are few row tiles the keys are cut into `splits` parts whose (maximum, sum, output) go to scratch memory.
@@ -286,7 +286,8 @@ template <int HD, int PARTS, int NT> __host__ __device__ constexpr int km_smem()
 
 template <typename A, int HD, int PARTS, int NT>
 __global__ void __launch_bounds__(128) kv8_attention_mma_kernel(Kv8AttnArgs a) {
-    constexpr int ROWS = NT == 8 ? 64 : 16, RB = HD < 128 ? HD : 128, KC = HD / 64, VW = HD / 32, MT = HD / 8, NB = NT < 4 ? NT : 4;
+    constexpr int ROWS = NT == 8 ? 64 : 16, RB = HD < 128 ? HD : 128, KC = HD / 64, VW = HD / 32, MT = HD / 8;
+    constexpr int NB = NT < 4 ? NT : 4;                  // products side by side
     constexpr int QP = HD * 2 + 16;                      // bytes of a row of queries in shared memory
     constexpr int S = km_stages<NT>();
     extern __shared__ __align__(128) unsigned char smem_m[];

@@ -19,10 +19,10 @@
 // portions of 17 tokens on 20,000 keys, 42.6 without; with row tiles that differ, 588 instead of 568 below).
 //
 // What else was built: two buffers of 64 keys a row tile in the same tensor memory, so that scores are made ahead (601 us
-// for 2,048 tokens on 14,336 keys, when this took 565: products of 64 keys read the queries from shared memory twice as often); the
-// same with two threads a row, which take its steps in turn (571: the exponentials are the same); half a row a thread
-// (754: the halves have to meet at every tile); an eighth, a quarter or a third of the exponentials by a polynomial (571, 632,
-// 660 when this took 558: the issue slots are what the softmax lacks, not the special function unit).
+// for 2,048 tokens on 14,336 keys, when this took 565: products of 64 keys read the queries from shared memory twice as
+// often); the same with two threads a row, which take its steps in turn (571: the exponentials are the same); half a row a
+// thread (754: the halves have to meet at every tile); an eighth, a quarter or a third of the exponentials by a polynomial
+// (571, 632, 660 when this took 558: the issue slots are what the softmax lacks, not the special function unit).
 // Tensor memory: S / P 2 x 128 columns, O 2 x head_dim.  Shared memory (head_dim 128): queries 64 KB, two stages of keys
 // of 16 KB and two of values of 32 KB each.
 //
@@ -75,9 +75,11 @@ struct Kv8TcArgs {
 
 __host__ __device__ constexpr int k8_codes(int hd) { return 128 * hd; }          // a tile of codes: 128 rows
 __host__ __device__ constexpr int k8_values(int hd) { return K8_KEYS * hd * 2; }
-// queries [2 row tiles, PAIR: one][hi, lo], PAIR: values on their way, two stages of keys and of values, of eight tiles each key's row, factor and value factor,
-// outputs on their way, the barriers
-__host__ __device__ constexpr int k8_smem(int hd, bool pair) { return (pair ? 4 + K8_AHEAD : 6) * k8_codes(hd) + 2 * k8_values(hd) + 8 * 128 * 12 + 256 * 128 + 256; }
+// queries [2 row tiles, PAIR: one][hi, lo], PAIR: values on their way, two stages of keys and of values, of eight tiles each
+// key's row, factor and value factor, outputs on their way, the barriers
+__host__ __device__ constexpr int k8_smem(int hd, bool pair) {
+    return (pair ? 4 + K8_AHEAD : 6) * k8_codes(hd) + 2 * k8_values(hd) + 8 * 128 * 12 + 256 * 128 + 256;
+}
 
 template <int R> __device__ __forceinline__ void k8_more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(R)); }
 template <int R> __device__ __forceinline__ void k8_less_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(R)); }
@@ -151,11 +153,6 @@ __device__ __forceinline__ uint64_t k8_add2(uint64_t a, uint64_t b) {
 }
 __device__ __forceinline__ float k8_lo(uint64_t x) { return __uint_as_float((uint32_t)x); }
 __device__ __forceinline__ float k8_hi(uint64_t x) { return __uint_as_float((uint32_t)(x >> 32)); }
-__device__ __forceinline__ float k8_max3(float a, float b, float c) {
-    float r;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-    return r;
-}
 __device__ __forceinline__ uint32_t k8_mul_bf16x2(uint32_t a, uint32_t b) {
     uint32_t r;
     asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
