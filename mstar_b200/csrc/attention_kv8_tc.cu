@@ -22,7 +22,8 @@
 // for 2,048 tokens on 14,336 keys, when this took 565: products of 64 keys read the queries from shared memory twice as
 // often); the same with two threads a row, which take its steps in turn (571: the exponentials are the same); half a row a
 // thread (754: the halves have to meet at every tile); an eighth, a quarter or a third of the exponentials by a polynomial
-// (571, 632, 660 when this took 558: the issue slots are what the softmax lacks, not the special function unit).
+// (571, 632, 660 when this took 558); one power of two for all queries of a CTA, folded into the keys' factors, so that the
+// scores take one product less (565).  What the softmax lacks is neither: its steps wait for one another.
 // Tensor memory: S / P 2 x 128 columns, O 2 x head_dim.  Shared memory (head_dim 128): queries 64 KB, two stages of keys
 // of 16 KB and two of values of 32 KB each.
 //
