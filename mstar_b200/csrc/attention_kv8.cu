@@ -235,21 +235,27 @@ template <typename A, int R> static int launch_simt(const Kv8AttnArgs& a, dim3 g
 }
 
 // ---------------------------------------------------------------------------------------- on the tensor cores
-// m16n8k16 products of float16 with float sums.  e4m3 is exact in float16, so the codes of keys and values are converted
-// in registers, and only queries and weights are rounded: in the 32-bit mode (PARTS 2) each is two float16, x = hi + lo,
-// 22 bits, with a product each.  A row of queries is first scaled by a power of two to have its largest number in [2^13,
-// 2^14), so that the parts are not subnormal.  The rows' scales are put on the scores as in attention_kv8_decode.cu: the
-// values' weights are 2^(s_j + e_j - m'), in [0, 2^8], with a maximum of their own.
+// Scores: m16n8k16 products of float16 with float sums.  e4m3 is exact in float16, so the codes of keys are converted in
+// registers; a row of queries is scaled by a power of two to have its largest number in [2^13, 2^14) and is one float16
+// (exact for a bfloat16 but for numbers 2^-27 below the largest), in the 32-bit mode two, x = hi + lo: within 2^-22 of a number
+// or 2^-38 of the row's largest, a product each.  The keys' scales are factors of the scores.
+//
+// Outputs: products of bfloat16.  Values become bfloat16 with their row's scale, which is exact for every scale (kv8.cuh), and
+// weights 2^(s_j - m) are two bfloat16 parts in the 16-bit mode (16 bits), three in the 32-bit mode (all 24 bits of a float),
+// down to 2^-126 of the largest: a small weight, or a row of small values beside one of large values, keeps its bits.
+// (Weights in float16 relative to the largest 2^(s_j + e_j), with the values' exponents in them, took a product less, but what
+// lay 2^25 below the largest was lost in every feature.  Times so: 15.8, 327, 103, 18.4 us for the four calls below.)
 //
 // A warp owns 16 rows (token, query head of the group) and, of every tile of 64 keys, 8 NT: with NT 8 a block's four
 // warps have 64 rows, with NT 2 (16 rows or fewer) they share a tile's keys and leave a part each.  Tiles of codes come by
-// cp.async, one tile ahead (three with few rows), into swizzled shared memory; which features and keys the fragments'
-// elements are is chosen as in the decode kernel, and the queries lie in shared memory in that order.
+// cp.async, one tile ahead (three with few rows), into swizzled shared memory.  Which features and keys the elements of the
+// scores' operands are is chosen as in the decode kernel, and the queries lie in shared memory in that order.  The values of a
+// tile are converted once, each warp a quarter of the keys (with NT 2 its own), into a bfloat16 tile.
 //
-// Bound by instructions: about 1,000 of a warp for a tile of 64 keys of 64 features in the 32-bit mode, of which the
-// products fill the tensor pipe for 800 of some 1,600 clocks.  Two portions of 251 tokens, 32 heads of 64 over 8, a window
-// of 200 take 15.8 us (on CUDA cores 108), two of 512 on 6,000 cached 327 us (123 TFLOP/s, half of what the pipe does);
-// single tokens of 8 requests on 2,048 keys 18 us.
+// Bound by instructions and the tensor pipe.  In the 32-bit mode two portions of 251 tokens, 32 heads of 64 over 8, a window of
+// 200, take 16.0 us (on CUDA cores 108), two of 512 on 6,000 cached 350 (115 TFLOP/s; five products for two), in the 16-bit
+// mode 512 tokens of 12 heads of 256 over 4 on 2,000 cached 141; float single tokens of 8 requests on 800 to 2,048 keys, 24
+// heads of 128 over 8, 22 us.
 __device__ __forceinline__ uint32_t f16x2_of_codes(uint32_t two) {
     uint32_t r;
     asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t}" : "=r"(r) : "r"(two));
@@ -275,26 +281,32 @@ __device__ __forceinline__ uint32_t f16x2(float lo, float hi) {
     return *reinterpret_cast<const uint32_t*>(&v);
 }
 __device__ __forceinline__ float2 floats_of(uint32_t two) { return __half22float2(*reinterpret_cast<const __half2*>(&two)); }
+// Two neighbouring elements
+__device__ __forceinline__ void store2(float* p, float a, float b) { *reinterpret_cast<float2*>(p) = make_float2(a, b); }
+__device__ __forceinline__ void store2(bf16* p, float a, float b) { *reinterpret_cast<uint32_t*>(p) = pack_bf16(a, b); }
 
 #define KM_SLACK 8.f
 template <int HD> __host__ __device__ constexpr int km_tile() { return 64 * HD; }
 // tiles of which a block holds copies, on the way or there: with few rows a tile is soon worked off
 template <int NT> __host__ __device__ constexpr int km_stages() { return NT == 8 ? 2 : 4; }
 template <int HD, int PARTS, int NT> __host__ __device__ constexpr int km_smem() {
-    return km_stages<NT>() * (2 * km_tile<HD>() + 64 * 12) + PARTS * (NT == 8 ? 64 : 16) * (HD * 2 + 16) + 64 * 4;
+    return km_stages<NT>() * (2 * km_tile<HD>() + 64 * 12) + 2 * km_tile<HD>() + PARTS * (NT == 8 ? 64 : 16) * (HD * 2 + 16) + 64 * 4;
 }
 
 template <typename A, int HD, int PARTS, int NT>
 __global__ void __launch_bounds__(128) kv8_attention_mma_kernel(Kv8AttnArgs a) {
-    constexpr int ROWS = NT == 8 ? 64 : 16, RB = HD < 128 ? HD : 128, KC = HD / 64, VW = HD / 32, MT = HD / 8;
+    constexpr int ROWS = NT == 8 ? 64 : 16, RB = HD < 128 ? HD : 128, KC = HD / 64, MT = HD / 8;
+    constexpr int PP = PARTS + 1;                        // parts of a weight
     constexpr int NB = NT < 4 ? NT : 4;                  // products side by side
     constexpr int QP = HD * 2 + 16;                      // bytes of a row of queries in shared memory
     constexpr int S = km_stages<NT>();
     extern __shared__ __align__(128) unsigned char smem_m[];
     unsigned char* k_s = smem_m;                         // [S][64 keys x HD codes], then values
     unsigned char* v_s = k_s + S * km_tile<HD>();
-    unsigned char* q_s = v_s + S * km_tile<HD>();        // [PARTS][ROWS][QP]
-    float2* sc_s = reinterpret_cast<float2*>(q_s + PARTS * ROWS * QP);     // [S][64] 2^e of the key, e of the value
+    unsigned char* b_s = v_s + S * km_tile<HD>();        // [64 keys x HD bfloat16]: a tile's values
+    unsigned char* q_s = b_s + 2 * km_tile<HD>();        // [PARTS][ROWS][QP]
+    // [S][64] 2^e of the key, the value's factors as bits
+    float2* sc_s = reinterpret_cast<float2*>(q_s + PARTS * ROWS * QP);
     uint32_t* row_s = reinterpret_cast<uint32_t*>(sc_s + S * 64);         // [S][64]
     float* qscale_s = reinterpret_cast<float*>(row_s + S * 64);           // [ROWS]
     pdl_wait();
@@ -399,7 +411,8 @@ __global__ void __launch_bounds__(128) kv8_attention_mma_kernel(Kv8AttnArgs a) {
     auto keep_scales = [&](int i) {
         if (tid < 64 && i < tiles) {
             const bool bad = ks == KV8_BAD_BYTE || vs == KV8_BAD_BYTE;
-            sc_s[i % S * 64 + tid] = make_float2(bad ? __int_as_float(0x7fc00000) : kv8_scale(ks), (float)(vs - 127));
+            sc_s[i % S * 64 + tid] = make_float2(bad ? __int_as_float(0x7fc00000) : kv8_scale(ks),
+                                                     __uint_as_float(kv8_value_factors(bad ? 0 : vs - 127)));
         }
     };
     // where a 16-byte run c of row r lies in a block of a tile: the swizzle of 128- or 64-byte rows
@@ -449,10 +462,12 @@ __global__ void __launch_bounds__(128) kv8_attention_mma_kernel(Kv8AttnArgs a) {
         first[h] = first_of(min(row0 + wr + g + 8 * h, last_row));
     }
 
-    float o[MT][4], m[2] = {-INFINITY, -INFINITY}, w[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+    float o[MT][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < MT; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
     const int kg = (g & 1) ? g ^ 4 : g, kt = (2 * t + 1) ^ 4;      // a product's row or key i is key i, or i ^ 4 where i is odd
+    // the row (key of 16) and the 16-byte run of features that this lane names of the values' four matrices of 8 x 8
+    const int vr = (lane & 1 ? (lane & 7) ^ 4 : lane & 7) + (lane & 8), vc = lane >> 4;
     const uint32_t q_at = smem_u32(q_s) + (wr + (lane & 15)) * QP + (lane >> 4) * 16;
 
     for (int i = 0; i < tiles; ++i) {
@@ -466,6 +481,24 @@ __global__ void __launch_bounds__(128) kv8_attention_mma_kernel(Kv8AttnArgs a) {
         const unsigned char* vt_s = v_s + i % S * km_tile<HD>();
         const float2* sc = sc_s + i % S * 64;
         const int v0 = (tile0 + i) * 64;
+        // ---- values: a run of 16 codes a lane and turn, of the warp's 16 keys, becomes two runs of 16 bytes
+        {
+            constexpr int CPR = HD / 16, BR = HD * 2;
+#pragma unroll
+            for (int k = 0; k < CPR / 2; ++k) {
+                const int r = warp * 16 + (k * 32 + lane) / CPR, run = lane % CPR;
+                const uint4 x = *reinterpret_cast<const uint4*>(vt_s + (run >> 3) * (64 * RB) + at(r, run & 7));
+                uint32_t y[8];
+                kv8_values16(x, __float_as_uint(sc[r].y), y);
+                // (the runs of a row that lie 128 bytes apart take their two stores in the other order: different banks)
+                const int odd = (run >> 2) & 1;
+                unsigned char* to = b_s + r * BR;
+                *reinterpret_cast<uint4*>(to + (((2 * run + odd) ^ (r & 7)) << 4)) =
+                    odd ? make_uint4(y[4], y[5], y[6], y[7]) : make_uint4(y[0], y[1], y[2], y[3]);
+                *reinterpret_cast<uint4*>(to + (((2 * run + 1 - odd) ^ (r & 7)) << 4)) =
+                    odd ? make_uint4(y[0], y[1], y[2], y[3]) : make_uint4(y[4], y[5], y[6], y[7]);
+            }
+        }
         // ---- scores: s[n][2h + k], row g + 8h, keys 8 (n0 + n) + 2t and + kt
         float s[NT][4];
 #pragma unroll
@@ -494,16 +527,15 @@ __global__ void __launch_bounds__(128) kv8_attention_mma_kernel(Kv8AttnArgs a) {
                             mma_f16_16816(s[n + y], qf[p][k], f16x2_of_codes(b[y][k]), f16x2_of_codes_hi(b[y][k]));
             }
         }
-        // ---- weights.  s becomes the scores; the exponents of the values' weights are s + ev
-        float top[2] = {-INFINITY, -INFINITY}, vtop[2] = {-INFINITY, -INFINITY}, ev[NT][2];
+        // ---- weights
+        float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
-                const float2 f = sc[(n0 + n) * 8 + (k ? kt : 2 * t)];
-                ev[n][k] = f.y;
+                const float f = sc[(n0 + n) * 8 + (k ? kt : 2 * t)].x;
 #pragma unroll
-                for (int h = 0; h < 2; ++h) s[n][2 * h + k] *= f.x * qs[h];
+                for (int h = 0; h < 2; ++h) s[n][2 * h + k] *= f * qs[h];
             }
         if (v0 + 63 > last_of(row0) || (v0 < first_of(last_row) && v0 + 63 >= kept)) {
 #pragma unroll
@@ -519,26 +551,19 @@ __global__ void __launch_bounds__(128) kv8_attention_mma_kernel(Kv8AttnArgs a) {
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                top[j >> 1] = fmaxf(top[j >> 1], s[n][j]);
-                vtop[j >> 1] = fmaxf(vtop[j >> 1], s[n][j] + ev[n][j & 1]);
-            }
-        if (__any_sync(0xffffffffu, (top[0] > m[0] + KM_SLACK) | (top[1] > m[1] + KM_SLACK) | (vtop[0] > w[0] + KM_SLACK) |
-                                        (vtop[1] > w[1] + KM_SLACK))) {
+            for (int j = 0; j < 4; ++j) top[j >> 1] = fmaxf(top[j >> 1], s[n][j]);
+        // m: what scores are taken off from, at least the largest so far and 2^KM_SLACK above it where it was set, so that no
+        // weight is above 1 and the sums of values no larger than values are
+        if (__any_sync(0xffffffffu, (top[0] > m[0]) | (top[1] > m[1]))) {
             float up[2];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
 #pragma unroll
-                for (int d = 1; d < 4; d <<= 1) {
-                    top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], d));
-                    vtop[h] = fmaxf(vtop[h], __shfl_xor_sync(0xffffffffu, vtop[h], d));
-                }
-                top[h] = fmaxf(top[h], m[h]);
-                vtop[h] = fmaxf(vtop[h], w[h]);
-                if (m[h] != -INFINITY) l[h] *= exp2_approx(m[h] - top[h]);
-                up[h] = w[h] == -INFINITY ? 0.f : exp2_approx(w[h] - vtop[h]);
-                m[h] = top[h];
-                w[h] = vtop[h];
+                for (int d = 1; d < 4; d <<= 1) top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], d));
+                const float now = top[h] > m[h] ? top[h] + KM_SLACK : m[h];
+                up[h] = m[h] == -INFINITY ? 1.f : exp2_approx(m[h] - now);      // (l is 0 or NaN, o zeros or NaNs, where it is -inf)
+                l[h] *= up[h];
+                m[h] = now;
             }
 #pragma unroll
             for (int k = 0; k < MT; ++k) {
@@ -549,60 +574,45 @@ __global__ void __launch_bounds__(128) kv8_attention_mma_kernel(Kv8AttnArgs a) {
             }
         }
         const float mr[2] = {m[0] == -INFINITY ? 0.f : m[0], m[1] == -INFINITY ? 0.f : m[1]};
-        const float wr2[2] = {w[0] == -INFINITY ? 0.f : w[0], w[1] == -INFINITY ? 0.f : w[1]};
-        // ---- values, 16 keys at a time
+        // the values are there: of all warps, or of this one
+        if constexpr (NT == 8) __syncthreads();
+        else __syncwarp();
+        // ---- outputs, 16 keys at a time
 #pragma unroll
         for (int u = 0; u < NT / 2; ++u) {
-            uint32_t pf[PARTS][4];
+            uint32_t pf[PP][4];
 #pragma unroll
             for (int x = 0; x < 2; ++x)
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     const int n = 2 * u + x;
-                    l[h] += exp2_approx(s[n][2 * h] - mr[h]) + exp2_approx(s[n][2 * h + 1] - mr[h]);
-                    const float p0 = exp2_approx(s[n][2 * h] + ev[n][0] - wr2[h]), p1 = exp2_approx(s[n][2 * h + 1] + ev[n][1] - wr2[h]);
-                    const uint32_t hi = f16x2(p0, p1);
-                    pf[0][2 * x + h] = hi;
-                    if constexpr (PARTS == 2) {
-                        const float2 b = floats_of(hi);
-                        pf[PARTS - 1][2 * x + h] = f16x2(p0 - b.x, p1 - b.y);
+                    float p0 = exp2_approx(s[n][2 * h] - mr[h]), p1 = exp2_approx(s[n][2 * h + 1] - mr[h]);
+                    l[h] += p0 + p1;
+#pragma unroll
+                    for (int p = 0; p < PP; ++p) {       // what the parts before leave, rounded
+                        const uint32_t b = pack_bf16(p0, p1);
+                        pf[p][2 * x + h] = b;
+                        p0 -= __uint_as_float(b << 16);
+                        p1 -= __uint_as_float(b & 0xffff0000u);
                     }
                 }
-            uint32_t v[4][VW];
-            const int key0 = (n0 + 2 * u) * 8;
+            const int r = (n0 + 2 * u) * 8 + vr;
+            const uint32_t v_at = smem_u32(b_s) + r * (HD * 2);
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const int r = key0 + 8 * (k >> 1) + ((k & 1) ? kt : 2 * t);
-                if constexpr (HD == 64) {
-                    const uint2 x = *reinterpret_cast<const uint2*>(vt_s + at(r, g >> 1) + (g & 1) * 8);
-                    v[k][0] = x.x;
-                    v[k][1] = x.y;
-                } else {
+            for (int k = 0; k < MT; k += 2) {            // blocks k and k + 1 of 8 features
+                uint32_t v[4];
+                ldmatrix_x4_trans(v, v_at + (((k + vc) ^ (r & 7)) << 4));
 #pragma unroll
-                    for (int c = 0; c < VW / 4; ++c) {
-                        const int run = g * (VW / 4) + c;
-                        const uint4 x = *reinterpret_cast<const uint4*>(vt_s + (run >> 3) * (64 * RB) + at(r, run & 7));
-                        v[k][4 * c] = x.x; v[k][4 * c + 1] = x.y; v[k][4 * c + 2] = x.z; v[k][4 * c + 3] = x.w;
-                    }
+                for (int p = PP - 1; p >= 0; --p) {      // (the small parts first)
+                    mma_bf16_16816(o[k], pf[p], v[0], v[1]);
+                    mma_bf16_16816(o[k + 1], pf[p], v[2], v[3]);
                 }
-            }
-            // block 4 j + e of 8 features: feature 4 j + e of every lane group's run of HD / 8
-#pragma unroll
-            for (int j = 0; j < VW; ++j) {
-                const uint32_t a01 = __byte_perm(v[0][j], v[1][j], 0x5140), a23 = __byte_perm(v[0][j], v[1][j], 0x7362);
-                const uint32_t b01 = __byte_perm(v[2][j], v[3][j], 0x5140), b23 = __byte_perm(v[2][j], v[3][j], 0x7362);
-                const uint32_t lo[4] = {f16x2_of_codes(a01), f16x2_of_codes_hi(a01), f16x2_of_codes(a23), f16x2_of_codes_hi(a23)};
-                const uint32_t hi[4] = {f16x2_of_codes(b01), f16x2_of_codes_hi(b01), f16x2_of_codes(b23), f16x2_of_codes_hi(b23)};
-#pragma unroll
-                for (int p = 0; p < PARTS; ++p)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) mma_f16_16816(o[4 * j + e], pf[p], lo[e], hi[e]);
             }
         }
     }
     cp_async_wait<0>();
     pdl_launch_dependents();
-    // ---- the rows' sums, and the outputs: o[k][2h + e], row g + 8h, feature k of the runs of lane groups 2t + e
+    // ---- the rows' sums, and the outputs: o[k][2h + e], row g + 8h, feature 8 k + 2 t + e
     const int part = NT == 8 ? range : range * 4 + warp;
     const bool parts = NT == 2 || a.parts.splits > 1;
 #pragma unroll
@@ -612,23 +622,18 @@ __global__ void __launch_bounds__(128) kv8_attention_mma_kernel(Kv8AttnArgs a) {
         const int row = row0 + wr + g + 8 * h;
         if (row >= rows || (parts && !kv8_has_room(a.parts, first_token + row / G))) continue;
         const size_t head = (size_t)(first_token + row / G) * a.nq + kvh * G + row % G;
-        // 2^(m' - m): the two maxima differ by the values' exponents and the slack at most
-        const float back = w[h] == -INFINITY ? 0.f : exp2_approx(w[h] - m[h]);
-        const float f = parts ? back : l[h] == 0.f ? 0.f : back / l[h];
         const size_t at_part = (head - (size_t)kv8_first_token(a.parts) * a.nq) * a.parts.splits + part;
         if (parts && t == 0) {
             a.parts.ml[2 * at_part] = m[h];
             a.parts.ml[2 * at_part + 1] = l[h];
         }
+        const float f = parts ? 1.f : l[h] == 0.f ? 0.f : 1.f / l[h];
 #pragma unroll
-        for (int e = 0; e < 2; ++e)
-#pragma unroll
-            for (int k = 0; k < MT; k += 4) {
-                const float x[4] = {o[k][2 * h + e] * f, o[k + 1][2 * h + e] * f, o[k + 2][2 * h + e] * f, o[k + 3][2 * h + e] * f};
-                const int d = (2 * t + e) * (HD / 8) + k;
-                if (parts) store4(a.parts.o + at_part * HD + d, x);
-                else store4((A*)a.out + head * HD + d, x);
-            }
+        for (int k = 0; k < MT; ++k) {
+            const int d = 8 * k + 2 * t;
+            if (parts) store2(a.parts.o + at_part * HD + d, o[k][2 * h], o[k][2 * h + 1]);
+            else store2((A*)a.out + head * HD + d, o[k][2 * h] * f, o[k][2 * h + 1] * f);
+        }
     }
 }
 

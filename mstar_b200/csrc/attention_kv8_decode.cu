@@ -22,12 +22,18 @@
 // to 4 query heads a kv head there is none: hi and lo are columns 0 - 3 and 4 - 7 of one product, and the threads that
 // would have idle columns take half of the keys of the softmax.
 //
-// Of the values' product the weights are float16, in which e4m3 is exact, so the codes are converted.  The rows' scales
-// are put on the scores: a key's by a product, and a value's as an addend of the exponent, since 2^s_j * 2^e_j v_j =
-// 2^(s_j + e_j) v_j.  The weights are therefore 2^(s_j + e_j - m') with a maximum m' of their own, so that they use
-// float16's range whatever the values' scales are; the normaliser's are 2^(s_j - m).  Both maxima follow the scores only
-// when these exceed them by more than 2^8, which a vote of the warp finds: exchanging the maxima at every tile costs as
-// much as its exponentials.
+// The rows' scales are put on the scores: a key's by a product, and a value's as an addend of the exponent, since 2^s_j *
+// 2^e_j v_j = 2^(s_j + e_j) v_j.  The values' weights are therefore 2^(s_j + e_j - m') with a maximum m' of their own, the
+// normaliser's 2^(s_j - m).  Both maxima follow the scores only when these exceed them by more than 2^8, which a vote of
+// the warp finds: exchanging the maxima at every tile costs as much as its exponentials.
+//
+// The values' product is one of bfloat16, codes as they are and weights in two parts (16 bits, down to 2^-126 of the
+// largest), so that a key of a small weight, or of small values beside one of large values, counts in the features where
+// the large ones have zeros.  With up to 4 query heads a kv head the low parts are columns 4 - 7 of the same product, otherwise
+// they take one of their own.  A code becomes a bfloat16 by moving its sign, exponent and mantissa, three to four
+// instructions for two of them.  (Float16 weights, and codes by a conversion each, took 15.1 us for one token on 16,384
+// keys instead of 16.8 and 41.7 for 64 on 800 to 2,048 instead of 48, but float16 ends at 2^-24, so that what lies further
+// below the largest was lost in every feature.  Float16 only for tiles whose weights all allow it, found by a vote: 17.3 and 47.)
 //
 // The tiles of a (token, kv head) are dealt out in turn to the warps of a cluster of blocks, so that the lengths that
 // are there decide the balance, not the bounds a launch was sized for.  The warps of a block are joined in shared
@@ -36,13 +42,12 @@
 // memory, sums in a fixed order.
 //
 // A warp's ring is two tiles, so that twelve warps of head_dim 128 fit an SM instead of eight (sixteen of 64): its
-// instructions, issued in order and each waiting for the last, bound it, not the copies.  64 requests on 2,048 keys,
-// 8 kv heads of 128: 42 us (47 with three tiles; 30 at the copy bandwidth), one on 16,384: 15.2, 64 on windows of 1,024
-// keys of 64: 17.5.
+// instructions, issued in order and each waiting for the last, bound it, not the copies.  64 requests, 8 kv heads of 128:
+// 51.1 us on 2,048 keys each (41.5 at the copy bandwidth), 48.2 on 800 to 2,048 (29.5); one on 16,384: 16.8 (5.2); 64 on
+// windows of 1,024 keys of 64: 20.2 (10.6).
 //
 // Semantics are those of attention_generic.cu.
 #include <cooperative_groups.h>
-#include <cuda_fp16.h>
 
 #include "kv8.cuh"
 #include "mma_util.cuh"
@@ -59,20 +64,14 @@ struct Kv8DecodeArgs {
     PageSplit page;
 };
 
-__device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t two) {
-    uint32_t r;
-    asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t}" : "=r"(r) : "r"(two));
-    return r;
-}
-__device__ __forceinline__ uint32_t e4m3x2_hi_to_f16x2(uint32_t two) {
-    uint32_t r;
-    asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, hi;\n\t}" : "=r"(r) : "r"(two));
-    return r;
-}
-__device__ __forceinline__ void mma_f16_16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
-                                              uint32_t b0, uint32_t b1) {
+// Of a word of four codes, two of each of two keys, the second or the first of both as bfloat16 times 2^-120: sign, exponent
+// and mantissa in bfloat16's places (subnormal codes become subnormal numbers).
+__device__ __forceinline__ uint32_t codes_second(uint32_t x) { return (x & 0x80008000u) | ((x >> 4) & 0x07f007f0u); }
+__device__ __forceinline__ uint32_t codes_first(uint32_t x) { return ((x << 8) & 0x80008000u) | ((x << 4) & 0x07f007f0u); }
+__device__ __forceinline__ void mma_bf16_values(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                                uint32_t b0, uint32_t b1) {
     asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
@@ -93,10 +92,6 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
-    const __half2 v = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&v);
-}
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
 // 2^(a - b) for maxima that may still be -inf (of a part without keys: 0)
@@ -105,6 +100,7 @@ __device__ __forceinline__ float ratio(float a, float b) { return a == -INFINITY
 #define DEC8_KEYS 32     // keys of a tile
 #define DEC8_STAGES 2    // tiles of a warp's ring
 #define DEC8_SLACK 8.f   // how far (in powers of two) scores may exceed the maxima
+#define DEC8_RAISE 112.f // weights are at most 2^(112 + 8)
 // Shared memory of a warp: tiles of keys and of values (blocks of [32 rows x at most 128 bytes], swizzled), then a scale
 // pair a key, then each tile's scale bytes; the outputs that the warps leave at the end lie over the tiles.
 template <int D> __host__ __device__ constexpr int dec8_tile() { return DEC8_KEYS * D; }
@@ -378,28 +374,28 @@ kv8_decode_kernel(Kv8DecodeArgs a) {
             w1 = y1;
         }
         const float z0 = m0 == -INFINITY ? 0.f : m0, z1 = m1 == -INFINITY ? 0.f : m1;
-        const float q0 = w0 == -INFINITY ? 0.f : w0, q1 = w1 == -INFINITY ? 0.f : w1;
-        uint32_t pf[2][2];
+        // (the weights' exponents are raised so that the products with codes times 2^-120 are as large as they would be without)
+        const float q0 = (w0 == -INFINITY ? 0.f : w0) - DEC8_RAISE, q1 = (w1 == -INFINITY ? 0.f : w1) - DEC8_RAISE;
+        uint32_t pf[2][2], pl[2][2];          // the weights' bfloat16 parts
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
             for (int k = 0; k < E; ++k) {
                 l0 += ex2(s[u][2 * k] - z0);
                 l1 += ex2(s[u][2 * k + 1] - z1);
-                pf[u][k] = pack_f16(ex2(p[u][2 * k] - q0), ex2(p[u][2 * k + 1] - q1));
+                const float p0 = ex2(p[u][2 * k] - q0), p1 = ex2(p[u][2 * k + 1] - q1);
+                const uint32_t hi = pack_bf16(p0, p1);
+                pf[u][k] = transpose_8x8(hi);
+                pl[u][k] = transpose_8x8(pack_bf16(p0 - __uint_as_float(hi << 16), p1 - __uint_as_float(hi & 0xffff0000u)));
             }
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-            for (int k = 0; k < E; ++k) pf[u][k] = transpose_8x8(pf[u][k]);
         if constexpr (H == 4) {
-            // row g < 4 of the transpose is head g with the first eight keys, row g + 4 the same head with the others
-#pragma unroll
-            for (int u = 0; u < 2; ++u) pf[u][1] = __shfl_xor_sync(0xffffffffu, pf[u][0], 16);
+            // row g < 4 of a transpose is head g with the first eight keys, row g + 4 the same head with the others: columns
+            // 0 - 3 of the product take the high parts of both, columns 4 - 7 the low ones
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
-                pf[u][0] = g < 4 ? pf[u][0] : 0u;
-                pf[u][1] = g < 4 ? pf[u][1] : 0u;
+                const uint32_t got = __shfl_xor_sync(0xffffffffu, g < 4 ? pl[u][0] : pf[u][0], 16);
+                pf[u][1] = g < 4 ? got : pl[u][0];
+                pf[u][0] = g < 4 ? pf[u][0] : got;
             }
         }
         // ---- values
@@ -430,13 +426,17 @@ kv8_decode_kernel(Kv8DecodeArgs a) {
             }
 #pragma unroll
             for (int j = 0; j < VW; ++j) {
-                // features 4j, 4j + 1 and 4j + 2, 4j + 3 of this thread's run, two keys side by side
-                const uint32_t a01 = __byte_perm(v[0][j], v[1][j], 0x5140), a23 = __byte_perm(v[0][j], v[1][j], 0x7362);
-                const uint32_t b01 = __byte_perm(v[2][j], v[3][j], 0x5140), b23 = __byte_perm(v[2][j], v[3][j], 0x7362);
-                mma_f16_16816(o[2 * j], e4m3x2_to_f16x2(a01), e4m3x2_hi_to_f16x2(a01), e4m3x2_to_f16x2(b01),
-                              e4m3x2_hi_to_f16x2(b01), pf[u][0], pf[u][1]);
-                mma_f16_16816(o[2 * j + 1], e4m3x2_to_f16x2(a23), e4m3x2_hi_to_f16x2(a23), e4m3x2_to_f16x2(b23),
-                              e4m3x2_hi_to_f16x2(b23), pf[u][0], pf[u][1]);
+                // features 4j, 4j + 1 and 4j + 2, 4j + 3 of this thread's run, of one key and of the other
+                const uint32_t a01 = __byte_perm(v[0][j], v[1][j], 0x5410), a23 = __byte_perm(v[0][j], v[1][j], 0x7632);
+                const uint32_t b01 = __byte_perm(v[2][j], v[3][j], 0x5410), b23 = __byte_perm(v[2][j], v[3][j], 0x7632);
+                const uint32_t a0 = codes_first(a01), a1 = codes_second(a01), a2 = codes_first(b01), a3 = codes_second(b01);
+                const uint32_t a4 = codes_first(a23), a5 = codes_second(a23), a6 = codes_first(b23), a7 = codes_second(b23);
+                if constexpr (H == 8) {
+                    mma_bf16_values(o[2 * j], a0, a1, a2, a3, pl[u][0], pl[u][1]);
+                    mma_bf16_values(o[2 * j + 1], a4, a5, a6, a7, pl[u][0], pl[u][1]);
+                }
+                mma_bf16_values(o[2 * j], a0, a1, a2, a3, pf[u][0], pf[u][1]);
+                mma_bf16_values(o[2 * j + 1], a4, a5, a6, a7, pf[u][0], pf[u][1]);
             }
         }
         // ---- the tile S turns ahead takes this one's place
@@ -451,6 +451,12 @@ kv8_decode_kernel(Kv8DecodeArgs a) {
     __syncthreads();
 
     // ---- the warps of the block: statistics (m, m', l) and outputs of H heads each
+    if constexpr (H == 4) {                  // the sums of the high and of the low parts
+#pragma unroll
+        for (int k = 0; k < MT; ++k)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[k][i] += __shfl_xor_sync(0xffffffffu, o[k][i], 2);
+    }
     constexpr int LD = D + 4;
 #pragma unroll
     for (int d = H == 4 ? 2 : 4; d < 32; d <<= 1) {
@@ -505,9 +511,10 @@ kv8_decode_kernel(Kv8DecodeArgs a) {
         return v;
     };
     auto finish = [&](const float4& all, const float4& v, int h, int d) {
-        // 2^(m' - m) / l: the two maxima differ by the values' exponents and the slack at most
+        // 2^(m' - m) / l: the two maxima differ by the values' exponents and the slack at most.  (Sums are 2^(DEC8_RAISE - 120)
+        // times what they stand for; that factor by itself, since 2^(m' - m) may be as large as 2^127.)
         const float f = all.z == 0.f ? 0.f : ex2(all.y == -INFINITY ? 0.f : all.y - all.x) / all.z;
-        const float out[4] = {v.x * f, v.y * f, v.z * f, v.w * f};
+        const float out[4] = {v.x * f * 256.f, v.y * f * 256.f, v.z * f * 256.f, v.w * f * 256.f};
         store4(a.out + (size_t)token * a.nq * D + (size_t)(kvh * G + h0 + h) * D + d, out);
     };
     // four features a thread; block c joins the features [c D / C, (c + 1) D / C) of every head

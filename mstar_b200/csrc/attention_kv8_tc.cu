@@ -154,18 +154,8 @@ __device__ __forceinline__ uint64_t k8_add2(uint64_t a, uint64_t b) {
 }
 __device__ __forceinline__ float k8_lo(uint64_t x) { return __uint_as_float((uint32_t)x); }
 __device__ __forceinline__ float k8_hi(uint64_t x) { return __uint_as_float((uint32_t)(x >> 32)); }
-__device__ __forceinline__ uint32_t k8_mul_bf16x2(uint32_t a, uint32_t b) {
-    uint32_t r;
-    asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-    return r;
-}
 // bits 0 .. n - 1
 __device__ __forceinline__ uint32_t k8_below(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }
-// The factors that make a code's bits in bfloat16's places its value for the row's exponent e: 2^min(120 + e, 127) in
-// the low half, 2^max(e - 7, 0) in the high one.
-__device__ __forceinline__ uint32_t k8_value_factors(int e) {
-    return ((uint32_t)(min(120 + e, 127) + 127) << 7) | ((uint32_t)(max(e - 7, 0) + 127) << 23);
-}
 
 template <int HD, bool PAIR>
 __global__ void __launch_bounds__(K8_THREADS, 1) kv8_attention_tc_kernel(Kv8TcArgs a) {
@@ -250,7 +240,7 @@ __global__ void __launch_bounds__(K8_THREADS, 1) kv8_attention_tc_kernel(Kv8TcAr
                 const bool bad = kb == KV8_BAD_BYTE || vb == KV8_BAD_BYTE;
                 row_s[at] = row;
                 kf_s[at] = bad ? __int_as_float(0x7fc00000) : kv8_scale(kb);
-                vf_s[at] = k8_value_factors(bad ? 0 : vb - 127);
+                vf_s[at] = kv8_value_factors(bad ? 0 : vb - 127);
             };
             const bool two = kt < 32;
             // table entries are read two tiles ahead of their rows' use, scales one (a warp issues in order, and would
@@ -461,13 +451,13 @@ __global__ void __launch_bounds__(K8_THREADS, 1) kv8_attention_tc_kernel(Kv8TcAr
                 uint32_t out[8];
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {       // codes 0 and 2 of a word, then 1 and 3
-                    out[2 * k] = k8_mul_bf16x2(((in[k] << 8) & 0x80008000u) | ((in[k] << 4) & 0x07f007f0u), f1);
-                    out[2 * k + 1] = k8_mul_bf16x2((in[k] & 0x80008000u) | ((in[k] >> 4) & 0x07f007f0u), f1);
+                    out[2 * k] = kv8_mul_bf16x2(((in[k] << 8) & 0x80008000u) | ((in[k] << 4) & 0x07f007f0u), f1);
+                    out[2 * k + 1] = kv8_mul_bf16x2((in[k] & 0x80008000u) | ((in[k] >> 4) & 0x07f007f0u), f1);
                 }
                 if ((f >> 16) != 0x3f80u) {         // values above 2^15
                     const uint32_t f2 = __byte_perm(f, f, 0x3232);
 #pragma unroll
-                    for (int k = 0; k < 8; ++k) out[k] = k8_mul_bf16x2(out[k], f2);
+                    for (int k = 0; k < 8; ++k) out[k] = kv8_mul_bf16x2(out[k], f2);
                 }
                 unsigned char* base = v_s + (j & 1) * VT + (c >> 3) * (128 * 128) + r * 128;
                 *reinterpret_cast<uint4*>(base + (((c & 7) ^ (r & 7)) << 4)) = make_uint4(out[0], out[1], out[2], out[3]);

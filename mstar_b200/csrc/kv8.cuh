@@ -56,6 +56,33 @@ __device__ __forceinline__ void kv8_unpack4(uint32_t w, float* v) {
     v[3] = b.y;
 }
 
+// Values as bfloat16 with their row's scale, which is exact for every scale: sign, exponent and mantissa of a code are moved to
+// bfloat16's places, which reads as the code times 2^-120, subnormal codes included, and a product by 2^(120 + e) puts it
+// right: by 2^min(120 + e, 127), in the low half of the factors, and by 2^max(e - 7, 0), in the high one.
+__device__ __forceinline__ uint32_t kv8_value_factors(int e) {
+    return ((uint32_t)(min(120 + e, 127) + 127) << 7) | ((uint32_t)(max(e - 7, 0) + 127) << 23);
+}
+__device__ __forceinline__ uint32_t kv8_mul_bf16x2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+// 16 codes of a row in their order
+__device__ __forceinline__ void kv8_values16(const uint4& x, uint32_t f, uint32_t (&y)[8]) {
+    const uint32_t in[4] = {x.x, x.y, x.z, x.w}, f1 = __byte_perm(f, f, 0x1010);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const uint32_t lo = __byte_perm(in[k], 0u, 0x1404), hi = __byte_perm(in[k], 0u, 0x3424);      // a code above a zero byte
+        y[2 * k] = kv8_mul_bf16x2((lo & 0x80008000u) | ((lo >> 4) & 0x07f007f0u), f1);
+        y[2 * k + 1] = kv8_mul_bf16x2((hi & 0x80008000u) | ((hi >> 4) & 0x07f007f0u), f1);
+    }
+    if ((f >> 16) != 0x3f80u) {                           // a scale above 2^7
+        const uint32_t f2 = __byte_perm(f, f, 0x3232);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) y[k] = kv8_mul_bf16x2(y[k], f2);
+    }
+}
+
 // Division of a number in [0, 2^31) by a fixed page size d: with s = ceil(log2 d) and m = ceil(2^(31 + s) / d) < 2^32 + 1,
 // m d - 2^(31 + s) < d <= 2^s, so that n m / 2^(31 + s) exceeds n / d by less than 2^-31 n / d < 1 / d and has its floor.
 struct PageSplit {

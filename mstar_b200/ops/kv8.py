@@ -209,10 +209,11 @@ def kv8_splits(blocks: int, max_keys: int, sms: int) -> int:
 
 def kv8_mma_splits(blocks: int, max_keys: int, sms: int, few: bool) -> int:
     """The same for the kernel of the 32-bit mode.  64 rows: two blocks an SM, parts of at least 256 keys.
-    (256 blocks on 220 keys, 152 on 1,000, 512 on 6,500 took 15.7, 59.3, 326 us uncut and 19.4, 55.9, 314 in two
+    (256 blocks on 220 keys, 152 on 1,000, 512 on 6,500, heads of 64: 16.4, 42.0, 350 us uncut, 20.6, 39.7, 335 in two
     parts.)  16 rows or fewer: a block's four warps leave a part each; three blocks on two SMs, 64 keys a warp
-    at least.  (8 pairs of a token and a kv head on 16,384 keys, 64 on 2,048 and 512 on 1,028 took 32, 18 and
-    40 us so, 42, 26 and 36 with a quarter, half and twice as many.)"""
+    at least.  (8 pairs of a token and a kv head on 16,384 keys, 64 on 2,048 and 512 on 1,028, heads of 128: 39, 24 and
+    76 us so, 41, 37 and 76 with half as many parts, 51, 28 and 81 with twice as many; heads of 64: 30, 21, 37 so, 29, 23,
+    37 and 39, 16, 40.)"""
     if few:
         return 4 * max(1, min(64, -(-3 * sms // (2 * max(blocks, 1))), -(-max_keys // 256)))
     return max(1, min(64, -(-2 * sms // max(blocks, 1)), -(-max_keys // 256)))
@@ -260,10 +261,11 @@ def kv8_decode_shape(pairs: int, max_keys: int, head_dim: int, few: bool, sms: i
     query heads; ``few``: 4) in the decode kernel.  All blocks run at once (larger clusters leave SMs
     free), with the smallest share of a pair's keys on the SM that has most; among those clusters of two
     at most where that does, and then as many warps as fit.  Where no shape runs at once: single blocks of
-    four.  (Heads of 128, 3 a kv head, 2,048 keys, measured with 16 shapes each: 8, 24, 64, 128, 256, 400, 512
-    pairs take 5.7 with 8 x 8, 6.9 with 4 x 8, 9.6 with 2 x 8, 15.7 with 2 x 6, 23.5 with 1 x 6, 32.8 with 1 x 4,
-    42.2 with 1 x 3, which is the best or within 0.4 us of it; 1 x 4 takes 18.3, 22.3, 26.5, 32.8 and 47.1 for
-    the last five.)"""
+    four.  (2,048 keys, 24 shapes each.  Heads of 128, 3 a kv head: 8, 24, 64, 128, 256, 400, 512 pairs take 5.9 us
+    with 8 x 8, 7.3 with 4 x 8, 11.5 with 2 x 8, 19.1 with 2 x 6, 28.8 with 1 x 6, 40.2 with 1 x 4, 51.1 with 1 x 3;
+    the best of all shapes is within 0.1 but for 17.9 (1 x 8) at 128.  8 a kv head, heads of 64: within 0.2, but for
+    62.4 (1 x 2) against 64.8 at 512 pairs and 7.6 (4 x 4) against 8.1 at 64 of 64.  Heads of 256: within 0.1 while all
+    blocks run at once; 256, 400, 512 pairs take 70.5, 104.8, 137.3 with 1 x 4 where 1 x 3 or 1 x 2 take 61.3, 90.5, 117.1.)"""
     heads = 4 if few else 8
     # a warp's two tiles of 32 keys and values with their scales; warps that the registers allow an SM
     ring, most = 2 * 64 * (head_dim + 1) + 256, 16 if head_dim == 64 else 12 if few and head_dim == 128 else 8
