@@ -56,9 +56,18 @@ def _prompts(args) -> list:
 
 
 def _deployed_kv_dtype(kv: dict):
-    """The ``dtype`` of a deployment's ``kv_cache`` section; a compute type's name says what is so anyway."""
+    """The ``dtype`` of a deployment's ``kv_cache`` section where it names a type of this engine's caches.  Anything else
+    leaves the cache in the compute type, as such files ran before the key was read; a name that is not a compute type's
+    is reported."""
+    from mstar_b200.cache.storage import KV_CACHE_DTYPES
+
     dtype = kv.get("dtype")
-    return None if dtype in ("bfloat16", "float16", "float32") else dtype
+    if dtype in KV_CACHE_DTYPES:
+        return dtype
+    if dtype is not None and dtype not in ("bfloat16", "bf16", "float32", "fp32", "f32", "float16", "fp16", "half"):
+        logging.getLogger(__name__).warning("kv_cache dtype %r is not one of %s: keys and values are kept in the compute type",
+                                            dtype, ", ".join(KV_CACHE_DTYPES))
+    return None
 
 
 def _generate(args) -> None:
