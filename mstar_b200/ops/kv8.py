@@ -24,13 +24,6 @@ import torch
 from . import _DT, _error_ptr, _need_cuda, _stream, lib, num_sms
 from .lib import KernelError, check
 
-try:
-    # (size, stride, dtype) on the current device: 0.7 us a call, where Tensor.new_empty takes 1.8
-    from torch._C._dynamo.guards import _empty_strided_cuda as _empty
-except ImportError:
-    def _empty(size, stride, dtype):
-        return torch.empty_strided(size, stride, dtype=dtype, device=torch.device("cuda", _device()))
-
 KV8_DTYPE = torch.float8_e4m3fn
 _INT = torch.int32
 _F32, _BF16, _BYTE = torch.float32, torch.bfloat16, torch.uint8
@@ -139,7 +132,7 @@ def rope_kv8_write(qkv: torch.Tensor, positions, cache_pos, token_req, block_tab
             device == positions.get_device() == cache_pos.get_device() == token_req.get_device()
             == block_table.get_device() == kv_cache.get_device() == kv_scales.get_device() == _device()):
         _refuse_device(what, qkv, positions, cache_pos, token_req, block_table, kv_cache, kv_scales)
-    q = _empty((n, num_heads * head_dim), (num_heads * head_dim, 1), qkv.dtype)
+    q = qkv.new_empty(n, num_heads * head_dim)          # (sizes as numbers: 1.4 us, 1.8 as a tuple)
     if n == 0:
         return q
     check(lib.get("kv8_cache").mstar_rope_kv8_write_packed(_pack_write(
@@ -170,8 +163,7 @@ def kv8_read_rows(kv_cache: torch.Tensor, kv_scales: torch.Tensor, block_table, 
             device == kv_scales.get_device() == block_table.get_device() == token_req.get_device()
             == cache_pos.get_device() == _device()):
         _refuse_device(what, kv_cache, kv_scales, block_table, token_req, cache_pos)
-    row = heads * head_dim
-    out = _empty((n, 2, heads, head_dim), (2 * row, row, head_dim, 1), dtype)
+    out = kv_scales.new_empty(n, 2, heads, head_dim, dtype=dtype)
     if n:
         check(lib.get("kv8_cache").mstar_kv8_read_rows_packed(_pack_read(
             kv_cache.data_ptr(), kv_scales.data_ptr(), block_table.data_ptr(), *table, token_req.data_ptr(),
@@ -224,7 +216,7 @@ def _parts(q, tokens, num_heads, head_dim, splits) -> tuple:
     if splits == 1:
         return None, 0, 0
     rows = tokens * num_heads * splits
-    t = _empty((rows * (head_dim + 2),), (1,), _F32)
+    t = q.new_empty(rows * (head_dim + 2), dtype=_F32)
     return t, t.data_ptr(), t.data_ptr() + 4 * rows * head_dim
 
 

@@ -1,0 +1,40 @@
+"""Calls of the 8-bit cache's operators that the larger tests do not make."""
+import pytest
+import torch
+from torch.utils._python_dispatch import TorchDispatchMode
+
+from kv8_util import Case
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda:0"
+F32, BF16 = torch.float32, torch.bfloat16
+
+
+def i32(v):
+    return torch.as_tensor(v, dtype=torch.int32, device=DEV)
+
+
+@pytest.mark.parametrize("act", [F32, BF16])
+def test_modes_see_what_the_operators_allocate(act):
+    """Outputs and the memory for parts come by torch's dispatcher, so that a mode around the calls sees them."""
+    from mstar_b200 import ops
+
+    class Sizes(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            out = func(*args, **(kwargs or {}))
+            if isinstance(out, torch.Tensor):
+                seen.append((tuple(out.shape), out.dtype))
+            return out
+
+    seen: list = []
+    c = Case([3], [1500], 4, 2, 128, 16, act, seed=1)
+    codes, scales = c.cache()
+    qkv, pos, req, table = torch.randn(3, 8 * 128, device=DEV).to(act), i32([0, 1, 2]), i32([0] * 3), c.table.to(DEV)
+    with Sizes():
+        ops.rope_kv8_write(qkv, pos, pos, req, table, None, codes, scales, 4, 2, 128, 0, False, 16)
+        assert seen.pop() == ((3, 4 * 128), act)
+        ops.kv8_read_rows(codes, scales, table, req, pos, act)
+        assert seen.pop() == ((3, 2, 2, 128), act)
+        c.prefill()
+    assert any(dtype == F32 and len(shape) == 1 and shape[0] >= 3 * 4 * 130 * 2 for shape, dtype in seen)
