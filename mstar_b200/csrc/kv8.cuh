@@ -110,7 +110,7 @@ struct SeenKeys {
 };
 __device__ __forceinline__ SeenKeys seen_keys(int first, int last, int window, int keep_first) {
     SeenKeys s;
-    s.lo = window > 0 ? max(0, first - window + 1) : 0;
+    s.lo = window > 0 && first >= window ? first - window + 1 : 0;      // (`first` may be negative, the window 2^31 - 1)
     s.kept = min(keep_first, s.lo);
     s.count = max(0, last + 1 - s.lo + s.kept);
     return s;

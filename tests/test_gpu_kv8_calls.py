@@ -38,3 +38,21 @@ def test_modes_see_what_the_operators_allocate(act):
         assert seen.pop() == ((3, 2, 2, 128), act)
         c.prefill()
     assert any(dtype == F32 and len(shape) == 1 and shape[0] >= 3 * 4 * 130 * 2 for shape, dtype in seen)
+
+
+@pytest.mark.parametrize("act", [F32, BF16])
+@pytest.mark.parametrize("hd", [48, 64, 128, 256])
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31 - 4, 2 ** 30])
+def test_the_largest_windows_hide_nothing(act, hd, window):
+    """More new tokens than keys (the first stand below place 0) under a window that no place passes: as without one."""
+    for lens_q, lens_kv in (([9, 70], [3, 40]), ([40], [38])):
+        c = Case([1] * len(lens_q), lens_kv, 4, 2, hd, 16, act, seed=2)
+        tokens = sum(lens_q)
+        c.q = torch.randn(tokens, 4 * hd, generator=torch.Generator().manual_seed(3)).to(act)
+        c.lens_q, c.req, c.indptr = lens_q, [0] * tokens, [0] + [sum(lens_q[:r + 1]) for r in range(len(lens_q))]
+        want = c.prefill()
+        assert (want[:lens_q[0] - lens_kv[0]] == 0).all() and (want[lens_q[0] - 1] != 0).all()
+        c.window, c.keep = window, 0
+        assert torch.equal(c.prefill(), want)
+        c.keep = 5
+        assert torch.equal(c.prefill(), want)
