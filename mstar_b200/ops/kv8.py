@@ -28,6 +28,7 @@ KV8_DTYPE = torch.float8_e4m3fn
 _INT = torch.int32
 _F32, _BF16, _BYTE = torch.float32, torch.bfloat16, torch.uint8
 _device = torch._C._cuda_getDevice
+_FAR = 2 ** 31 - 1          # distances of rows are 32-bit numbers in the kernels
 # the entry points' arguments as one string (csrc/kv8.cuh)
 _pack_write = Struct("=22q").pack
 _pack_read = Struct("=15q").pack
@@ -77,7 +78,9 @@ def _check_table(what, block_table, read=False) -> tuple:
     strides = block_table.stride()
     if block_table.dtype is not _INT or len(strides) != 2 or strides[1] != 1 or strides[0] < 1:
         _refuse(what, "the block table is int32 [entries, pages], its rows without gaps")
-    width = block_table.shape[1]
+    entries, width = block_table.shape
+    if strides[0] > _FAR and entries > 1:
+        _refuse(what, "the block table's rows lie 2^31 entries apart or more")
     if read and width < 1:
         _refuse(what, "the block table has no pages")
     return strides[0], width
@@ -110,6 +113,8 @@ def rope_kv8_write(qkv: torch.Tensor, positions, cache_pos, token_req, block_tab
     if len(shape) != 2 or shape[1] != (num_heads + 2 * num_kv_heads) * head_dim or strides[1] != 1:
         _refuse(what, f"qkv {tuple(shape)} is not [tokens, ({num_heads} + 2 * {num_kv_heads}) * {head_dim}] "
                       "with rows without gaps")
+    if strides[0] > _FAR and shape[0] > 1:
+        _refuse(what, "qkv's rows lie 2^31 numbers apart or more")
     if num_heads < 1 or num_kv_heads < 1:
         _refuse(what, "there is at least one query head and one kv head")
     if rotary_dim % 2 or not 0 <= rotary_dim <= head_dim:
@@ -181,6 +186,8 @@ def _check_attention(what, q, out, rows, num_heads, num_kv_heads, head_dim, wind
     shape, strides = q.shape, q.stride()
     if len(shape) != 2 or shape[0] < rows or shape[1] < width or strides[1] != 1:
         _refuse(what, f"q {tuple(shape)} is not [at least {rows}, at least {width}] with rows without gaps")
+    if strides[0] > _FAR and shape[0] > 1:
+        _refuse(what, "q's rows lie 2^31 numbers apart or more")
     shape = out.shape
     if out.dtype is not q.dtype or len(shape) != 2 or shape[0] < rows or shape[1] != width or not out.is_contiguous():
         _refuse(what, f"out is contiguous {q.dtype} [at least {rows}, {width}], got {out.dtype} {tuple(shape)}")
@@ -281,6 +288,12 @@ def kv8_decode_shape(pairs: int, max_keys: int, head_dim: int, few: bool, sms: i
 KV8_TC_HEAD_DIMS = (64, 128)
 
 
+def kv8_tc_reaches(rows: int, q_stride: int) -> bool:
+    """Whether the tensor-core kernel, which holds a query's place in units of 8 numbers in 32 bits (the last is taken),
+    can name all rows."""
+    return rows * q_stride < 2 ** 35 - 8
+
+
 def kv8_tc_splits(blocks: int, max_keys: int, sms: int, one_tile: bool) -> tuple:
     """(parts that the keys of ``blocks`` blocks of row tiles are cut into in the tensor-core kernel, whether a
     block makes two of them): a block an SM, at least two tiles of 128 keys each, at most 64 parts.  With
@@ -368,7 +381,7 @@ def paged_prefill_attention_kv8(q: torch.Tensor, out: torch.Tensor, kv_cache: to
     most = _most_keys(max_kv_len, max_q_len, window, keep_first)
     q_ptr, out_ptr, codes = q.data_ptr(), out.data_ptr(), kv_cache.data_ptr()
     if (q.dtype is _BF16 and head_dim in KV8_TC_HEAD_DIMS and group <= 128 and q_stride % 8 == 0
-            and (q_ptr | codes) % 16 == 0):
+            and (q_ptr | codes) % 16 == 0 and kv8_tc_reaches(q.shape[0], q_stride)):
         per_tile = 128 // group
         tiles = -(-max_q_len // (2 * per_tile))
         splits, pair = kv8_tc_splits(tiles * num_kv_heads * entries, most, _sms(device), max_q_len <= per_tile)
