@@ -559,7 +559,8 @@ __global__ void __launch_bounds__(K8_THREADS, 1) kv8_attention_tc_kernel(Kv8TcAr
                         *reinterpret_cast<uint2*>(to + QT) = make_uint2(lo[0], lo[1]);
                     }
                 }
-                row_scale = byte != KV8_BAD_BYTE ? kv8_scale(byte) * a.scale_log2e : __int_as_float(0x7fc00000);
+                // (never zero, however small the scale: a score that is not seen is -inf before the product)
+                row_scale = byte != KV8_BAD_BYTE ? fmaxf(kv8_scale(byte) * a.scale_log2e, 1.17549435e-38f) : __int_as_float(0x7fc00000);
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 if (!PAIR || x == 0) mbar_arrive(q_ready + 8 * x);
             }

@@ -195,8 +195,8 @@ def _check_attention(what, q, out, rows, num_heads, num_kv_heads, head_dim, wind
         _refuse(what, "out does not start on a 16-byte boundary")
     if not (0 <= window < 2 ** 31 and 0 <= keep_first < 2 ** 31):
         _refuse(what, f"window {window} and keep_first {keep_first} are not negative, and fit 31 bits")
-    if not scale > 0.0:
-        _refuse(what, f"the scale {scale} is not positive")
+    if not 2.0 ** -126 <= scale <= 2.0 ** 126:
+        _refuse(what, f"the scale {scale} is not positive, or not in [2^-126, 2^126]")
     return strides[0]
 
 

@@ -3,7 +3,7 @@ import pytest
 import torch
 from torch.utils._python_dispatch import TorchDispatchMode
 
-from kv8_util import Case
+from kv8_util import HALF, Case
 
 pytestmark = pytest.mark.gpu
 
@@ -56,3 +56,20 @@ def test_the_largest_windows_hide_nothing(act, hd, window):
         assert torch.equal(c.prefill(), want)
         c.keep = 5
         assert torch.equal(c.prefill(), want)
+
+
+@pytest.mark.parametrize("act", [F32, BF16])
+@pytest.mark.parametrize("hd", [48, 64, 128, 256])
+@pytest.mark.parametrize("scale", [2.0 ** -126, 1e-30, 1e-12])
+def test_scales_next_to_zero_give_means(act, hd, scale):
+    """All visible keys weigh the same, for zeros as for ordinary queries: sums of n <= 90 terms, each rounded once or twice."""
+    for lens_q, lens_kv in (([1, 1], [3, 90]), ([3, 40], [3, 90])):
+        c = Case(lens_q, lens_kv, 4, 2, hd, 16, act, seed=4)
+        c.scale = scale
+        c.q[::2] = 0
+        got = (c.decode() if max(lens_q) == 1 else c.prefill()).double().cpu().view(len(c.req), 4, hd)
+        for t, (r, p) in enumerate(zip(c.req, c.pos)):
+            at = torch.arange(p + 1)
+            v = c.values[c.table[r].long()[at // 16], 1, :, at % 16].repeat_interleave(2, dim=1)      # [keys, heads, hd]
+            bound = HALF[act] * v.mean(0).abs() + (2.0 ** -17 + 2.0 ** -8 * (act == BF16)) * v.abs().mean(0)
+            assert ((got[t] - v.mean(0)).abs() <= bound).all()

@@ -52,3 +52,10 @@ def test_queries_beyond_the_tensor_core_kernels_reach_take_the_other():
     assert kv8_tc_reaches(2048, 6144) and kv8_tc_reaches(15, 2 ** 31 - 8)
     assert not kv8_tc_reaches(17, 2 ** 31 - 8) and not kv8_tc_reaches(2 ** 25, 1024)
     assert kv8_tc_reaches(2 ** 25, 1023) and (2 ** 25 * 1023) >> 3 < 0xffffffff       # (which stands for no row)
+
+
+@pytest.mark.parametrize("name", ["paged_decode_attention_kv8", "paged_prefill_attention_kv8"])
+@pytest.mark.parametrize("scale", [float("inf"), 1e39, 2.0 ** 127, 1e-39, 1e-320, -1.0])
+def test_scales_that_are_no_ordinary_floats_are_refused(name, scale):
+    with pytest.raises(ops.KernelError, match="scale"):
+        getattr(ops, name)(**args(name, scale=scale))
