@@ -143,9 +143,9 @@ class AttentionSpec:
 
     @property
     def eight_bit(self) -> bool:
-        """Whether its keys and values can be kept in 8 bits: the plain attention, which may keep
-        first keys beside its window there."""
-        return replace(self, keep_first=0).plain and self.head_dim % 8 == 0 and self.head_dim <= 256
+        """Whether its keys and values can be kept in 8 bits, as far as its head size can: the plain attention,
+        which may keep first keys beside its window there."""
+        return replace(self, keep_first=0).plain
 
 
 @dataclass(frozen=True)

@@ -68,13 +68,6 @@ struct Kv8DecodeArgs {
 // and mantissa in bfloat16's places (subnormal codes become subnormal numbers).
 __device__ __forceinline__ uint32_t codes_second(uint32_t x) { return (x & 0x80008000u) | ((x >> 4) & 0x07f007f0u); }
 __device__ __forceinline__ uint32_t codes_first(uint32_t x) { return ((x << 8) & 0x80008000u) | ((x << 4) & 0x07f007f0u); }
-__device__ __forceinline__ void mma_bf16_values(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
-                                                uint32_t b0, uint32_t b1) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
 __device__ __forceinline__ void mma_e4m3_16832(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                                uint32_t b0, uint32_t b1) {
     asm volatile(
@@ -106,10 +99,10 @@ __device__ __forceinline__ float ratio(float a, float b) { return a == -INFINITY
 template <int D> __host__ __device__ constexpr int dec8_tile() { return DEC8_KEYS * D; }
 template <int D> __host__ __device__ constexpr int dec8_stage() { return 2 * dec8_tile<D>() + 2 * DEC8_KEYS; }
 template <int D> __host__ __device__ constexpr int dec8_ring() { return DEC8_STAGES * dec8_stage<D>() + DEC8_KEYS * 8; }
-// Of a block: the warps' statistics, the blocks' statistics [16][H][4], and a place for the parts of all blocks of what
+// Of a block: the warps' statistics, the blocks' statistics [8][8][4], and a place for the parts of all blocks of what
 // this block joins, [C][H][D / C].
 template <int D, int H> __host__ __device__ constexpr int dec8_smem(int warps, int blocks) {
-    return warps * dec8_ring<D>() + (warps * 32 + (blocks > 1 ? 16 * 32 + H * D : 0)) * 4;
+    return warps * dec8_ring<D>() + (warps * 32 + (blocks > 1 ? 8 * 32 + H * D : 0)) * 4;
 }
 template <int D> __host__ __device__ constexpr int dec8_most_warps() { return D == 64 ? 16 : D == 128 ? 8 : 4; }
 
@@ -429,14 +422,14 @@ kv8_decode_kernel(Kv8DecodeArgs a) {
                 // features 4j, 4j + 1 and 4j + 2, 4j + 3 of this thread's run, of one key and of the other
                 const uint32_t a01 = __byte_perm(v[0][j], v[1][j], 0x5410), a23 = __byte_perm(v[0][j], v[1][j], 0x7632);
                 const uint32_t b01 = __byte_perm(v[2][j], v[3][j], 0x5410), b23 = __byte_perm(v[2][j], v[3][j], 0x7632);
-                const uint32_t a0 = codes_first(a01), a1 = codes_second(a01), a2 = codes_first(b01), a3 = codes_second(b01);
-                const uint32_t a4 = codes_first(a23), a5 = codes_second(a23), a6 = codes_first(b23), a7 = codes_second(b23);
+                const uint32_t lo[4] = {codes_first(a01), codes_second(a01), codes_first(b01), codes_second(b01)};
+                const uint32_t hi[4] = {codes_first(a23), codes_second(a23), codes_first(b23), codes_second(b23)};
                 if constexpr (H == 8) {
-                    mma_bf16_values(o[2 * j], a0, a1, a2, a3, pl[u][0], pl[u][1]);
-                    mma_bf16_values(o[2 * j + 1], a4, a5, a6, a7, pl[u][0], pl[u][1]);
+                    mma_bf16_16816(o[2 * j], lo, pl[u][0], pl[u][1]);
+                    mma_bf16_16816(o[2 * j + 1], hi, pl[u][0], pl[u][1]);
                 }
-                mma_bf16_values(o[2 * j], a0, a1, a2, a3, pf[u][0], pf[u][1]);
-                mma_bf16_values(o[2 * j + 1], a4, a5, a6, a7, pf[u][0], pf[u][1]);
+                mma_bf16_16816(o[2 * j], lo, pf[u][0], pf[u][1]);
+                mma_bf16_16816(o[2 * j + 1], hi, pf[u][0], pf[u][1]);
             }
         }
         // ---- the tile S turns ahead takes this one's place
@@ -466,7 +459,7 @@ kv8_decode_kernel(Kv8DecodeArgs a) {
     float* o_s = reinterpret_cast<float*>(smem8);         // [W][H][LD]
     float4* st_s = reinterpret_cast<float4*>(smem8 + (size_t)W * dec8_ring<D>());     // [W][8]
     float4* all_st = st_s + W * 8;                        // [C][8]: of the blocks
-    float* all_o = reinterpret_cast<float*>(all_st + 16 * 8);
+    float* all_o = reinterpret_cast<float*>(all_st + 8 * 8);
     if (g == 0 && 2 * t < H) {
         st_s[warp * 8 + 2 * t] = make_float4(m0, w0, l0, 0.f);
         st_s[warp * 8 + 2 * t + 1] = make_float4(m1, w1, l1, 0.f);
@@ -566,7 +559,6 @@ static int launch_decode(const Kv8DecodeArgs& a, int tokens, int blocks, int war
     if (dev < 0 || dev >= 64) return -1;
     if (!configured[dev]) {
         e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
-        if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
         // several blocks an SM need nearly all of its shared memory
         if (e == cudaSuccess)
             e = cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, (int)cudaSharedmemCarveoutMaxShared);
@@ -596,8 +588,8 @@ static int launch_decode(const Kv8DecodeArgs& a, int tokens, int blocks, int war
     return e != cudaSuccess ? (int)e : launch_status();
 }
 
-// Token i is row i of q (rows q_stride apart, 16-byte aligned), out, token_req and cache_pos.  `blocks` blocks (1, 2, 4,
-// 8 or 16, a cluster) of `warps` warps share the keys of a (token, kv head, 8 query heads, or up to 4 where a kv head has
+// Token i is row i of q (rows q_stride apart, 16-byte aligned), out, token_req and cache_pos.  `blocks` blocks (1, 2, 4
+// or 8, a cluster) of `warps` warps share the keys of a (token, kv head, 8 query heads, or up to 4 where a kv head has
 // no more).  page_size: a multiple of 8.  Returns 0, a CUDA error code or -1 (shape refused).
 MSTAR_API int mstar_kv8_decode(const void* q, int q_stride, void* out, const void* codes, const void* scales, int pages,
                                const int* block_table, int bt_stride, int bt_width, const int* token_req, const int* cache_pos,
@@ -606,7 +598,7 @@ MSTAR_API int mstar_kv8_decode(const void* q, int q_stride, void* out, const voi
     if (tokens <= 0) return 0;
     if (nkv <= 0 || nq % nkv != 0 || page_size <= 0 || page_size % 8 != 0 || pages <= 0 || bt_width <= 0 ||
         tokens > 65535 || blocks < 1 ||
-        blocks > 16 || (blocks & (blocks - 1)) != 0 || ((uintptr_t)q & 15) != 0 || q_stride % 8 != 0 ||
+        blocks > 8 || (blocks & (blocks - 1)) != 0 || ((uintptr_t)q & 15) != 0 || q_stride % 8 != 0 ||
         ((uintptr_t)codes & 15) != 0 || ((uintptr_t)scales & 7) != 0 || ((uintptr_t)out & 7) != 0 ||
         (long long)pages * 2 * nkv * page_size > 0xffffffffll || (hd != 64 && hd != 128 && hd != 256))
         return -1;

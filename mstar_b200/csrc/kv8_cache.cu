@@ -252,14 +252,14 @@ static int launch_write(const void* qkv, void* q_out, const Kv8WriteArgs& a, int
     return e != cudaSuccess ? (int)e : launch_status();
 }
 
-// qkv: `tokens` rows of (nq + 2 nkv) * hd elements, `in_stride` apart.  nkv 0: queries only.  hd a multiple of 8, at
-// most 256; rot even, at most hd.  Returns 0, a CUDA error code or -1 (shape refused).
+// qkv: `tokens` rows of (nq + 2 nkv) * hd elements, `in_stride` apart.  hd a multiple of 8, at most 256; rot even, at most
+// hd.  Returns 0, a CUDA error code or -1 (shape refused).
 MSTAR_API int mstar_rope_kv8_write(const void* qkv, int act_dtype, int in_stride, void* q_out, const int* positions,
                                    const int* cache_pos, const int* token_req, const int* block_table, int bt_stride,
                                    int bt_width, const float* inv_freq, void* codes, void* scales, int pages, int tokens, int nq,
                                    int nkv, int hd, int rot, int interleaved, int page_size, void* stream) {
     if (tokens <= 0) return 0;
-    if (hd <= 0 || hd % 8 != 0 || hd > 256 || rot < 0 || rot % 2 != 0 || rot > hd || nq < 0 || nkv < 0 || page_size <= 0 ||
+    if (hd <= 0 || hd % 8 != 0 || hd > 256 || rot < 0 || rot % 2 != 0 || rot > hd || nq <= 0 || nkv <= 0 || page_size <= 0 ||
         pages <= 0 || ((uintptr_t)codes & 7) != 0)
         return -1;
     const Kv8WriteArgs a{positions, cache_pos, token_req, block_table, inv_freq, (uint8_t*)codes, (uint8_t*)scales, nq,

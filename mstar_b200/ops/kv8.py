@@ -68,7 +68,7 @@ def _check_cache(what, kv_cache, kv_scales, num_kv_heads, page_size, head_dim) -
         _refuse(what, f"the scales' shape {tuple(kv_scales.shape)} is not the cache's {tuple(shape[:4])}")
     if not (kv_cache.is_contiguous() and kv_scales.is_contiguous()):
         _refuse(what, "the cache and its scales must be contiguous")
-    if head_dim % 8 or not 0 < head_dim <= 256:
+    if not kv8_supported(head_dim):
         _refuse(what, f"head_dim {head_dim} is not a multiple of 8 up to 256")
     return pages
 

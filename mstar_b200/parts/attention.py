@@ -88,7 +88,8 @@ class Attention:
                                    window=spec.chunk or spec.window, keep_first=spec.keep_first if spec.window
                                    else 0,
                                    v_head_dim=None if spec.value_dim == spec.head_dim
-                                   else spec.value_dim, eight_bit=spec.eight_bit), state=state)
+                                   else spec.value_dim,
+                                   eight_bit=spec.eight_bit and ops.kv8_supported(spec.head_dim)), state=state)
 
     def __init__(self, spec, params: dict, runtime: Runtime):
         if spec.num_heads % spec.num_kv_heads:

@@ -59,3 +59,16 @@ def test_queries_beyond_the_tensor_core_kernels_reach_take_the_other():
 def test_scales_that_are_no_ordinary_floats_are_refused(name, scale):
     with pytest.raises(ops.KernelError, match="scale"):
         getattr(ops, name)(**args(name, scale=scale))
+
+
+def test_a_layer_says_whether_its_head_size_can_be_held():
+    import dataclasses
+
+    from mstar_b200.config.layout import PositionSpec
+    from mstar_b200.parts.attention import Attention
+    from test_kv8 import PLAIN
+
+    for hd, able in ((64, True), (8, True), (256, True), (20, False), (264, False)):
+        spec = dataclasses.replace(PLAIN, head_dim=hd, position=PositionSpec(head_dim=hd, rotary_dim=4))
+        assert Attention.cache_need(spec).kv.eight_bit is able
+    assert not Attention.cache_need(dataclasses.replace(PLAIN, softcap=30.0)).kv.eight_bit
