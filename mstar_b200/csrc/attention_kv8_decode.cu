@@ -567,9 +567,12 @@ static int launch_decode(const Kv8DecodeArgs& a, int tokens, int blocks, int war
     }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(blocks * a.nkv * a.head_groups, tokens);
-    // No more blocks an SM than an even share: with room for more, some SMs take them and others none (256 blocks of four
-    // warps: 10.6 us, 9.1 so).  Clusters do not fill a group of SMs to the last place: the larger, the more is left free.
-    const long long all = (long long)cfg.gridDim.x * tokens * (blocks >= 8 ? 13 : blocks == 4 ? 11 : 10) / 10;
+    // No more blocks an SM than an even share, by asking for so much shared memory that one more does not fit (an SM has 228
+    // KB, of which a block takes 1 KB besides; 128 bytes to spare): with room for more, some SMs take them and others none
+    // (heads of 64, 2,048 keys, 32, 96, 192 pairs: 5.8, 9.5, 16.3 us so, 6.8, 10.7, 17.5 without).  Clusters of eight do not
+    // fill the groups of SMs that they have to lie in, so that their share is counted over ten thirteenths of the SMs
+    // (16 pairs of heads of 64 and of 128: 5.9 and 7.9 us so, 9.1 and 13.3 over all).
+    const long long all = (long long)cfg.gridDim.x * tokens * (blocks >= 8 ? 13 : 10) / 10;
     const long long share = (all + device_sm_count() - 1) / device_sm_count();
     smem = max(smem, (int)min(227ll * 1024, 228 * 1024 / (share + 1) - 896));
     cfg.blockDim = dim3(32 * warps);

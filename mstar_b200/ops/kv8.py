@@ -257,14 +257,16 @@ KV8_DECODE_HEAD_DIMS = (64, 128, 256)
 @functools.lru_cache(maxsize=4096)
 def kv8_decode_shape(pairs: int, max_keys: int, head_dim: int, few: bool, sms: int) -> tuple:
     """(blocks of a cluster, warps of a block) that share the keys of each of ``pairs`` (token, kv head, 8
-    query heads; ``few``: 4) in the decode kernel.  All blocks run at once (larger clusters leave SMs
-    free), with the smallest share of a pair's keys on the SM that has most; among those clusters of two
-    at most where that does, and then as many warps as fit.  Where no shape runs at once: single blocks of
-    four.  (2,048 keys, 24 shapes each.  Heads of 128, 3 a kv head: 8, 24, 64, 128, 256, 400, 512 pairs take 5.9 us
-    with 8 x 8, 7.3 with 4 x 8, 11.5 with 2 x 8, 19.1 with 2 x 6, 28.8 with 1 x 6, 40.2 with 1 x 4, 51.1 with 1 x 3;
-    the best of all shapes is within 0.1 but for 17.9 (1 x 8) at 128.  8 a kv head, heads of 64: within 0.2, but for
-    62.4 (1 x 2) against 64.8 at 512 pairs and 7.6 (4 x 4) against 8.1 at 64 of 64.  Heads of 256: within 0.1 while all
-    blocks run at once; 256, 400, 512 pairs take 70.5, 104.8, 137.3 with 1 x 4 where 1 x 3 or 1 x 2 take 61.3, 90.5, 117.1.)"""
+    query heads; ``few``: 4) in the decode kernel.  All blocks run at once (larger clusters leave SMs free: 5 % of
+    them for every block of a cluster beyond two where an SM has one; 16 pairs of heads of 128 and of 256 take 7.9
+    and 12.9 us so, 11.1 and 17.6 without), with the smallest share of a pair's keys on the SM that has most; among
+    those clusters of two at most where that does, and then as many warps as fit.  Where no shape runs at once:
+    single blocks of four.  (2,048 keys, 24 shapes each.  Heads of 128, 3 a kv head: 8, 24, 64, 128, 256, 400, 512
+    pairs take 5.9 us with 8 x 8, 7.3 with 4 x 8, 11.5 with 2 x 8, 19.1 with 2 x 6, 28.8 with 1 x 6, 40.2 with 1 x 4,
+    51.1 with 1 x 3; the best of all shapes is within 0.1 but for 17.9 (1 x 8) at 128.  8 a kv head, and heads of 64:
+    within 0.2, but for 62.4 (1 x 2) against 64.8 at 512 pairs of 128 and 7.6 (4 x 4) against 8.1 at 64 of 64.  Heads
+    of 256: within 0.1 while all blocks run at once; 256, 400, 512 pairs take 70.5, 104.8, 137.3 with 1 x 4 where 1 x 3
+    or 1 x 2 take 61.3, 90.5, 117.1.)"""
     heads = 4 if few else 8
     # a warp's two tiles of 32 keys and values with their scales; warps that the registers allow an SM
     ring, most = 2 * 64 * (head_dim + 1) + 256, 16 if head_dim == 64 else 12 if few and head_dim == 128 else 8
