@@ -6,8 +6,8 @@
 // angles, whose latency they share.  The rotated queries go to a tensor of their own, so that the projection's output stays
 // as it was and the attention after it reads rows without gaps.
 //
-// Angles: position * frequency is exact in double (24 + 24 bits), is taken to half-turns and brought into [-1, 1]
-// there, so that far positions lose nothing (in float, position 100,000 would be off by 0.004).  A key next to the border of
+// Angles: position * frequency is exact in double (24 + 24 bits), is taken to half-turns (off by less than 2^-52 of the angle)
+// and brought into [-1, 1] there (in float, position 100,000 would be off by 0.004; here by 2^-35).  A key next to the border of
 // two codes that came out on the wrong side would be off by a whole code, 1/16 of its value (with a rotation in float one
 // number in some 10^6), so sines and cosines are double, and the rotation is too in the 32-bit mode.  In the 16-bit mode it
 // is done in pairs of floats: c = c_hi + c_lo with 16 bits in c_hi, so that its product with a bfloat16 is exact, the two

@@ -73,3 +73,45 @@ def test_scales_next_to_zero_give_means(act, hd, scale):
             v = c.values[c.table[r].long()[at // 16], 1, :, at % 16].repeat_interleave(2, dim=1)      # [keys, heads, hd]
             bound = HALF[act] * v.mean(0).abs() + (2.0 ** -17 + 2.0 ** -8 * (act == BF16)) * v.abs().mean(0)
             assert ((got[t] - v.mean(0)).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("act", [F32, BF16])
+@pytest.mark.parametrize("nkv,hd,rot,inter", [(4, 128, 64, False), (4, 128, 32, True), (8, 64, 16, False), (3, 24, 12, False),
+                                              (2, 200, 72, False), (2, 48, 48, True), (2, 48, 40, False), (2, 256, 128, False),
+                                              (5, 8, 2, True)])
+@pytest.mark.parametrize("shift", [0, 1])
+def test_partly_rotated_and_odd_keys_get_their_nearest_codes(act, nkv, hd, rot, inter, shift):
+    """A million numbers each, on the path of whole runs and on the scalar one (odd sizes, rows off 16 bytes): the rotation is
+    off by half a step of a float (2^-24) and 2^-38 of its two products, and the angle by less than 2^-52 of itself, so that what is held is off by half a code's
+    step of the exact result and by that much.  Numbers that are not turned have their nearest codes."""
+    from mstar_b200 import ops
+
+    T, page = max(1024, 2 ** 20 // (nkv * hd)), 16
+    g = torch.Generator(device=DEV).manual_seed(hd + rot)
+    width = (1 + 2 * nkv) * hd
+    wide = torch.randn(T, width + 8, generator=g, device=DEV).to(act)
+    qkv = wide[:, shift:shift + width]
+    freq = torch.tensor([10000.0 ** (-2.0 * j / rot) for j in range(rot // 2)], dtype=F32, device=DEV)
+    pos, at, req = i32(range(70_000, 70_000 + T)), i32(range(T)), i32([0] * T)
+    pages = -(-T // page)
+    codes = torch.zeros(pages, 2, nkv, page, hd, dtype=torch.uint8, device=DEV).view(torch.float8_e4m3fn)
+    scales = torch.zeros(pages, 2, nkv, page, dtype=torch.uint8, device=DEV)
+    table = i32([list(range(pages))])
+    q = ops.rope_kv8_write(qkv, pos, at, req, table, freq, codes, scales, 1, nkv, hd, rot, inter, page)
+    got = ops.kv8_read_rows(codes, scales, table, req, at, F32)[:, 0].double()
+    x = qkv[:, :(1 + nkv) * hd].double().view(T, 1 + nkv, hd)
+    angle = (pos.double()[:, None] * freq.double())[:, None]
+    lo, hi = (slice(0, rot, 2), slice(1, rot, 2)) if inter else (slice(0, rot // 2), slice(rot // 2, rot))
+    want, size = x.clone(), torch.zeros_like(x)
+    want[..., lo] = x[..., lo] * angle.cos() - x[..., hi] * angle.sin()
+    want[..., hi] = x[..., hi] * angle.cos() + x[..., lo] * angle.sin()
+    size[..., lo] = size[..., hi] = x[..., lo].abs() + x[..., hi].abs()
+    # (the angle, exact in double, becomes half-turns by a product with 1 / pi in double: the constant is off by 2^-54 of
+    # itself and the product by 2^-53, together less than angle * 2^-52, which at 73,000 is 2^-35.8 of the two products)
+    near = 2.0 ** -24 * want.abs() * (size > 0) + (2.0 ** -38 + 75_000 * 2.0 ** -52) * size
+    err = (q.double() - want[:, 0]).abs()
+    assert (err <= HALF[act] * want[:, 0].abs() + near[:, 0]).all()
+    unit = torch.exp2(scales[:, 0].permute(0, 2, 1).reshape(-1, nkv, 1)[:T].double() - 127.0)
+    want, near = want[:, 1:], near[:, 1:]
+    step = unit * torch.exp2((want.abs() / unit).clamp(min=2.0 ** -6).log2().floor() - 3)
+    assert ((got - want).abs() - step / 2 <= near).all()
