@@ -246,6 +246,11 @@ template <typename A, int R> static int launch_simt(const Kv8AttnArgs& a, dim3 g
 // (Weights in float16 relative to the largest 2^(s_j + e_j), with the values' exponents in them, took a product less, but what
 // lay 2^25 below the largest was lost in every feature.  Times so: 15.8, 327, 103, 18.4 us for the four calls below.)
 //
+// The tensor cores cut the sums that they add to instead of rounding them: over 6,500 keys that was 1.2e-5 of the output, all
+// one way.  So in the 32-bit mode a tile's products are summed from zero and added in float arithmetic (9.5e-7; 359 us for
+// the two portions of 512 tokens below instead of 350), over 4 or 8 blocks of 8 features at a time, as the registers allow
+// (4 of heads of 64: 435 us; 8 of heads of 256, 100 tokens on 2,000: 79.5 instead of 72.9; 8 with few rows: 24.3, not 23.4).
+//
 // A warp owns 16 rows (token, query head of the group) and, of every tile of 64 keys, 8 NT: with NT 8 a block's four
 // warps have 64 rows, with NT 2 (16 rows or fewer) they share a tile's keys and leave a part each.  Tiles of codes come by
 // cp.async, one tile ahead (three with few rows), into swizzled shared memory.  Which features and keys the elements of the
@@ -253,9 +258,9 @@ template <typename A, int R> static int launch_simt(const Kv8AttnArgs& a, dim3 g
 // tile are converted once, each warp a quarter of the keys (with NT 2 its own), into a bfloat16 tile.
 //
 // Bound by instructions and the tensor pipe.  In the 32-bit mode two portions of 251 tokens, 32 heads of 64 over 8, a window of
-// 200, take 16.0 us (on CUDA cores 108), two of 512 on 6,000 cached 350 (115 TFLOP/s; five products for two), in the 16-bit
+// 200, take 15.8 us (on CUDA cores 108), two of 512 on 6,000 cached 359 (112 TFLOP/s; five products for two), in the 16-bit
 // mode 512 tokens of 12 heads of 256 over 4 on 2,000 cached 141; float single tokens of 8 requests on 800 to 2,048 keys, 24
-// heads of 128 over 8, 22 us.
+// heads of 128 over 8, 23 us.
 __device__ __forceinline__ uint32_t f16x2_of_codes(uint32_t two) {
     uint32_t r;
     asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t}" : "=r"(r) : "r"(two));
@@ -297,6 +302,7 @@ template <typename A, int HD, int PARTS, int NT>
 __global__ void __launch_bounds__(128) kv8_attention_mma_kernel(Kv8AttnArgs a) {
     constexpr int ROWS = NT == 8 ? 64 : 16, RB = HD < 128 ? HD : 128, KC = HD / 64, MT = HD / 8;
     constexpr int PP = PARTS + 1;                        // parts of a weight
+    constexpr int KB = NT == 8 && HD < 256 ? 8 : 4;      // blocks of 8 features that are summed side by side
     constexpr int NB = NT < 4 ? NT : 4;                  // products side by side
     constexpr int QP = HD * 2 + 16;                      // bytes of a row of queries in shared memory
     constexpr int S = km_stages<NT>();
@@ -577,10 +583,10 @@ __global__ void __launch_bounds__(128) kv8_attention_mma_kernel(Kv8AttnArgs a) {
         // the values are there: of all warps, or of this one
         if constexpr (NT == 8) __syncthreads();
         else __syncwarp();
-        // ---- outputs, 16 keys at a time
+        // ---- outputs.  In the 32-bit mode the tile's products are summed by themselves and then added, which rounds
+        uint32_t pf[NT / 2][PP][4];
 #pragma unroll
-        for (int u = 0; u < NT / 2; ++u) {
-            uint32_t pf[PP][4];
+        for (int u = 0; u < NT / 2; ++u)
 #pragma unroll
             for (int x = 0; x < 2; ++x)
 #pragma unroll
@@ -591,23 +597,34 @@ __global__ void __launch_bounds__(128) kv8_attention_mma_kernel(Kv8AttnArgs a) {
 #pragma unroll
                     for (int p = 0; p < PP; ++p) {       // what the parts before leave, rounded
                         const uint32_t b = pack_bf16(p0, p1);
-                        pf[p][2 * x + h] = b;
+                        pf[u][p][2 * x + h] = b;
                         p0 -= __uint_as_float(b << 16);
                         p1 -= __uint_as_float(b & 0xffff0000u);
                     }
                 }
-            const int r = (n0 + 2 * u) * 8 + vr;
-            const uint32_t v_at = smem_u32(b_s) + r * (HD * 2);
 #pragma unroll
-            for (int k = 0; k < MT; k += 2) {            // blocks k and k + 1 of 8 features
-                uint32_t v[4];
-                ldmatrix_x4_trans(v, v_at + (((k + vc) ^ (r & 7)) << 4));
+        for (int k = 0; k < MT; k += KB) {               // KB blocks of 8 features
+            float sum[KB][4];
 #pragma unroll
-                for (int p = PP - 1; p >= 0; --p) {      // (the small parts first)
-                    mma_bf16_16816(o[k], pf[p], v[0], v[1]);
-                    mma_bf16_16816(o[k + 1], pf[p], v[2], v[3]);
-                }
+            for (int i = 0; i < KB; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sum[i][e] = PARTS == 2 ? 0.f : o[k + i][e];
+#pragma unroll
+            for (int u = 0; u < NT / 2; ++u) {
+                const int r = (n0 + 2 * u) * 8 + vr;
+                uint32_t v[KB / 2][4];
+#pragma unroll
+                for (int i = 0; i < KB / 2; ++i)
+                    ldmatrix_x4_trans(v[i], smem_u32(b_s) + r * (HD * 2) + (((k + 2 * i + vc) ^ (r & 7)) << 4));
+#pragma unroll
+                for (int p = PP - 1; p >= 0; --p)        // (the small parts first)
+#pragma unroll
+                    for (int i = 0; i < KB; ++i) mma_bf16_16816(sum[i], pf[u][p], v[i / 2][2 * (i & 1)], v[i / 2][2 * (i & 1) + 1]);
             }
+#pragma unroll
+            for (int i = 0; i < KB; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[k + i][e] = PARTS == 2 ? o[k + i][e] + sum[i][e] : sum[i][e];
         }
     }
     cp_async_wait<0>();

@@ -41,7 +41,7 @@ def case_of(rows, q, lens_q, lens_kv, nq, nkv, hd, page, act, window=0, keep=0):
     return c
 
 
-def exact(c, w, rounded=lambda p: p):
+def exact(c, w, rounded=lambda p: p, sums=None):
     """(the output, the bound below which a kernel's output stays), [tokens, heads * dim] in float64 on the GPU.
 
     The bound, elementwise, with h half a step of the output's type, A = sum of weight * |value| and u = 2^-23 (tensor cores
@@ -49,7 +49,7 @@ def exact(c, w, rounded=lambda p: p):
     float16 parts (nothing more where it is a bfloat16 in two codes: 2^-17.8 of the row's largest number there, below) and
     by (D / 8 + 10) u S for the float sums of tiles of 16 features, its scaling and its difference to the maximum, in
     numerator and denominator; an exponential by 2^-21; a weight by ``w``; sums over n keys in steps of 16 and of
-    three parts by (3 n / 16 + 24) u.  Nothing is allowed in absolute terms: a key counts for what it weighs in every feature."""
+    three parts by (3 n / 16 + 24) u, or ``sums``.  Nothing is allowed in absolute terms: a key counts for what it weighs in every feature."""
     T, G, hd = len(c.req), c.nq // c.nkv, c.hd
     values = values_of(c.codes, c.scales).to(DEV)
     q = c.q.double().view(T, c.nq, hd).to(DEV)
@@ -64,7 +64,7 @@ def exact(c, w, rounded=lambda p: p):
             out[t, i] = rounded(p) @ v
             spread = float((k.abs() @ q[t, i].abs()).max()) * c.scale
             codes = 2.0 ** -17.8 * float(q[t, i].abs().max() * k.abs().sum(-1).max()) * c.scale if c.act == BF16 else 0.0
-            rel = 2 * ((2.0 ** -22 + (hd / 8 + 10) * u) * spread + codes + 2.0 ** -21) + w + (3 * len(at) / 16 + 24) * u
+            rel = 2 * ((2.0 ** -22 + (hd / 8 + 10) * u) * spread + codes + 2.0 ** -21) + w + ((3 * len(at) / 16 + 24) * u if sums is None else sums)
             bound[t, i] = HALF[c.act] * out[t, i].abs() + rel * (p @ v.abs())
     return out.view(T, -1), 1.02 * bound.view(T, -1)
 
@@ -165,3 +165,22 @@ def test_the_32_bit_mode_keeps_its_bits(hd):
         assert ((got.double() - want).abs() <= bound).all()
         rounded, _ = exact(c, 0.0, lambda p: p.half().double())
         assert float(((rounded - want).abs() / bound).max()) > 2.0
+
+
+@pytest.mark.parametrize("nq,nkv,hd", [(4, 2, 64), (4, 2, 128), (2, 1, 256)])
+@pytest.mark.parametrize("new", [1, 3, 40])
+def test_long_sums_of_the_32_bit_mode_do_not_drift(nq, nkv, hd, new):
+    """30,000 keys in one part, or one a warp, whose values have one sign: sums that are cut instead of rounded lose half a
+    step of a float at every product of 16 keys, 7e-5 in all.  Allowed are a tile's sum of 12 products, cut (12 u), a rounded
+    sum for every tile of 64 keys (of 16 with few rows, but a warp has a quarter of the keys then) of the outputs and of the
+    normaliser (n / 64 halves of u each), and 16 u for a row's sum of a tile's weights and the joining of parts."""
+    n, u = 30_000, 2.0 ** -23
+    g = torch.Generator().manual_seed(17)
+    rows = torch.randn(n, 2, nkv, hd, generator=g).double()
+    rows[:, 1] = 1.0 + 0.1 * rows[:, 1]
+    q = 0.02 * torch.randn(new, nq * hd, generator=g)
+    c = case_of([rows], q, [new], [n], nq, nkv, hd, 16, F32)
+    want, bound = exact(c, 2.0 ** -24, sums=(n / 64 + 12 + 16) * u)
+    got = c.decode(max_len=1) if new == 1 else c.prefill(max_len=1)
+    assert float((bound / want.abs()).max()) < 1e-4
+    assert float(((got.double() - want).abs() / bound).max()) <= 1.0
