@@ -58,8 +58,8 @@ class LLM:
         number for all groups or a list with one per group; ``max_num_pages`` None sizes the
         pools from ``kv_cache_memory_fraction`` of the memory free after loading.
         ``kv_cache_dtype``: None or "auto" keeps keys and values in the compute type, "float8_e4m3"
-        in 8 bits a number with a scale a row: half the bytes of bfloat16, for models whose layers
-        all have the plain attention."""
+        in 8 bits a number with a scale a row (4 significant bits): half the bytes of bfloat16, for models
+        whose layers all have the plain attention.  In the 32-bit mode queries count with 22 bits then."""
         self.model: Model = model if isinstance(model, Model) else load_model(
             model, dtype=dtype, device=device)
         self.device = self.model.runtime.device
